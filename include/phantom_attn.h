@@ -33,7 +33,13 @@
 extern "C" {
 #endif
 
-enum pa_dtype { PA_DTYPE_F32 = 0, PA_DTYPE_F16 = 1, PA_DTYPE_BF16 = 2 };
+enum pa_dtype {
+  PA_DTYPE_F32 = 0,
+  PA_DTYPE_F16 = 1,
+  PA_DTYPE_BF16 = 2,
+  PA_DTYPE_I8 = 3,   /* these two: paged caches only */
+  PA_DTYPE_E4M3 = 4  /* the OCP format: 4 exponent bits, 3 mantissa bits, largest value 448 */
+};
 
 enum pa_status {
   PA_OK = 0,
@@ -132,6 +138,64 @@ int64_t pa_fused_tc_lds_bytes(int64_t d, int dtype);
 /* LDS bytes one workgroup may use on `device`, written to *bytes.
  * Replaces smem_optin_bytes (csrc/common.cuh:35-40). */
 int pa_device_lds_limit(int device, int64_t* bytes);
+
+/* ---- Paged key/value cache: rows of earlier tokens kept in pages, and attention over them ----
+ *
+ * A cache is two arrays [pages][heads][page_size][d], one for keys and one for values. Position p of
+ * sequence s is row p % page_size of page page_table[s * table_stride + p / page_size]; a table entry
+ * outside [0, pages) is an absent page (not written, read as zeros, its keys not attended).
+ * lengths[s] is the number of tokens sequence s holds once the call's new tokens are in the cache: its
+ * new token i (of `count`) is at position lengths[s] - count + i. The new tokens of all sequences are
+ * packed one after another, [tokens][heads][d] with the strides given (in elements, multiples of 8, the
+ * d elements of a row contiguous); those of sequence s are the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1,
+ * or, with cu_seqlens NULL, tokens / seqs rows each. page_table, lengths and cu_seqlens are int32 on the
+ * device and read by the kernels. Whatever they hold, no access leaves the tensors: rows without a
+ * position in the table are not written and see no key; offsets are clamped to [0, tokens], and a row that
+ * offsets out of order give to two sequences may hold either's result.
+ *
+ * dtype is the tensors' (F16 or BF16); the cache's own is the same, or I8 or E4M3 with an fp32 scale for
+ * each row in k_scale / v_scale [pages][heads][page_size]: a row stands for code * scale.
+ * d in {64, 128}. All pointers to rows 16-byte aligned. */
+typedef struct pa_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* 8-bit caches only */
+  float* v_scale;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  int64_t pages, page_size, heads, d;
+  int64_t seqs, table_cols, table_stride;
+  int dtype;
+} pa_paged_cache;
+
+/* Writes the new tokens' keys and values to their positions. 8-bit caches: scale = amax / L and
+ * code = round(x * (L / amax)) to nearest even in fp32, L = 127 (int8) or 448 (e4m3), amax the row's
+ * largest magnitude; a row below 2^-100 is held as zeros, one with an element that is not finite gets a
+ * NaN scale. The positions written in one call must be distinct: of two rows for one position either, or
+ * parts of both, may remain. */
+int pa_cache_write(const pa_paged_cache* cache, const void* k, const void* v, int dtype, int64_t tokens,
+                   int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                   const int32_t* cu_seqlens, void* stream);
+
+/* Lays the first n positions of every sequence out as [seqs][heads][n][d] (the other entry points'
+ * layout) in dtype, code * scale rounded once; zeros from lengths[s] on. */
+int pa_cache_read(const pa_paged_cache* cache, void* k, void* v, int dtype, int64_t n, void* stream);
+
+/* Attention of the new tokens over the cache (which holds them already): new token i of sequence s sees
+ * the positions up to its own (causal != 0) or all lengths[s] of them, scores scaled by 1/sqrt(d); a
+ * token that sees nothing gets zeros. q and o are [tokens][heads_q][d] with the strides given, heads_q a
+ * multiple of the cache's heads (query head h reads head h / (heads_q / heads)); o must not overlap q.
+ * Rows behind the last sequence's are left as they are. max_new: an upper bound of the new tokens of a
+ * sequence, 0 if unknown; only the choice of the kernel depends on it. workspace:
+ * pa_paged_attn_workspace() bytes of device memory, 16-byte aligned, used until the call's kernels end
+ * (NULL if that is 0); calls that may overlap need one each. */
+int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int dtype, int64_t tokens, int64_t heads_q,
+                      int64_t q_token_stride, int64_t q_head_stride, int64_t o_token_stride, int64_t o_head_stride,
+                      const int32_t* cu_seqlens, int64_t max_new, int causal, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* Bytes of workspace that pa_paged_attn_fwd needs for a call of these sizes on the current device. */
+int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q, int64_t max_new);
 
 /* Message for the last nonzero status returned on this thread ("" if none). */
 const char* pa_last_error(void);

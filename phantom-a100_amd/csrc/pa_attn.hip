@@ -22,6 +22,7 @@
 #include "kernels/fa_f32.hpp"
 #include "kernels/fa_f32x3.hpp"
 #include "kernels/fa_mfma.hpp"
+#include "host_common.hpp"
 #include "kernels/unfused.hpp"
 #include "launch_model.hpp"
 
@@ -31,20 +32,9 @@
 
 namespace {
 
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-int hip_status(hipError_t e, const char* name) {
-  if (e == hipSuccess) return PA_OK;
-  return fail((int)e, "%s: HIP error: %s", name, hipGetErrorString(e));
-}
+using pa::device_cus;
+using pa::fail;
+using pa::hip_status;
 
 size_t dtype_bytes(int dt) { return dt == PA_DTYPE_F32 ? 4 : 2; }
 
@@ -75,19 +65,6 @@ int check_aligned16(const char* name, const void* q, const void* k, const void* 
 float scale_log2_for(int64_t d) { return pa::kLog2e / sqrtf((float)d); }
 
 // ------------------------------------------------------------------ fused MFMA (fp16 / bf16)
-// Compute units of the current device (looked up once per device), 0 if unknown.
-int device_cus() {
-  static std::atomic<int> cus[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 0;
-  int n = cus[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
-    cus[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 // The persistent d = 128 launch is on unless the environment sets PA_PERSISTENT=0 when the library
 // is loaded; pa_set_persistent() switches it afterwards (a process-wide flag, read once per launch).
 int persistent_from_env() {
@@ -674,7 +651,7 @@ int pa_device_lds_limit(int device, int64_t* bytes) {
   return PA_OK;
 }
 
-const char* pa_last_error(void) { return g_err; }
+const char* pa_last_error(void) { return pa::g_err; }
 
 const char* pa_version(void) { return "phantom_attn " PA_VERSION_STRING " (gfx950)"; }
 

@@ -14,6 +14,9 @@ through its C ABI (include/phantom_attn.h); there is no CPU or PyTorch fallback.
     fused_tuned  fp16 MFMA fused kernel at a chosen (br, bc) tile and 1 or 2 LDS stages
     fused_tc     fp16/bf16 MFMA fused kernel                          d=64 or 128
 
+For serving (paged.py): cache_write and cache_read, a paged key/value cache in 16 or 8 bits, and paged_attn,
+the attention of new tokens over it, d=64 or 128, fp16/bf16, query heads in groups per key/value head.
+
 Extensions over the reference: fused_tc accepts bfloat16 and d=128; the fused entry points take
 `out_dtype=torch.float32` to return fp32 output from fp16/bf16 inputs.
 """
@@ -199,6 +202,10 @@ def reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
         return torch.nn.functional.scaled_dot_product_attention(
             q.float(), k.float(), v.float(), is_causal=causal)
 
+
+# The paged key/value cache and attention over it (serving): paged.py. Imported here, after the call helpers
+# that it shares.
+from .paged import cache_read, cache_write, paged_attn  # noqa: E402, F401
 
 # Every version, in the order the project builds them.
 KERNELS = {"naive": naive, "tiled": tiled, "fused": fused,

@@ -108,3 +108,117 @@ def check_lds(name: str, need: int, limit: int, detail: str = "") -> None:
         if detail:
             _fail(f"{name}: {detail} needs {need} bytes of shared memory; this GPU allows {limit}")
         _fail(f"{name}: needs {need} bytes of shared memory, GPU allows {limit}")
+
+
+# ---------------------------------------------------------------- the paged cache (paged.py)
+EIGHT_BIT = (torch.int8, torch.float8_e4m3fn)
+
+
+def check_paged(name: str, rows, k_cache, v_cache, page_table, lengths, k_scale, v_scale, *,
+                require_cuda: bool = True) -> None:
+    """The cache's own tensors; `rows` is a tensor of the call's new tokens (None for cache_read)."""
+    device, dtype = k_cache.device, k_cache.dtype
+    tensors = [k_cache, v_cache, page_table, lengths] + [t for t in (rows, k_scale, v_scale) if t is not None]
+    for t in tensors:
+        if require_cuda and not t.is_cuda:
+            _fail(f"{name}: inputs must be CUDA tensors")
+        if t.device != device:
+            _fail(f"{name}: inputs must be on the same device")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        _fail(f"{name}: k_cache and v_cache must be shaped (pages, heads, page_size, d), both alike")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        _fail(f"{name}: k_cache and v_cache must be contiguous")
+    if dtype != v_cache.dtype:
+        _fail(f"{name}: k_cache and v_cache must share a dtype")
+    if dtype not in TC_DTYPES and dtype not in EIGHT_BIT:
+        _fail(f"{name}: the cache's dtype must be float16, bfloat16, int8 or float8_e4m3fn")
+    if rows is not None:
+        if rows.dtype not in TC_DTYPES:
+            _fail(f"{name}: float16 or bfloat16 only")
+        if dtype != rows.dtype and dtype not in EIGHT_BIT:
+            _fail(f"{name}: the cache's dtype must be the inputs' or an 8-bit one")
+    check_head_dim(name, k_cache, TC_HEAD_DIMS)
+    if k_cache.numel() == 0 or page_table.numel() == 0:
+        _fail(f"{name}: inputs must be non-empty")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.stride(1) != 1 and page_table.shape[1] > 1:
+        _fail(f"{name}: page_table must be a (B, columns) int32 tensor with contiguous rows")
+    if lengths.shape != page_table.shape[:1] or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        _fail(f"{name}: lengths must be a contiguous (B,) int32 tensor")
+    check_aligned(name, k_cache, v_cache)
+    if dtype in EIGHT_BIT:
+        for s in (k_scale, v_scale):
+            if s is None or s.shape != k_cache.shape[:3] or s.dtype != torch.float32 or not s.is_contiguous():
+                _fail(f"{name}: an 8-bit cache needs k_scale and v_scale, contiguous (pages, heads, page_size) float32")
+    elif k_scale is not None or v_scale is not None:
+        _fail(f"{name}: k_scale and v_scale are for 8-bit caches")
+
+
+def check_rows(name: str, x, k_cache, lengths, cu_seqlens) -> None:
+    """A tensor of new tokens, (tokens, heads, d)."""
+    if x.dim() != 3 or x.shape[2] != k_cache.shape[3]:
+        _fail(f"{name}: the new tokens' tensors must be shaped (tokens, heads, d) with the cache's d")
+    if x.numel() == 0:
+        _fail(f"{name}: inputs must be non-empty")
+    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8:
+        _fail(f"{name}: rows must be contiguous, at strides of whole 16-byte steps")
+    check_aligned(name, x)
+    if cu_seqlens is None:
+        if x.shape[0] % lengths.shape[0]:
+            _fail(f"{name}: without cu_seqlens the tokens must divide evenly over the sequences")
+    elif (cu_seqlens.shape != (lengths.shape[0] + 1,) or cu_seqlens.dtype != torch.int32
+          or not cu_seqlens.is_contiguous() or cu_seqlens.device != k_cache.device):
+        _fail(f"{name}: cu_seqlens must be a contiguous (B + 1,) int32 tensor on the inputs' device")
+
+
+def check_same_rows(name: str, k, v, k_cache) -> None:
+    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.shape[1] != k_cache.shape[1]:
+        _fail(f"{name}: k and v must share shape, dtype and device and have the cache's heads")
+
+
+def check_query_heads(name: str, q, k_cache) -> None:
+    if q.shape[1] % k_cache.shape[1]:
+        _fail(f"{name}: the query heads must be a multiple of the cache's heads")
+
+
+def _span(t) -> tuple[int, int]:
+    """The bytes from a tensor's first element to past its last one."""
+    size = t.element_size()
+    return t.data_ptr(), t.data_ptr() + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def check_out(name: str, q, out) -> None:
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        _fail(f"{name}: out must have q's shape, dtype and device")
+    if out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8:
+        _fail(f"{name}: rows must be contiguous, at strides of whole 16-byte steps")
+    check_aligned(name, out)
+    (tokens, heads, d), (ts, hs, _) = out.shape, out.stride()
+    by_token = (heads == 1 or hs >= d) and (tokens == 1 or ts >= (heads - 1) * hs + d)
+    by_head = (tokens == 1 or ts >= d) and (heads == 1 or hs >= (tokens - 1) * ts + d)
+    if not by_token and not by_head:
+        _fail(f"{name}: out's rows must not overlap")
+    (a0, a1), (b0, b1) = _span(q), _span(out)
+    if a0 < b1 and b0 < a1:
+        _fail(f"{name}: out must not share memory with q")
+
+
+def check_max_new(name: str, max_new) -> int:
+    if isinstance(max_new, bool) or not isinstance(max_new, int) or max_new < 1:
+        _fail(f"{name}: max_new must be a positive number of tokens")
+    return min(max_new, 2 ** 30)
+
+
+def check_max_len(name: str, n) -> None:
+    if isinstance(n, bool) or not isinstance(n, int) or n < 1 or n > 2 ** 30:
+        _fail(f"{name}: max_len must be a number of tokens from 1 to 2^30")
+
+
+def read_dtype(name: str, k_cache, dtype) -> torch.dtype:
+    """The dtype of the rows read back: the cache's own 16-bit one, or the caller's choice for an 8-bit cache."""
+    if k_cache.dtype in EIGHT_BIT:
+        if dtype not in TC_DTYPES:
+            _fail(f"{name}: dtype must be float16 or bfloat16 for an 8-bit cache")
+        return dtype
+    if dtype is not None and dtype != k_cache.dtype:
+        _fail(f"{name}: dtype must be the cache's own ({k_cache.dtype})")
+    return k_cache.dtype

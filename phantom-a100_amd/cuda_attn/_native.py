@@ -14,12 +14,23 @@ LIB_NAME = "libphantom_attn.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
 # include/phantom_attn.h: enum pa_dtype / pa_status
-DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I8, DTYPE_E4M3 = 0, 1, 2, 3, 4
 OK, ERR_INVALID, ERR_UNSUPPORTED = 0, -1, -2
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """pa_paged_cache."""
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("page_table", _p), ("lengths", _p),
+                ("pages", _i64), ("page_size", _i64), ("heads", _i64), ("d", _i64),
+                ("seqs", _i64), ("table_cols", _i64), ("table_stride", _i64), ("dtype", _i)]
+
+
+_cache = ctypes.POINTER(PagedCacheArgs)
+
 
 # name -> (restype, argtypes); must list every function the header declares.
 PROTOTYPES = {
@@ -34,6 +45,10 @@ PROTOTYPES = {
     "pa_fused_tuned_lds_bytes": (_i64, [_i, _i, _i, _i64, _i]),
     "pa_fused_tc_lds_bytes": (_i64, [_i64, _i]),
     "pa_device_lds_limit": (_i, [_i, ctypes.POINTER(_i64)]),
+    "pa_cache_write": (_i, [_cache, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _p, _p]),
+    "pa_cache_read": (_i, [_cache, _p, _p, _i, _i64, _p]),
+    "pa_paged_attn_fwd": (_i, [_cache, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i, _p, _i64, _p]),
+    "pa_paged_attn_workspace": (_i64, [_cache, _i, _i64, _i64, _i64]),
     "pa_last_error": (ctypes.c_char_p, []),
     "pa_version": (ctypes.c_char_p, []),
 }
