@@ -187,15 +187,17 @@ int pa_cache_read(const pa_paged_cache* cache, void* k, void* v, int dtype, int6
  * multiple of the cache's heads (query head h reads head h / (heads_q / heads)); o must not overlap q.
  * Rows behind the last sequence's are left as they are. max_new: an upper bound of the new tokens of a
  * sequence, 0 if unknown; only the choice of the kernel depends on it. workspace:
- * pa_paged_attn_workspace() bytes of device memory, 16-byte aligned, used until the call's kernels end
- * (NULL if that is 0); calls that may overlap need one each. */
+ * pa_paged_attn_workspace() bytes of device memory, 16-byte aligned, used until the call's kernels end;
+ * calls that may overlap need one each. */
 int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int dtype, int64_t tokens, int64_t heads_q,
                       int64_t q_token_stride, int64_t q_head_stride, int64_t o_token_stride, int64_t o_head_stride,
                       const int32_t* cu_seqlens, int64_t max_new, int causal, void* workspace, int64_t workspace_bytes,
                       void* stream);
 
-/* Bytes of workspace that pa_paged_attn_fwd needs for a call of these sizes on the current device. */
-int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q, int64_t max_new);
+/* Bytes of workspace that pa_paged_attn_fwd needs for a call with these arguments; a negative PA_ERR_* code if it
+ * refuses them. It depends on sizes alone, not on what the tensors hold. No GPU needed. */
+int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
+                                const int32_t* cu_seqlens, int64_t max_new);
 
 /* Message for the last nonzero status returned on this thread ("" if none). */
 const char* pa_last_error(void);

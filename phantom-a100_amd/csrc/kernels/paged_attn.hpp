@@ -16,57 +16,515 @@ struct RowsQ {
   int group, heads;                            // query heads per key/value head, and query heads
 };
 
-// One workgroup per (new token, query head): 256 / (D / 8) keys at a time, 8 dims a lane, each group of D / 8
-// lanes with a running maximum and sum of its own; the groups are joined through LDS at the end.
-template <typename T, typename C, int D>
-__global__ void __launch_bounds__(256) paged_attn_rows(PagedCache c, RowsQ a, float scale_log2, int causal) {
-  constexpr int LPR = D / 8, KPB = 256 / LPR;
-  __shared__ float acc_s[KPB][D];
-  __shared__ float m_s[KPB], l_s[KPB];
-  const int t = (int)blockIdx.x / a.heads, hq = (int)blockIdx.x % a.heads, h = hq / a.group;
-  const int sub = (int)threadIdx.x % LPR, kg = (int)threadIdx.x / LPR;
-  const int seq = find_seq(c, t);
-  if (seq >= c.seqs) return;
-  const SeqRows s = load_seq(c, seq);
-  if (t < s.first || t >= s.first + s.count) return;
-  const int seen = keys_seen(s, t - s.first, c.capacity, causal);
-  float q[8], o[8] = {}, m = -INFINITY, l = 0.f;
-  cached8(static_cast<const T*>(a.q) + t * a.q_token + hq * a.q_head, 8 * sub, 1.f, q);
-  for (int pos = kg; pos < seen; pos += KPB) {
-    const int at = cache_row(c, seq, h, pos);
-    if (at < 0) continue;
-    float x[8], ks = 1.f, vs = 1.f, dot = 0.f;
-    if constexpr (cache_type<C>::k8bit) ks = c.k_scale[at], vs = c.v_scale[at];
-    cached8(static_cast<const C*>(c.k) + (int64_t)at * D, 8 * sub, ks, x);
+// What a workgroup leaves for the join: a part of a tile that an earlier workgroup began (slot 0; bit kEnds if
+// it is the tile's last part), a tile begun and not ended (slot 1).
+struct PartRecord {
+  int seq, head, tile, flags;
+};
+constexpr int kPartContinues = 1, kPartEnds = 2, kPartBegins = 4;
+
+struct AttnWork {
+  TileShape tiles;
+  int min_units;       // a workgroup takes at least so many units of work
+  int whole, causal;
+  float scale_log2;
+  PartRecord* records;
+  float* parts;        // [workgroup][slot][row][D], then the rows' maxima and sums [workgroup][slot][2][row]
+};
+
+// Workspace of a call: a record and two slots of `rows` rows for each workgroup.
+__host__ __device__ __forceinline__ int64_t attn_record_bytes(int64_t wgs) { return (wgs * sizeof(PartRecord) + 255) / 256 * 256; }
+__host__ __device__ __forceinline__ int64_t attn_workspace(int64_t wgs, int rows, int d) {
+  return attn_record_bytes(wgs) + wgs * 2 * rows * (d + 2) * (int64_t)sizeof(float);
+}
+__device__ __forceinline__ float* part_rows(const AttnWork& w, int wg, int slot, int rows, int d) {
+  return w.parts + ((int64_t)wg * 2 + slot) * rows * d;
+}
+__device__ __forceinline__ float* part_stats(const AttnWork& w, int wgs, int wg, int slot, int rows, int d) {
+  return w.parts + (int64_t)wgs * 2 * rows * d + ((int64_t)wg * 2 + slot) * 2 * rows;
+}
+
+// Row r of a tile: its new token among the sequence's and its query head; false if the tile has no such row.
+__device__ __forceinline__ bool tile_row(const TileShape& t, const SeqRows& s, int head, int tile, int r, int& token, int& hq) {
+  const int in_tile = r / t.heads, g = head % t.splits * t.heads + r % t.heads;
+  token = tile * t.tokens + in_tile;
+  hq = head / t.splits * t.group + g;
+  return in_tile < t.tokens && token < s.count && g < t.group;
+}
+
+// Wave-uniform values in scalar registers: the walk and its branches are the same in every lane, which the
+// compiler cannot see where they come from LDS.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)(uint32_t)uniform((int)(uint32_t)x) | (int64_t)uniform((int)(x >> 32)) << 32;
+}
+__device__ __forceinline__ SeqRows uniform(SeqRows s) { return {uniform(s.first), uniform(s.count), uniform(s.length)}; }
+
+// The call's total units, and, where this workgroup has a share, its walk (active = false: it has none). All
+// threads of the workgroup take part; `lds` holds 256 + 4 sums.
+template <int THREADS>
+__device__ __forceinline__ bool start_walk(const PagedCache& c, const AttnWork& w, int64_t* lds, WorkWalk& walk) {
+  const int heads = c.heads * w.tiles.splits, tid = (int)threadIdx.x, lane = tid % kWave;
+  const int per = (c.seqs + THREADS - 1) / THREADS, s0 = min(tid * per, c.seqs), s1 = min(s0 + per, c.seqs);
+  auto units = [&](int s) -> int64_t {
+    const SeqRows r = load_seq(c, s);
+    return heads * tiles_cost(r, w.tiles, w.causal, tiles_of(r, w.tiles));
+  };
+  int64_t mine = 0;
+  for (int s = s0; s < s1; ++s) mine += units(s);
+  int64_t upto = mine;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dot = fmaf(q[j], x[j], dot);
-    dot += dpp_move<0xB1>(dot);
-    dot += dpp_move<0x4E>(dot);
-    dot += dpp_move<0x141>(dot);
-    if constexpr (LPR == 16) dot += dpp_move<0x140>(dot);
-    dot *= scale_log2;
-    const float mn = fmaxf(m, dot);
-    const float old = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
-    const float p = mn == -INFINITY ? 0.f : exp2_fast(dot - mn);
-    cached8(static_cast<const C*>(c.v) + (int64_t)at * D, 8 * sub, vs, x);
-    m = mn;
-    l = fmaf(l, old, p);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = fmaf(p, x[j], o[j] * old);
+  for (int d = 1; d < kWave; d *= 2) {
+    const int64_t other = __shfl_up(upto, d);
+    if (lane >= d) upto += other;
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc_s[kg][8 * sub + j] = o[j];
-  if (sub == 0) m_s[kg] = m, l_s[kg] = l;
+  if (lane == kWave - 1) lds[tid / kWave] = upto;
   __syncthreads();
-  if ((int)threadIdx.x < D) {
-    float mx = -INFINITY, sum = 0.f, out = 0.f;
-    for (int g = 0; g < KPB; ++g) mx = fmaxf(mx, m_s[g]);
-    for (int g = 0; g < KPB; ++g) {
-      const float w = m_s[g] == -INFINITY ? 0.f : exp2_fast(m_s[g] - mx);
-      sum = fmaf(w, l_s[g], sum);
-      out = fmaf(w, acc_s[g][threadIdx.x], out);
+  int64_t total = 0, before = upto - mine;
+#pragma unroll
+  for (int i = 0; i < THREADS / kWave; ++i) {
+    if (i < tid / kWave) before += lds[i];
+    total += lds[i];
+  }
+  total = uniform(total);
+  const int64_t most = total / w.min_units;
+  const int active = most < 1 ? 1 : most < (int64_t)gridDim.x ? (int)most : (int)gridDim.x;
+  if ((int)blockIdx.x >= active || total == 0) return false;
+  const int64_t at = share_of(total, active, (int)blockIdx.x), end = share_of(total, active, (int)blockIdx.x + 1);
+  // The thread whose sequences hold `at` looks for the one that does.
+  if (before <= at && at < before + mine) {
+    int s = s0;
+    for (int64_t u; s + 1 < s1 && before + (u = units(s)) <= at; ++s) before += u;
+    lds[8] = before;
+    lds[9] = s;
+  }
+  __syncthreads();
+  walk = WorkWalk{w.tiles, c.seqs, heads, c.capacity, w.causal != 0, w.whole != 0, at, end, uniform(lds[8]), uniform((int)lds[9])};
+  return true;
+}
+
+// ---- Eight or sixteen codes as 16-bit matrix operands (exact) ----
+// Pairs of f16 or bf16 in a dword.
+template <typename P> __device__ __forceinline__ unsigned pack16(P x) { return __builtin_bit_cast(unsigned, x); }
+// Four codes of one dword.
+__device__ __forceinline__ void widen4(unsigned w, e4m3*, f16*, unsigned& lo, unsigned& hi) {
+  lo = pack16(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, false));
+  hi = pack16(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, true));
+}
+__device__ __forceinline__ void widen4(unsigned w, e4m3*, bf16*, unsigned& lo, unsigned& hi) {
+  lo = pack16(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, false));
+  hi = pack16(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, true));
+}
+// int8 in fp16: 1024 + (x + 128) is 0x6400 with the biased byte as its low bits; 1152 less is x.
+__device__ __forceinline__ void widen4(unsigned w, i8*, f16*, unsigned& lo, unsigned& hi) {
+  const unsigned u = w ^ 0x80808080u;
+  const f16x2 bias = {(f16)1152.f, (f16)1152.f};
+  lo = pack16(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x07010700u)) - bias);
+  hi = pack16(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x07030702u)) - bias);
+}
+__device__ __forceinline__ void widen4(unsigned w, i8*, bf16*, unsigned& lo, unsigned& hi) {
+  const bf16x2 a = {(bf16)(float)(int8_t)w, (bf16)(float)(int8_t)(w >> 8)};
+  const bf16x2 b = {(bf16)(float)(int8_t)(w >> 16), (bf16)(float)(int8_t)(w >> 24)};
+  lo = pack16(a), hi = pack16(b);
+}
+// The 16 codes of a lane as two operands of 8.
+template <typename C, typename T>
+__device__ __forceinline__ void widen16(u32x4 w, u32x4& a, u32x4& b) {
+  unsigned x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) widen4(w[i], static_cast<C*>(nullptr), static_cast<T*>(nullptr), x[2 * i], x[2 * i + 1]);
+  a = u32x4{x[0], x[1], x[2], x[3]};
+  b = u32x4{x[4], x[5], x[6], x[7]};
+}
+
+// Largest magnitude, as its bits, of pairs of 16-bit values so far; not finite iff it has all exponent bits.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 max_bits(u16x2 acc, u32x4 w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc = __builtin_elementwise_max(acc, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  return acc;
+}
+template <typename T> constexpr unsigned short kInfBits = 0;
+template <> constexpr unsigned short kInfBits<f16> = 0x7c00;
+template <> constexpr unsigned short kInfBits<bf16> = 0x7f80;
+
+// x over the lanes of equal lane % 16.
+__device__ __forceinline__ float groups_max(float x) { x = fmaxf(x, partner16(x)); return fmaxf(x, partner32(x)); }
+__device__ __forceinline__ float groups_sum(float x) { x += partner16(x); return x + partner32(x); }
+
+// ---- Few rows a tile: single tokens, and the few tokens of one ----
+//
+// A tile has 16 NB rows; its keys go past once, and what bounds the kernel is reading them: 4 D bytes (2 D in 8
+// bits) for 4 D x rows operations. The waves of a workgroup take the steps of its segment (32 keys each) in
+// turn, each with a maximum, sum and O of its own, and join them through LDS at the segment's end: no barrier
+// inside the walk over the keys.
+//   S^T (32 keys x 16 queries) = K . Q^T   v_mfma 16x16x32, A = K as loaded (lane: key l % 16, 16 bytes), B = Q^T
+//   O^T (D x 16 queries) += V^T . P^T      A = V^T by transposing reads of the wave's own V rows in LDS
+// S^T leaves lane l with queries l % 16 and keys 4 (l / 16) + r of both halves of the step, which are the
+// k-slots of P^T once V^T is read in that order, so P^T goes from registers to the product.
+// 8-bit rows are widened to 16 bits (exact) on their way; a key's scale multiplies its scores, a value's scale
+// its P before the one rounding of P to the type.
+// A value that is not finite must reach the rows that see it and no others, and 0 x infinity would be a NaN:
+// a step that has one takes its P.V product in fp32 over the visible pairs instead.
+constexpr int few_waves(int nb) { return nb == 4 ? 1 : 2; }   // workgroups on a CU
+template <typename T, typename C, int D, int NB>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(NB))))
+paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
+  typedef typename vec8<T>::type V8;
+  constexpr bool k8 = cache_type<C>::k8bit;
+  constexpr int WAVES = 4, ROWS = 16 * NB, RB = D * 2;            // RB: bytes of a V row in LDS
+  constexpr int CB = k8 ? D : 2 * D;                              // bytes of a cache row
+  constexpr int LPR = CB / 16, RPL = kWave / LPR, VL = kStep / RPL;   // V loads: lanes per row, rows per load, loads
+  constexpr int KK = D / 32;                                      // 32-dim steps of a key block
+  constexpr int KL = k8 ? D / 64 : KK;                            // K loads of a 16-key block
+  constexpr int CR = D / 8;                                       // 16-byte chunks of a V row in LDS
+  constexpr int NDB = D / 16;                                     // 16-dim blocks of O^T
+  constexpr int WAVE_BYTES = kStep * RB;
+  static_assert(WAVE_BYTES >= D * 16 * 4, "a wave's V rows make room for 16 rows of its O");
+  __shared__ __attribute__((aligned(1024))) unsigned char v_lds[WAVES][WAVE_BYTES];
+  __shared__ float stat_lds[WAVES][2][16];
+  __shared__ float scale_lds[WAVES][2][kStep];
+  __shared__ int64_t walk_lds[10];
+  const int tid = (int)threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int g = lane / 16, lq = lane % 16;
+
+  PartRecord rec = {0, 0, 0, 0};
+  WorkWalk walk;
+  const bool active = start_walk<256>(c, w, walk_lds, walk);
+  Segment sg;
+  unsigned char* vw = v_lds[wave];
+  // Swizzled 16-byte chunk of a V row: the 8 rows x 2 chunks that 32 lanes of a transposing read touch lie in
+  // distinct banks.
+  auto v_at = [](int row, int chunk) {
+    return row * RB + ((chunk ^ (CR == 16 ? 2 * (row & 7) : 2 * ((row >> 1) & 3))) * 16);
+  };
+
+  // Its reads and writes by lane: one base each, the rest by constants (a hoisted address for every one costs
+  // 30 registers). A write of load i is i RPL rows below the lane's first, whose swizzle differs where loads
+  // alternate between the halves of 8 rows.
+  const int w_row = lane / LPR, w_chunk = lane % LPR * (k8 ? 2 : 1);
+  int w_base = v_at(w_row, w_chunk), r_base = v_at(4 * g + lq / 4, lq % 4 / 2) + 8 * (lq % 2);
+  auto v_write = [&](int i) { return i * RPL * RB + (w_base ^ (RPL == 4 && CR == 16 && i % 2 ? 128 : 0)); };
+
+  while (active && uniform((int)walk.next([&](int s) { return uniform(load_seq(c, s)); }, sg)) != 0) {
+    sg = {uniform(sg.rows), uniform(sg.seq), uniform(sg.head), uniform(sg.tile), uniform(sg.from), uniform(sg.to), uniform(sg.steps)};
+    const int kv_head = sg.head / w.tiles.splits;
+    // ---- the tile's queries
+    u32x4 qf[NB][KK];
+    int seen[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      int token, hq;
+      const bool mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, 16 * b + lq, token, hq);
+      seen[b] = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
+      const T* qp = static_cast<const T*>(a.q) + (mine ? (int64_t)(sg.rows.first + token) * a.q_token + hq * a.q_head : 0);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const int dim = k8 ? 64 * (kk / 2) + 16 * g + 8 * (kk % 2) : 32 * kk + 8 * g;
+        qf[b][kk] = mine ? *reinterpret_cast<const u32x4*>(qp + dim) : u32x4{0, 0, 0, 0};
+      }
     }
-    static_cast<T*>(a.o)[t * a.o_token + hq * a.o_head + threadIdx.x] = from_f32<T>(sum == 0.f ? 0.f : out / sum);
+    int all_seen = seen[0], any_seen = seen[0];   // keys that every row, and that some row, sees
+    {
+      // (rows of no token count for neither)
+      int lo = INT32_MAX, hi = 0;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        int token, hq;
+        if (tile_row(w.tiles, sg.rows, sg.head, sg.tile, 16 * b + lq, token, hq)) lo = min(lo, seen[b]), hi = max(hi, seen[b]);
+      }
+#pragma unroll
+      for (int d = 1; d < 16; d *= 2) lo = min(lo, __shfl_xor(lo, d)), hi = max(hi, __shfl_xor(hi, d));
+      all_seen = __builtin_amdgcn_readfirstlane(lo);
+      any_seen = __builtin_amdgcn_readfirstlane(hi);
+    }
+    float m[NB], l[NB], vref = 1e-30f;
+    f32x4 o[NB][NDB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      m[b] = -INFINITY;
+      l[b] = 0.f;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) o[b][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- loads of a step: each lane looks up one key (lane % 32), the others get it by lane. A step's page
+    // table entries are loaded a step before its rows are, and looked at (find_row) when they are needed.
+    u32x4 kr[2][KL], vr[VL];
+    float ks = 0.f, vs = 0.f;
+    const int* table = c.table + sg.seq * c.table_stride;
+    auto load_page = [&](int step) { return table[page_of((uint32_t)min(step * kStep + lane % 32, c.capacity - 1), c.div)]; };
+    auto find_row = [&](int step, int page) {
+      const int key = step * kStep + lane % 32;
+      const uint32_t at = ((uint32_t)page * c.heads + kv_head) * c.page_size + (key - page_of((uint32_t)key, c.div) * c.page_size);
+      return key < any_seen && (unsigned)page < (unsigned)c.pages ? (int)at : -1;
+    };
+    auto load_step = [&](int row) {
+      const int at = max(row, 0);   // (an absent row reads the cache's first one, and counts for nothing)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const unsigned char* p = static_cast<const unsigned char*>(c.k) + (int64_t)__shfl(at, 16 * b + lq) * CB;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) kr[b][i] = *reinterpret_cast<const u32x4*>(p + 64 * i + 16 * g);
+      }
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const unsigned char* p = static_cast<const unsigned char*>(c.v) + (int64_t)__shfl(at, i * RPL + lane / LPR) * CB;
+        vr[i] = *reinterpret_cast<const u32x4*>(p + lane % LPR * 16);
+      }
+      if constexpr (k8) ks = c.k_scale[at], vs = c.v_scale[at];
+    };
+
+    int step = sg.from + wave, row = -1, page = 0;
+    if (step < sg.to) {
+      page = load_page(step);
+      row = find_row(step, page);
+      page = load_page(step + WAVES);
+      load_step(row);
+    }
+    for (; step < sg.to; step += WAVES) {
+      const unsigned present = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);   // of the step's 32 keys
+      const int key0 = step * kStep;
+      const bool clean = present == 0xffffffffu && key0 + kStep <= all_seen;
+      // ---- V to LDS, S^T
+      u16x2 top = {0, 0};
+      asm volatile("" : "+v"(w_base), "+v"(r_base));
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int r = i * RPL + w_row;
+        if (present != 0xffffffffu && !(present >> r & 1)) vr[i] = u32x4{0, 0, 0, 0};
+        if constexpr (k8) {
+          u32x4 x, y;
+          widen16<C, T>(vr[i], x, y);
+          top = max_bits(max_bits(top, x), y);
+          *reinterpret_cast<u32x4*>(vw + v_write(i)) = x;
+          *reinterpret_cast<u32x4*>(vw + (v_write(i) ^ 16)) = y;
+        } else {
+          top = max_bits(top, vr[i]);
+          *reinterpret_cast<u32x4*>(vw + v_write(i)) = vr[i];
+        }
+      }
+      const bool odd = __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= kInfBits<T>) != 0;
+      f32x4 s[NB][2];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) s[b][0] = s[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          u32x4 x, y;
+          if constexpr (k8) {
+            widen16<C, T>(kr[h][kk / 2], x, y);
+            if (kk % 2) x = y;
+          } else {
+            x = kr[h][kk];
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            s[b][h] = mfma16x16x32(__builtin_bit_cast(V8, x), __builtin_bit_cast(V8, qf[b][kk]), s[b][h]);
+        }
+      f32x4 ksc[2], vsc[2];
+      if constexpr (k8) {
+        if (lane < 32) scale_lds[wave][0][lane] = ks, scale_lds[wave][1][lane] = vs;
+        if constexpr (std::is_same<T, f16>::value) {
+          // P times a value's scale must stay in fp16's range: O is held in units of vref, the largest scale so far.
+          const float big = wave_allreduce(row >= 0 && fabsf(vs) < INFINITY ? fabsf(vs) : 0.f, MaxOp{});
+          if (big > vref) {
+            const float f = vref / big;
+            vref = big;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int db = 0; db < NDB; ++db) o[b][db] *= f;
+          }
+        }
+      }
+      // ---- the next step's rows, into the registers that this one's have left
+      __builtin_amdgcn_sched_barrier(0);
+      if (step + WAVES < sg.to) {
+        row = find_row(step + WAVES, page);
+        page = load_page(step + 2 * WAVES);
+        load_step(row);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (k8) {
+        const float unit = std::is_same<T, f16>::value ? 1.f / vref : 1.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          ksc[h] = *reinterpret_cast<const f32x4*>(&scale_lds[wave][0][16 * h + 4 * g]) * w.scale_log2;
+          vsc[h] = *reinterpret_cast<const f32x4*>(&scale_lds[wave][1][16 * h + 4 * g]) * unit;
+        }
+      }
+      // ---- softmax
+      V8 pf[NB];
+      float p32[NB][8];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float t[8], mx = -INFINITY;
+        // Keys (of this lane, j = 4 half + r) that the row sees: bit j.
+        unsigned sees = 0xff;
+        if (!clean) {
+          sees = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int k = 16 * (j / 4) + 4 * g + j % 4;
+            sees |= key0 + k < seen[b] && (present >> k & 1) ? 1u << j : 0u;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          t[j] = s[b][j / 4][j % 4] * (k8 ? ksc[j / 4][j % 4] : w.scale_log2);
+          if (!clean) t[j] = sees >> j & 1 ? t[j] : -INFINITY;
+          mx = fmaxf(mx, t[j]);
+        }
+        const float m_new = fmaxf(m[b], groups_max(mx));
+        const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+        if (__builtin_amdgcn_ballot_w64(m_new > m[b]) != 0) {
+          const float f = m[b] == -INFINITY ? 0.f : exp2_fast(m[b] + neg_m);
+          l[b] *= f;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) o[b][db] *= f;
+          m[b] = m_new;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float p = exp2_fast(t[j] + neg_m);
+          l[b] += p;
+          if constexpr (k8) {
+            p *= vsc[j / 4][j % 4];
+            if (!clean) p = sees >> j & 1 ? p : 0.f;   // (0 x a scale that is not finite)
+          }
+          p32[b][j] = p;
+          pf[b][j] = from_f32<T>(p);
+        }
+      }
+      // ---- O^T += V^T . P^T
+      if (!odd) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const unsigned char* p = vw + (r_base ^ (32 * db));
+          const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p));
+          const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p + 16 * RB));
+          const i16x8 x = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+#pragma unroll
+          for (int b = 0; b < NB; ++b) o[b][db] = mfma16x16x32(__builtin_bit_cast(V8, x), pf[b], o[b][db]);
+        }
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < kStep; ++k) {
+          const int from = (k % 16) / 4 * 16 + lq, j = k / 16 * 4 + k % 4;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            float p = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p = i == j ? p32[b][i] : p;
+            p = __shfl(p, from);
+            if (key0 + k < seen[b] && (present >> k & 1)) {
+#pragma unroll
+              for (int db = 0; db < NDB; ++db) {
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                const T4 x = *reinterpret_cast<const T4*>(vw + v_at(k, 2 * db + g / 2) + 8 * (g % 2));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[b][db][r] = fmaf(p, to_f32(x[r]), o[b][db][r]);
+              }
+            }
+          }
+        }
+      }
+    }
+
+    // ---- join the waves, 16 rows at a time through the V rows' LDS
+    const bool done = sg.from == 0 && sg.to == sg.steps;
+    const int slot = sg.from == 0 ? 1 : 0;
+    if (!done) {
+      if (sg.from == 0) rec = {sg.seq, sg.head, sg.tile, rec.flags | kPartBegins};
+      else rec.flags |= kPartContinues | (sg.to == sg.steps ? kPartEnds : 0);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float ls = groups_sum(l[b]);
+      const float unit = k8 && std::is_same<T, f16>::value ? vref : 1.f;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        *reinterpret_cast<f32x4*>(vw + lq * (D * 4) + (((4 * db + g) ^ lq) * 16)) = o[b][db] * unit;
+      // (Scores that are all NaN leave no maximum and a NaN sum, which must not count as a row that sees nothing.)
+      if (lane < 16) stat_lds[wave][0][lane] = m[b] == -INFINITY && ls != 0.f ? 0.f : m[b], stat_lds[wave][1][lane] = ls;
+      __syncthreads();
+      const int q = tid / 16, part = tid % 16;   // 16 threads a row, D / 16 dims each
+      constexpr int EL = D / 16;
+      float mx = -INFINITY, sum = 0.f, x[EL] = {};
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) mx = fmaxf(mx, stat_lds[i][0][q]);
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        const float f = stat_lds[i][0][q] == -INFINITY ? 0.f : exp2_fast(stat_lds[i][0][q] - mx);
+        sum = fmaf(f, stat_lds[i][1][q], sum);
+#pragma unroll
+        for (int e = 0; e < EL; e += 4) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(&v_lds[i][q * (D * 4) + (((part * (EL / 4) + e / 4) ^ q) * 16)]);
+          if (f > 0.f)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[e + j] = fmaf(f, y[j], x[e + j]);
+        }
+      }
+      int token, hq;
+      if (tile_row(w.tiles, sg.rows, sg.head, sg.tile, 16 * b + q, token, hq)) {
+        if (done) {
+          typedef T TE __attribute__((ext_vector_type(EL)));
+          TE y;
+#pragma unroll
+          for (int e = 0; e < EL; ++e) y[e] = from_f32<T>(sum == 0.f ? 0.f : x[e] / sum);
+          *reinterpret_cast<TE*>(static_cast<T*>(a.o) + (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head + part * EL) = y;
+        } else {
+          float* to = part_rows(w, (int)blockIdx.x, slot, ROWS, D) + (16 * b + q) * D + part * EL;
+#pragma unroll
+          for (int e = 0; e < EL; e += 4) *reinterpret_cast<f32x4*>(to + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+          if (part == 0) {
+            float* st = part_stats(w, (int)gridDim.x, (int)blockIdx.x, slot, ROWS, D);
+            st[16 * b + q] = mx, st[ROWS + 16 * b + q] = sum;
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  if (tid == 0) w.records[blockIdx.x] = rec;
+}
+
+// Joins the parts of the tile that workgroup blockIdx.x of the attention kernel began and did not end: its own
+// and those of the workgroups after it, up to the one that ends the tile. 16 threads a row.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(256) paged_attn_join(PagedCache c, RowsQ a, AttnWork w, int wgs) {
+  constexpr int EL = D / 16;
+  const PartRecord rec = w.records[blockIdx.x];
+  if (!(rec.flags & kPartBegins)) return;
+  const SeqRows s = load_seq(c, rec.seq);
+  const int part = (int)threadIdx.x % 16;
+  for (int r = (int)blockIdx.y * 16 + (int)threadIdx.x / 16; r < ROWS; r += (int)gridDim.y * 16) {
+    int token, hq;
+    if (!tile_row(w.tiles, s, rec.head, rec.tile, r, token, hq)) continue;
+    float m = -INFINITY, sum = 0.f, x[EL] = {};
+    for (int i = (int)blockIdx.x; i < wgs; ++i) {
+      const int slot = i == (int)blockIdx.x ? 1 : 0;
+      const float* st = part_stats(w, wgs, i, slot, ROWS, D);
+      const float* from = part_rows(w, i, slot, ROWS, D) + r * D + part * EL;
+      const float mi = st[r], mn = fmaxf(m, mi);
+      const float f = m == -INFINITY ? 0.f : exp2_fast(m - mn), fi = mi == -INFINITY ? 0.f : exp2_fast(mi - mn);
+      sum = sum * f + st[ROWS + r] * fi;
+#pragma unroll
+      for (int e = 0; e < EL; e += 4) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(from + e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[e + j] = (f > 0.f ? x[e + j] * f : 0.f) + (fi > 0.f ? y[j] * fi : 0.f);
+      }
+      m = mn;
+      if (i != (int)blockIdx.x && (w.records[i].flags & kPartEnds)) break;
+    }
+    typedef T TE __attribute__((ext_vector_type(EL)));
+    TE y;
+#pragma unroll
+    for (int e = 0; e < EL; ++e) y[e] = from_f32<T>(sum == 0.f ? 0.f : x[e] / sum);
+    *reinterpret_cast<TE*>(static_cast<T*>(a.o) + (int64_t)(s.first + token) * a.o_token + hq * a.o_head + part * EL) = y;
   }
 }
 

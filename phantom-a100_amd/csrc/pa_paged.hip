@@ -78,6 +78,42 @@ hipError_t with_types(int dtype, int cache_dtype, int64_t d, F f) {
   return dtype == PA_DTYPE_F16 ? with_cache_type<pa::f16>(cache_dtype, d, f) : with_cache_type<pa::bf16>(cache_dtype, d, f);
 }
 
+constexpr int kCUs = 256;   // MI355X / gfx950
+
+// The launch of an attention call: tiles of 16 * nb rows, workgroups, and whether tiles are cut.
+struct AttnPlan {
+  int nb, wgs;
+  bool whole;
+};
+// A cache of at most so many positions a sequence is read in a few steps: its tiles are not cut over workgroups,
+// which saves the second launch that joins them.
+constexpr int kWholeCapacity = 256;
+AttnPlan attn_plan(const pa::PagedCache& c, int64_t heads_q, int64_t max_new) {
+  const int64_t group = heads_q / c.heads;
+  const int64_t new_tokens = !c.cu ? c.per_seq : max_new > 0 ? std::min<int64_t>(max_new, c.tokens) : c.tokens;
+  const int64_t rows = new_tokens * group;
+  const int nb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  // As many workgroups as are resident at once, or fewer where the work's bound is below their least share.
+  const pa::TileShape t = pa::make_tiles((int)group, 16 * nb);
+  const double tiles = (double)c.tokens / t.tokens + c.seqs;
+  const double units = tiles * c.heads * t.splits * ((double)pa::kTileCost + c.capacity);
+  const int resident = kCUs * pa::few_waves(nb);
+  const int wgs = (int)std::max(1.0, std::min<double>(resident, units / pa::kMinUnits + 1));
+  return {nb, wgs, c.capacity <= kWholeCapacity};
+}
+
+template <typename T, typename C, int D, int NB>
+hipError_t launch_few(const pa::PagedCache& c, const pa::RowsQ& a, const AttnPlan& plan, int causal, void* workspace,
+                      hipStream_t stream) {
+  const pa::AttnWork w{pa::make_tiles(a.group, 16 * NB), pa::kMinUnits, plan.whole, causal, pa::kLog2e / sqrtf((float)D),
+                       static_cast<pa::PartRecord*>(workspace),
+                       reinterpret_cast<float*>(static_cast<char*>(workspace) + pa::attn_record_bytes(plan.wgs))};
+  hipLaunchKernelGGL((pa::paged_attn_few<T, C, D, NB>), dim3((unsigned)plan.wgs), dim3(256), 0, stream, c, a, w);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || plan.whole) return e;
+  hipLaunchKernelGGL((pa::paged_attn_join<T, D, 16 * NB>), dim3((unsigned)plan.wgs, NB), dim3(256), 0, stream, c, a, w, plan.wgs);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 extern "C" {
@@ -143,23 +179,34 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
   };
   if (!apart(o_token_stride, tokens, o_head_stride, heads_q) && !apart(o_head_stride, heads_q, o_token_stride, tokens))
     return fail(PA_ERR_INVALID, "%s: out's rows must not overlap", name);
-  if (tokens * heads_q >= (1 << 24)) return fail(PA_ERR_UNSUPPORTED, "%s: too many rows for one launch", name);
-  (void)max_new, (void)workspace, (void)workspace_bytes;
+  if (max_new < 0) return fail(PA_ERR_INVALID, "%s: max_new must not be negative", name);
+  const AttnPlan plan = attn_plan(c, heads_q, max_new);
+  if (workspace_bytes < pa::attn_workspace(plan.wgs, 16 * plan.nb, (int)cache->d) || !workspace || !aligned16(workspace))
+    return fail(PA_ERR_INVALID, "%s: the workspace is too small, null or not 16-byte aligned", name);
   const pa::RowsQ a{q, o, q_token_stride, q_head_stride, o_token_stride, o_head_stride, (int)(heads_q / cache->heads),
                     (int)heads_q};
-  const float scale_log2 = pa::kLog2e / sqrtf((float)cache->d);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   const hipError_t e = with_types(dtype, cache->dtype, cache->d, [&](auto t, auto ct, auto dim) {
-    hipLaunchKernelGGL((pa::paged_attn_rows<decltype(t), decltype(ct), decltype(dim)::value>),
-                       dim3((unsigned)(tokens * heads_q)), dim3(256), 0, static_cast<hipStream_t>(stream), c, a,
-                       scale_log2, causal);
-    return hipGetLastError();
+    typedef decltype(t) T;
+    typedef decltype(ct) C;
+    constexpr int D = decltype(dim)::value;
+    return plan.nb == 1 ? launch_few<T, C, D, 1>(c, a, plan, causal, workspace, st)
+         : plan.nb == 2 ? launch_few<T, C, D, 2>(c, a, plan, causal, workspace, st)
+                        : launch_few<T, C, D, 4>(c, a, plan, causal, workspace, st);
   });
   return hip_status(e, name);
 }
 
-int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q, int64_t max_new) {
-  (void)cache, (void)dtype, (void)tokens, (void)heads_q, (void)max_new;
-  return 0;
+int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
+                                const int32_t* cu_seqlens, int64_t max_new) {
+  const char* name = "paged_attn";
+  pa::PagedCache c;
+  if (int rc = check_cache(name, cache, dtype, &c)) return rc;
+  if (int rc = check_tokens(name, tokens, cu_seqlens, &c)) return rc;
+  if (heads_q <= 0 || heads_q > (1 << 16) || heads_q % cache->heads != 0 || max_new < 0)
+    return fail(PA_ERR_INVALID, "%s: the query heads must be a multiple of the cache's heads, max_new not negative", name);
+  const AttnPlan plan = attn_plan(c, heads_q, max_new);
+  return pa::attn_workspace(plan.wgs, 16 * plan.nb, (int)cache->d);
 }
 
 }  // extern "C"

@@ -48,4 +48,96 @@ __host__ __device__ __forceinline__ int keys_seen(const SeqRows& s, int i, int c
   return clamp_int(causal ? new_token_pos(s, i) + 1 : s.length, 0, capacity);
 }
 
+// ---- Work of an attention call, and its division over workgroups ----
+//
+// A tile is up to `rows` query rows that read the same keys: `heads` query heads of one key/value head times
+// `tokens` consecutive new tokens of one sequence. Tiles are counted sequence by sequence, head by head, token
+// by token; each costs about as many units as it has keys to read (closed forms, so that a workgroup finds its
+// place without a list). Workgroup w of n takes the units [share(w), share(w + 1)): the same number for every
+// workgroup whatever the lengths are, cut at steps of kStep keys. What a cut leaves of a tile are partial
+// results, joined afterwards.
+constexpr int kStep = 32;       // keys of a step
+constexpr int kTileCost = 64;   // units a tile costs beside its keys
+constexpr int kMinUnits = 128;  // least units of a workgroup: a step for each of four waves
+
+struct TileShape {
+  int group, heads, tokens, splits;   // query heads per key/value head; of a tile; tokens of a tile; tiles that cover the group
+};
+__host__ __device__ __forceinline__ TileShape make_tiles(int group, int rows) {
+  const int heads = group < rows ? group : rows;
+  return {group, heads, rows / heads, (group + heads - 1) / heads};
+}
+__host__ __device__ __forceinline__ int tiles_of(const SeqRows& s, const TileShape& t) {
+  return (s.count + t.tokens - 1) / t.tokens;
+}
+// Units of a sequence's first n tiles (n at most tiles_of) of one head. A causal tile counts the keys up to its
+// last token's; only the last tile can have fewer tokens than the others.
+__host__ __device__ __forceinline__ int64_t tiles_cost(const SeqRows& s, const TileShape& t, bool causal, int64_t n) {
+  const int before = s.length - s.count;
+  int64_t cost = n * (kTileCost + (causal ? (before > 0 ? before : 0) : s.length));
+  if (causal) {
+    const int64_t full = n < s.count / t.tokens ? n : s.count / t.tokens;
+    cost += t.tokens * (full * (full + 1) / 2) + (n > full ? s.count : 0);
+  }
+  return cost;
+}
+// Steps of a tile: those with a key that its last token sees, and one if there is none.
+__host__ __device__ __forceinline__ int tile_steps(const SeqRows& s, const TileShape& t, int tile, int capacity, bool causal) {
+  const int last = (tile + 1) * (int64_t)t.tokens < s.count ? (tile + 1) * t.tokens - 1 : s.count - 1;
+  const int keys = keys_seen(s, last, capacity, causal);
+  return keys == 0 ? 1 : (keys - 1) / kStep + 1;
+}
+__host__ __device__ __forceinline__ int64_t share_of(int64_t total, int n, int w) {
+  const int64_t each = total / n, rest = total % n;
+  return each * w + (w < rest ? w : rest);
+}
+
+// A workgroup's part of one tile: steps [from, to) of `steps`; `head` counts key/value heads times splits.
+struct Segment {
+  SeqRows rows;
+  int seq, head, tile, from, to, steps;
+};
+// The segments of units [at, end), from sequence `seq` (whose units begin at `begin`) on. load(s) gives a
+// sequence's rows. whole: tiles are not cut, one belongs to the workgroup whose units hold its first.
+struct WorkWalk {
+  TileShape tiles;
+  int seqs, heads, capacity;   // heads: key/value heads times splits
+  bool causal, whole;
+  int64_t at, end, begin;
+  int seq;
+
+  template <typename Load>
+  __host__ __device__ bool next(Load load, Segment& out) {
+    while (at < end && seq < seqs) {
+      const SeqRows s = load(seq);
+      const int n = tiles_of(s, tiles);
+      const int64_t per_head = tiles_cost(s, tiles, causal, n), all = per_head * heads;
+      if (at >= begin + all) {
+        begin += all;
+        ++seq;
+        continue;
+      }
+      const int64_t r = at - begin;
+      const int head = (int)(r / per_head);
+      const int64_t in_head = r - head * per_head;
+      int tile = 0;   // the last tile that begins at or before in_head
+      for (int hi = n - 1; tile < hi;) {
+        const int mid = tile + (hi - tile + 1) / 2;
+        if (tiles_cost(s, tiles, causal, mid) <= in_head) tile = mid; else hi = mid - 1;
+      }
+      const int64_t t0 = begin + head * per_head + tiles_cost(s, tiles, causal, tile);
+      const int64_t t1 = begin + head * per_head + tiles_cost(s, tiles, causal, tile + 1);
+      const int steps = tile_steps(s, tiles, tile, capacity, causal);
+      const int64_t from = at == t0 ? 0 : whole ? steps : (at - t0) / kStep;
+      const int64_t to = end >= t1 || whole ? steps : (end - t0) / kStep;
+      at = t1 < end ? t1 : end;
+      if (from < to && from < steps) {
+        out = {s, seq, head, tile, (int)from, (int)(to < steps ? to : steps), steps};
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
 }  // namespace pa

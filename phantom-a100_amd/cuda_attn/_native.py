@@ -48,7 +48,7 @@ PROTOTYPES = {
     "pa_cache_write": (_i, [_cache, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _p, _p]),
     "pa_cache_read": (_i, [_cache, _p, _p, _i, _i64, _p]),
     "pa_paged_attn_fwd": (_i, [_cache, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i, _p, _i64, _p]),
-    "pa_paged_attn_workspace": (_i64, [_cache, _i, _i64, _i64, _i64]),
+    "pa_paged_attn_workspace": (_i64, [_cache, _i, _i64, _i64, _p, _i64]),
     "pa_last_error": (ctypes.c_char_p, []),
     "pa_version": (ctypes.c_char_p, []),
 }

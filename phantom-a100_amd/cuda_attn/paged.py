@@ -108,9 +108,12 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     cache = _cache_args(k_cache, v_cache, page_table, lengths, k_scale, v_scale)
     tokens, heads_q, _ = q.shape
     code = _DTYPE_CODE[q.dtype]
-    need = _native.lib().pa_paged_attn_workspace(cache, code, tokens, heads_q, bound)
-    workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    cu = None if cu_seqlens is None else cu_seqlens.data_ptr()
+    need = _native.lib().pa_paged_attn_workspace(cache, code, tokens, heads_q, cu, bound)
+    if need < 0:
+        _native.check(need, "paged_attn")
+    workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     _call("pa_paged_attn_fwd", "paged_attn", q.device, cache, q.data_ptr(), out.data_ptr(), code, tokens, heads_q,
-          q.stride(0), q.stride(1), out.stride(0), out.stride(1), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-          bound, 1 if causal else 0, None if workspace is None else workspace.data_ptr(), need, _stream_ptr(q.device))
+          q.stride(0), q.stride(1), out.stride(0), out.stride(1), cu, bound, 1 if causal else 0, workspace.data_ptr(),
+          need, _stream_ptr(q.device))
     return out

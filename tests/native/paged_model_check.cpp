@@ -21,6 +21,62 @@ static uint32_t rnd() {
   return (uint32_t)(s >> 16);
 }
 
+// Every step of every tile belongs to exactly one workgroup, in order; a tile's parts after its first are the
+// first segments of the workgroups that follow, as the join of partial results takes them.
+static void check_work() {
+  for (int round = 0; round < 3000; ++round) {
+    const int group = 1 + rnd() % 20, rows = 16 << rnd() % 4, seqs = 1 + rnd() % 12, kv_heads = 1 + rnd() % 4;
+    const int capacity = 1 + rnd() % 3000, n = 1 + rnd() % 40, min_units = 128;
+    const bool causal = rnd() % 2, whole = rnd() % 4 == 0, wild = rnd() % 8 == 0;
+    const pa::TileShape tiles = pa::make_tiles(group, rows);
+    CHECK(tiles.heads * tiles.tokens <= rows && tiles.heads * tiles.splits >= group);
+    pa::SeqRows seq[12];
+    int first = 0;
+    for (int s = 0; s < seqs; ++s) {
+      const int count = rnd() % 3 == 0 ? 0 : rnd() % 3 ? 1 : rnd() % 300;
+      const int length = wild ? rnd() % 2000 : count + rnd() % 2500;
+      seq[s] = {first, count, length};
+      first += count;
+    }
+    const int heads = kv_heads * tiles.splits;
+    int64_t total = 0;
+    for (int s = 0; s < seqs; ++s) total += heads * pa::tiles_cost(seq[s], tiles, causal, pa::tiles_of(seq[s], tiles));
+    const int active = (int)(total / min_units < 1 ? 1 : total / min_units < n ? total / min_units : n);
+    // the tile that the next segment must continue or begin
+    int s = 0, head = 0, tile = 0, step = 0;
+    auto skip_empty = [&] { while (s < seqs && seq[s].count == 0) ++s; };
+    skip_empty();
+    for (int w = 0; w < active; ++w) {
+      const int64_t at = pa::share_of(total, active, w), end = pa::share_of(total, active, w + 1);
+      pa::WorkWalk walk{tiles, seqs, heads, capacity, causal, whole, at, end, 0, 0};
+      for (int i = 0; i < seqs; ++i) {   // the sequence that holds `at`
+        const int64_t all = heads * pa::tiles_cost(seq[i], tiles, causal, pa::tiles_of(seq[i], tiles));
+        if (walk.begin + all > at) break;
+        walk.begin += all;
+        walk.seq = i + 1;
+      }
+      pa::Segment g;
+      bool head_of_list = true;
+      while (walk.next([&](int i) { return seq[i]; }, g)) {
+        CHECK(g.seq == s && g.head == head && g.tile == tile && g.from == step && g.from < g.to && g.to <= g.steps);
+        CHECK(g.steps == pa::tile_steps(seq[s], tiles, tile, capacity, causal));
+        CHECK(g.from == 0 || (head_of_list && !whole));
+        head_of_list = false;
+        step = g.to;
+        if (step == g.steps) {
+          step = 0;
+          if (++tile == pa::tiles_of(seq[s], tiles)) {
+            tile = 0;
+            if (++head == heads) head = 0, ++s, skip_empty();
+          }
+        }
+      }
+      CHECK(step == 0 || !head_of_list);   // an unfinished tile is continued by the very next workgroup
+    }
+    CHECK(s == seqs && head == 0 && tile == 0 && step == 0);
+  }
+}
+
 int main() {
   const uint32_t top = 1u << 30;
   auto check_div = [&](uint32_t d) {
@@ -52,6 +108,7 @@ int main() {
               CHECK(pa::keys_seen(s, i, cap, false) == (s.length < cap ? s.length : cap));
             }
         }
+  check_work();
   std::printf("ok\n");
   return 0;
 }
