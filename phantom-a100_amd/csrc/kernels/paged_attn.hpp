@@ -5,6 +5,7 @@
 // key/value head h / group. A token that sees no key gets zeros.
 #pragma once
 
+#include "fa_mfma.hpp"
 #include "paged_cache.hpp"
 
 namespace pa {
@@ -58,12 +59,14 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ int64_t uniform(int64_t x) {
   return (int64_t)(uint32_t)uniform((int)(uint32_t)x) | (int64_t)uniform((int)(x >> 32)) << 32;
 }
+__device__ __forceinline__ float uniform_f(float x) { return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, x))); }
 __device__ __forceinline__ SeqRows uniform(SeqRows s) { return {uniform(s.first), uniform(s.count), uniform(s.length)}; }
 
-// The call's total units, and, where this workgroup has a share, its walk (active = false: it has none). All
-// threads of the workgroup take part; `lds` holds 256 + 4 sums.
+// The workgroup's number `wg` among the shares and, where it has a share, its walk (false: it has none). All
+// threads of the workgroup take part; `lds` holds 10 numbers. by_xcd: shares that follow each other go to one
+// XCD, whose L2 then serves the tiles of a head together.
 template <int THREADS>
-__device__ __forceinline__ bool start_walk(const PagedCache& c, const AttnWork& w, int64_t* lds, WorkWalk& walk) {
+__device__ __forceinline__ bool start_walk(const PagedCache& c, const AttnWork& w, bool by_xcd, int64_t* lds, int& wg, WorkWalk& walk) {
   const int heads = c.heads * w.tiles.splits, tid = (int)threadIdx.x, lane = tid % kWave;
   const int per = (c.seqs + THREADS - 1) / THREADS, s0 = min(tid * per, c.seqs), s1 = min(s0 + per, c.seqs);
   auto units = [&](int s) -> int64_t {
@@ -89,8 +92,9 @@ __device__ __forceinline__ bool start_walk(const PagedCache& c, const AttnWork& 
   total = uniform(total);
   const int64_t most = total / w.min_units;
   const int active = most < 1 ? 1 : most < (int64_t)gridDim.x ? (int)most : (int)gridDim.x;
-  if ((int)blockIdx.x >= active || total == 0) return false;
-  const int64_t at = share_of(total, active, (int)blockIdx.x), end = share_of(total, active, (int)blockIdx.x + 1);
+  wg = by_xcd && active == (int)gridDim.x ? xcd_remap((int)blockIdx.x, active) : (int)blockIdx.x;
+  if (wg >= active || total == 0) return false;
+  const int64_t at = share_of(total, active, wg), end = share_of(total, active, wg + 1);
   // The thread whose sequences hold `at` looks for the one that does.
   if (before <= at && at < before + mine) {
     int s = s0;
@@ -148,6 +152,14 @@ template <typename T> constexpr unsigned short kInfBits = 0;
 template <> constexpr unsigned short kInfBits<f16> = 0x7c00;
 template <> constexpr unsigned short kInfBits<bf16> = 0x7f80;
 
+// c plus a pair of 16-bit values.
+__device__ __forceinline__ float add_pair(unsigned x, float c, f16*) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), f16x2{(f16)1.f, (f16)1.f}, c, false);
+}
+__device__ __forceinline__ float add_pair(unsigned x, float c, bf16*) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), bf16x2{(bf16)1.f, (bf16)1.f}, c, false);
+}
+
 // x over the lanes of equal lane % 16.
 __device__ __forceinline__ float groups_max(float x) { x = fmaxf(x, partner16(x)); return fmaxf(x, partner32(x)); }
 __device__ __forceinline__ float groups_sum(float x) { x += partner16(x); return x + partner32(x); }
@@ -190,7 +202,8 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 
   PartRecord rec = {0, 0, 0, 0};
   WorkWalk walk;
-  const bool active = start_walk<256>(c, w, walk_lds, walk);
+  int wg;
+  const bool active = start_walk<256>(c, w, false, walk_lds, wg, walk);
   Segment sg;
   unsigned char* vw = v_lds[wave];
   // Swizzled 16-byte chunk of a V row: the 8 rows x 2 chunks that 32 lanes of a transposing read touch lie in
@@ -476,11 +489,11 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
           for (int e = 0; e < EL; ++e) y[e] = from_f32<T>(sum == 0.f ? 0.f : x[e] / sum);
           *reinterpret_cast<TE*>(static_cast<T*>(a.o) + (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head + part * EL) = y;
         } else {
-          float* to = part_rows(w, (int)blockIdx.x, slot, ROWS, D) + (16 * b + q) * D + part * EL;
+          float* to = part_rows(w, wg, slot, ROWS, D) + (16 * b + q) * D + part * EL;
 #pragma unroll
           for (int e = 0; e < EL; e += 4) *reinterpret_cast<f32x4*>(to + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
           if (part == 0) {
-            float* st = part_stats(w, (int)gridDim.x, (int)blockIdx.x, slot, ROWS, D);
+            float* st = part_stats(w, (int)gridDim.x, wg, slot, ROWS, D);
             st[16 * b + q] = mx, st[ROWS + 16 * b + q] = sum;
           }
         }
@@ -488,7 +501,447 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       __syncthreads();
     }
   }
-  if (tid == 0) w.records[blockIdx.x] = rec;
+  if (tid == 0) w.records[wg] = rec;
+}
+
+// ---- Many rows a tile: chunks of prompts ----
+//
+// A tile has BM rows, 32 for each wave; its keys go past in tiles of 64 that all waves share in LDS, and what
+// bounds the kernel is the matrix core beside the exponentials. Both products as in fa_mfma.hpp, transposed on
+// 32x32x16 MFMAs with a query per lane, and its two-stage pipeline: while tile t's scores become P(t) the
+// matrix core takes S(t+1), and while it takes O += V(t) P(t) the scores of t+1 get their row maxima. K(t+2)
+// and V(t+1) arrive meanwhile: 16-bit rows straight into LDS from 64-bit addresses, a row per page lookup;
+// 8-bit rows through registers, widened to 16 bits (exact) once for all waves. A key's scale multiplies its
+// scores, a value's scale its P before the one rounding of P to the type.
+// O and l are rescaled only when some row's maximum outgrew its reference by more than 2^8.
+// A value that is not finite must not reach rows that do not see it: a wave looks at the values of a tile that
+// some row sees and another does not, leaves a tile with such a value out of P . V, and adds it at the end in
+// fp32 over the visible pairs.
+__device__ __attribute__((aligned(16))) const unsigned char kZeroChunk[16] = {};
+
+constexpr int chunk_rows_of(int d) { return d == 128 ? 256 : 128; }
+constexpr int chunk_wgs(int d) { return d == 128 ? 1 : 2; }   // workgroups on a CU
+
+template <typename T, typename C, int D, int BM>
+__global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(2)))
+paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
+  typedef typename vec8<T>::type V8;
+  constexpr bool k8 = cache_type<C>::k8bit;
+  constexpr bool kUnits = k8 && std::is_same<T, f16>::value;   // O in units of the largest value scale so far
+  constexpr int BN = 64, THREADS = BM * 2, RB = D * 2, CB = k8 ? D : 2 * D, CR = D / 8;
+  constexpr int TILE_BYTES = BN * RB;
+  constexpr int QK_STEPS = D / 16, NKB = BN / 32, NDB = D / 32, PV_STEPS = BN / 16;
+  constexpr int CPT = BN * CB / 16 / THREADS;   // 16-byte loads per thread, matrix and tile
+  constexpr int LPR = CB / 16;                  // lanes a cache row
+  static_assert(CPT * THREADS * 16 == BN * CB, "a tile's loads split evenly");
+  constexpr float kLazyLog2 = 8.f;
+  __shared__ __attribute__((aligned(1024))) unsigned char k_lds0[TILE_BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char v_lds0[TILE_BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char k_lds1[TILE_BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char v_lds1[TILE_BYTES];
+  __shared__ __attribute__((aligned(16))) float ks_lds[2][BN], vs_lds[2][BN], top_lds[2];
+  __shared__ int64_t walk_lds[10];
+  const std::integral_constant<int, 0> even{};
+  const std::integral_constant<int, 1> odd{};
+  auto k_stage = [&](auto par) -> unsigned char* { if constexpr (decltype(par)::value) return k_lds1; else return k_lds0; };
+  auto v_stage = [&](auto par) -> unsigned char* { if constexpr (decltype(par)::value) return v_lds1; else return v_lds0; };
+  const int tid = (int)threadIdx.x, wave = uniform(tid / kWave), lane = tid % kWave;
+  const int lq = lane % 32, hi = lane / 32, g16 = lane / 16, i16 = lane % 16;
+
+  // Operand read addresses (fa_mfma.hpp): K row lq, chunk 2 kk + hi; V^T by transposing reads.
+  // The swizzles reach chunk bits that the step and the dim block do not, so those enter by XOR.
+  const int v_row = hi * 4 + i16 / 4, v_cl = 2 * (g16 % 2) + (i16 % 4) / 2;
+  int k_base = lq * RB + ((hi ^ k_swz<CR>(lq)) * 16), v_base = v_row * RB + ((v_cl ^ v_swz<CR>(v_row)) * 16) + 8 * (i16 % 2);
+  PartRecord rec = {0, 0, 0, 0};
+  WorkWalk walk;
+  int wg;
+  const bool active = start_walk<THREADS>(c, w, true, walk_lds, wg, walk);
+  Segment sg;
+  while (active && uniform((int)walk.next([&](int s) { return uniform(load_seq(c, s)); }, sg)) != 0) {
+    sg = {uniform(sg.rows), uniform(sg.seq), uniform(sg.head), uniform(sg.tile), uniform(sg.from), uniform(sg.to), uniform(sg.steps)};
+    const int kv_head = sg.head / w.tiles.splits;
+    int token, hq;
+    const bool mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, 32 * wave + lq, token, hq);
+    const int seen = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
+    V8 qf[QK_STEPS];
+    {
+      const T* qp = static_cast<const T*>(a.q) + (mine ? (int64_t)(sg.rows.first + token) * a.q_token + hq * a.q_head : 0) + 8 * hi;
+#pragma unroll
+      for (int kk = 0; kk < QK_STEPS; ++kk) {
+        const u32x4 x = mine ? *reinterpret_cast<const u32x4*>(qp + 16 * kk) : u32x4{0, 0, 0, 0};
+        qf[kk] = __builtin_bit_cast(V8, x);
+      }
+    }
+    // Keys that all of the wave's rows see, and that some row does (none: the wave has no rows).
+    int lo = mine ? seen : INT32_MAX, up = seen;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) lo = min(lo, __shfl_xor(lo, d)), up = max(up, __shfl_xor(up, d));
+    const int wave_all = uniform(lo), wave_any = uniform(up);
+    // Keys of the segment's tile: up to the last row's.
+    const int last_token = min((sg.tile + 1) * w.tiles.tokens, sg.rows.count) - 1;
+    const int key_begin = sg.from * kStep;
+    const int key_end = min(sg.to * kStep, keys_seen(sg.rows, last_token, c.capacity, w.causal));
+    const int nt = max(1, (key_end - key_begin + BN - 1) / BN);
+
+    // ---- tiles of keys: lane l looks up key l; each thread's chunk rows come from there by lane
+    const int* table = c.table + sg.seq * c.table_stride;
+    auto load_page = [&](int t) { return table[page_of((uint32_t)min(key_begin + t * BN + lane, c.capacity - 1), c.div)]; };
+    auto find_row = [&](int t, int page) {
+      const int key = key_begin + t * BN + lane;
+      const uint32_t at = ((uint32_t)page * c.heads + kv_head) * c.page_size + (key - page_of((uint32_t)key, c.div) * c.page_size);
+      return key < key_end && (unsigned)page < (unsigned)c.pages ? (int)at : -1;
+    };
+    // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row.
+    auto to_lds = [&](const void* cache, const int (&rows)[CPT], unsigned char* stage, bool is_v) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        const int slot = i * THREADS + tid, r = slot / CR, pc = slot % CR;
+        const int off = (pc ^ (is_v ? v_swz<CR>(r) : k_swz<CR>(r))) * 16;
+        const unsigned char* p = rows[i] < 0 ? kZeroChunk : static_cast<const unsigned char*>(cache) + (int64_t)rows[i] * CB + off;
+        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)p,
+                                         (__attribute__((address_space(3))) void*)(stage + (i * THREADS + wave * kWave) * 16), 16, 0, 0);
+      }
+    };
+    // 8-bit rows: load, then widen and store.
+    auto to_regs = [&](const void* cache, const int (&rows)[CPT], u32x4 (&x)[CPT]) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        const unsigned char* p = rows[i] < 0 ? kZeroChunk
+                                             : static_cast<const unsigned char*>(cache) + (int64_t)rows[i] * CB + (i * THREADS + tid) % LPR * 16;
+        x[i] = *reinterpret_cast<const u32x4*>(p);
+      }
+    };
+    auto widen = [&](const u32x4 (&x)[CPT], unsigned char* stage, bool is_v) {
+      if constexpr (k8)
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        const int r = (i * THREADS + tid) / LPR, ch = (i * THREADS + tid) % LPR * 2;
+        const int sw = is_v ? v_swz<CR>(r) : k_swz<CR>(r);
+        u32x4 lo16, hi16;
+        widen16<C, T>(x[i], lo16, hi16);
+        *reinterpret_cast<u32x4*>(stage + r * RB + ((ch ^ sw) * 16)) = lo16;
+        *reinterpret_cast<u32x4*>(stage + r * RB + (((ch + 1) ^ sw) * 16)) = hi16;
+      }
+    };
+    auto chunk_rows = [&](int row, int (&rows)[CPT]) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) rows[i] = __shfl(row, (i * THREADS + tid) / LPR);
+    };
+    // A tile's scales by lane = key (wave 0 the keys', wave 1 the values').
+    auto load_scale = [&](const float* scales, int row) { return scales[max(row, 0)]; };
+    auto store_v_scale = [&](int par, int row, float x) {
+      if (wave == 1) {
+        vs_lds[par][lane] = row >= 0 ? x : 0.f;
+        if constexpr (kUnits) {
+          const float top = wave_allreduce(row >= 0 && fabsf(x) < INFINITY ? fabsf(x) : 0.f, MaxOp{});
+          if (lane == 0) top_lds[par] = top;
+        }
+      }
+    };
+
+    // The wave's first tile that is not clean and has a value that is not finite: from there on, tiles that are
+    // not clean leave P . V out, and take_visible adds it at the end.
+    int skip_from = INT32_MAX;
+    float m_run = -INFINITY, vref = 1e-30f, l = 0.f;
+    f32x16 o[NDB];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[db] = f32x16{};
+
+    auto qk = [&](f32x16 (&s)[NKB], const unsigned char* ks) {
+#pragma unroll
+      for (int b = 0; b < NKB; ++b) s[b] = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < QK_STEPS; ++kk)
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+          s[b] = mfma32x32x16(*reinterpret_cast<const V8*>(ks + b * 32 * RB + (k_base ^ (32 * kk))), qf[kk], s[b]);
+    };
+    // Keys' scales (8 bits; with log2(e)/sqrt(d), so that scores are in the exponent's units).
+    auto scale_scores = [&](f32x16 (&s)[NKB], int par) {
+      if constexpr (k8)
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&ks_lds[par][32 * b + 8 * q4 + 4 * hi]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[b][4 * q4 + r] *= x[r];
+          }
+    };
+    // Keys of a tile that this lane's row sees, as bits: 32-key block b, bit 8 (r / 4) + r % 4 for the key of
+    // register r (the lane's keys begin 4 hi further on).
+    struct Bits { unsigned b[NKB]; };
+    auto visible = [&](int t, uint64_t present) {
+      Bits v;
+#pragma unroll
+      for (int b = 0; b < NKB; ++b) {
+        const int n = clamp_int(seen - (key_begin + t * BN + 32 * b), 0, 32);
+        const unsigned below = n == 32 ? ~0u : (1u << n) - 1;
+        v.b[b] = ((unsigned)(present >> (32 * b)) & below) >> (4 * hi);
+      }
+      return v;
+    };
+    auto mask = [&](f32x16 (&s)[NKB], int t, uint64_t present) {
+      const Bits v = visible(t, present);
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = v.b[b] & 1u << (8 * (r / 4) + r % 4) ? s[b][r] : -INFINITY;
+    };
+    auto row_max = [&](const f32x16 (&s)[NKB]) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+      return half_max(mx) * (k8 ? 1.f : w.scale_log2);
+    };
+    auto raise = [&](float mx) {   // the reference maximum, where some row's grew past 2^8
+      const float m_new = fmaxf(m_run, mx);
+      if (__builtin_amdgcn_ballot_w64(m_new > m_run + kLazyLog2) != 0) {
+        const float f = m_new > m_run ? exp2_fast(m_run - m_new) : 1.f;   // (m_run = -inf: 0)
+        m_run = m_new;
+        l *= f;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[db] *= f;
+      }
+    };
+    auto exponentiate = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int par, bool clean, int t, uint64_t present) {
+      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+      const float unit = kUnits ? 1.f / vref : 1.f;
+      Bits v;
+      if constexpr (k8) v = clean ? Bits{~0u, ~0u} : visible(t, present);
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          f32x4 x;
+          if constexpr (k8) x = *reinterpret_cast<const f32x4*>(&vs_lds[par][32 * b + 8 * q4 + 4 * hi]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float p = exp2_fast(k8 ? s[b][4 * q4 + r] + neg_m : fmaf(s[b][4 * q4 + r], w.scale_log2, neg_m));
+            if constexpr (k8) {
+              l += p;
+              p *= kUnits ? x[r] * unit : x[r];
+              if (!clean) p = v.b[b] & 1u << (8 * q4 + r) ? p : 0.f;   // (0 x a scale that is not finite)
+            }
+            pf[b * 2 + q4 / 2][(q4 % 2) * 4 + r] = from_f32<T>(p);
+          }
+        }
+    };
+    auto pv = [&](const V8 (&pf)[PV_STEPS], const unsigned char* vs) {
+#pragma unroll
+      for (int i = 0; i < PV_STEPS; ++i)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const unsigned char* p0 = vs + i * 16 * RB + (v_base ^ (64 * db));
+          const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p0));
+          const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p0 + 8 * RB));
+          const i16x8 x = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+          o[db] = mfma32x32x16(__builtin_bit_cast(V8, x), pf[i], o[db]);
+        }
+    };
+    // l of the lane's keys from the rounded P (8 bits: from P before its scale, in exponentiate). Not by a product
+    // with a constant operand: its zeros would carry one row's NaN into another's sum.
+    auto row_sum = [&](const V8 (&pf)[PV_STEPS]) {
+      if constexpr (!k8)
+#pragma unroll
+        for (int i = 0; i < PV_STEPS; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) l = add_pair(__builtin_bit_cast(u32x4, pf[i])[j], l, static_cast<T*>(nullptr));
+    };
+    // Whether the tile's values in LDS are all finite.
+    auto values_finite = [&](const unsigned char* vs) {
+      u16x2 top = {0, 0};
+#pragma unroll 4
+      for (int i = 0; i < TILE_BYTES / 16 / kWave; ++i) top = max_bits(top, *reinterpret_cast<const u32x4*>(vs + (i * kWave + lane) * 16));
+      return __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= kInfBits<T>) == 0;
+    };
+    // ---- the first tiles: K(0), V(0), K(1)
+    int page = load_page(0), page1 = load_page(1);
+    int row = find_row(0, page), row1 = find_row(1, page1);
+    page = load_page(2);
+    uint64_t present = __builtin_amdgcn_ballot_w64(row >= 0), present1 = __builtin_amdgcn_ballot_w64(row1 >= 0);
+    int rows[CPT], rows1[CPT];
+    chunk_rows(row, rows);
+    chunk_rows(row1, rows1);
+    u32x4 kx[CPT], vx[CPT];
+    float ksx = 0.f, vsx = 0.f;
+    if constexpr (k8) {
+      u32x4 k1[CPT];
+      to_regs(c.k, rows, kx);
+      to_regs(c.v, rows, vx);
+      to_regs(c.k, rows1, k1);
+      if (wave == 0) ks_lds[0][lane] = load_scale(c.k_scale, row) * w.scale_log2, ks_lds[1][lane] = load_scale(c.k_scale, row1) * w.scale_log2;
+      store_v_scale(0, row, load_scale(c.v_scale, row));
+      widen(kx, k_stage(even), false);
+      widen(vx, v_stage(even), true);
+      widen(k1, k_stage(odd), false);
+    } else {
+      to_lds(c.k, rows, k_stage(even), false);
+      to_lds(c.v, rows, v_stage(even), true);
+      to_lds(c.k, rows1, k_stage(odd), false);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    f32x16 sa[NKB], sb[NKB];
+    const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
+    auto is_clean = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= wave_all; };
+    if (wave_tiles > 0) {
+      qk(sa, k_stage(even));
+      scale_scores(sa, 0);
+      if (!is_clean(0, present)) mask(sa, 0, present);
+      raise(row_max(sa));
+    }
+    __syncthreads();   // iteration 0 replaces K(0)
+
+    auto iteration = [&](auto par, int t, f32x16 (&s)[NKB], f32x16 (&sn)[NKB]) {
+      constexpr int P = decltype(par)::value;
+      const std::integral_constant<int, P> cur{};
+      const std::integral_constant<int, 1 - P> nxt{};
+      // Loads: K(t+2) over K(t), V(t+1) over V(t-1).
+      const int row2 = find_row(t + 2, page);
+      const uint64_t present2 = __builtin_amdgcn_ballot_w64(row2 >= 0);
+      page = load_page(t + 3);
+      int rows2[CPT];
+      chunk_rows(row2, rows2);
+      if (t + 1 < nt) {
+        if constexpr (k8) {
+          to_regs(c.k, rows2, kx);
+          to_regs(c.v, rows1, vx);
+          if (wave == 0) ksx = load_scale(c.k_scale, row2);
+          if (wave == 1) vsx = load_scale(c.v_scale, row1);
+        } else {
+          to_lds(c.k, rows2, k_stage(cur), false);
+          to_lds(c.v, rows1, v_stage(nxt), true);
+        }
+      }
+      if (t < wave_tiles) {
+        V8 pf[PV_STEPS];
+        const bool clean = is_clean(t, present);
+        if constexpr (kUnits) {
+          const float top = uniform_f(top_lds[P]);
+          if (top > vref) {
+            const float f = vref / top;
+            vref = top;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) o[db] *= f;
+          }
+        }
+        // Phase A: S(t+1) with P(t). (Past the last tile the product is of what the stage holds, and unused.)
+        __builtin_amdgcn_s_setprio(2);
+        qk(sn, k_stage(nxt));
+        exponentiate(s, pf, P, clean, t, present);
+        __builtin_amdgcn_s_setprio(0);
+        const bool more = t + 1 < wave_tiles;
+        if (more) {
+          scale_scores(sn, 1 - P);
+          if (!is_clean(t + 1, present1)) mask(sn, t + 1, present1);
+        }
+        // Phase B: O += V(t) P(t) with the row maxima of S(t+1).
+        if (!clean && skip_from == INT32_MAX && !values_finite(v_stage(cur))) skip_from = t;
+        if (clean || skip_from == INT32_MAX) pv(pf, v_stage(cur));
+        row_sum(pf);
+        if (more) raise(row_max(sn));
+      }
+      if constexpr (k8) {
+        if (t + 1 < nt) {
+          widen(kx, k_stage(cur), false);
+          widen(vx, v_stage(nxt), true);
+          if (wave == 0) ks_lds[P][lane] = row2 >= 0 ? ksx * w.scale_log2 : 0.f;
+          store_v_scale(1 - P, row1, vsx);
+        }
+      }
+      present = present1, present1 = present2, row1 = row2;
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) rows1[i] = rows2[i];
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    };
+    for (int t = 0; t < nt; t += 2) {
+      iteration(even, t, sa, sb);
+      if (t + 1 < nt) iteration(odd, t + 1, sb, sa);
+    }
+
+    // ---- P . V of the tiles left out, over the visible pairs alone: scores again, all in fp32
+    if (skip_from < wave_tiles) {
+#pragma unroll 1
+      for (int t = skip_from; t < wave_tiles; ++t) {
+        const int row_t = find_row(t, load_page(t));
+        const uint64_t present_t = __builtin_amdgcn_ballot_w64(row_t >= 0);
+        if (is_clean(t, present_t)) continue;
+#pragma unroll 1
+        for (int k = 0; k < BN; ++k) {
+          if (!(present_t >> k & 1)) continue;
+          const int at = __builtin_amdgcn_readlane(row_t, k);
+          const bool vis = key_begin + t * BN + k < seen;
+          float dot = 0.f, x[8], ks = 1.f, vs = 1.f;
+          if constexpr (k8) ks = c.k_scale[at], vs = c.v_scale[at];
+#pragma unroll
+          for (int kk = 0; kk < QK_STEPS; ++kk) {
+            cached8(static_cast<const C*>(c.k) + (int64_t)at * D, 16 * kk + 8 * hi, 1.f, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dot = fmaf(to_f32(qf[kk][j]), x[j], dot);
+          }
+          dot += partner32(dot);
+          float p = exp2_fast(fmaf(dot, ks * w.scale_log2, m_run == -INFINITY ? 0.f : -m_run));
+          p = vis ? p * (kUnits ? vs / vref : vs) : 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            cached8(static_cast<const C*>(c.v) + (int64_t)at * D, 8 * i, 1.f, x);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float y = hi ? x[4 + r] : x[r];
+              o[i / 4][i % 4 * 4 + r] = fmaf(p, vis ? y : 0.f, o[i / 4][i % 4 * 4 + r]);
+            }
+          }
+        }
+      }
+    }
+
+    // ---- the wave's 32 rows: done, or a part for the join. (The stages are free: every wave passed the last barrier.)
+    const bool done = sg.from == 0 && sg.to == sg.steps;
+    const int slot = sg.from == 0 ? 1 : 0;
+    if (!done) {
+      if (sg.from == 0) rec = {sg.seq, sg.head, sg.tile, rec.flags | kPartBegins};
+      else rec.flags |= kPartContinues | (sg.to == sg.steps ? kPartEnds : 0);
+    }
+    const float sum = half_sum(l);
+    if (mine) {
+      if (done) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T* to = static_cast<T*>(a.o) + (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head + 4 * hi;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            T4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = from_f32<T>(sum == 0.f ? 0.f : o[db][4 * q4 + r] * (kUnits ? inv * vref : inv));
+            *reinterpret_cast<T4*>(to + 32 * db + 8 * q4) = x;
+          }
+      } else {
+        const int r = 32 * wave + lq;
+        float* to = part_rows(w, wg, slot, BM, D) + r * D + 4 * hi;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = kUnits ? o[db][4 * q4 + e] * vref : o[db][4 * q4 + e];
+            *reinterpret_cast<f32x4*>(to + 32 * db + 8 * q4) = x;
+          }
+        if (hi == 0) {
+          float* st = part_stats(w, (int)gridDim.x, wg, slot, BM, D);
+          st[r] = m_run == -INFINITY && sum != 0.f ? 0.f : m_run, st[BM + r] = sum;
+        }
+      }
+    }
+    __syncthreads();   // the next segment's loads replace the stages
+  }
+  if (tid == 0) w.records[wg] = rec;
 }
 
 // Joins the parts of the tile that workgroup blockIdx.x of the attention kernel began and did not end: its own

@@ -80,37 +80,38 @@ hipError_t with_types(int dtype, int cache_dtype, int64_t d, F f) {
 
 constexpr int kCUs = 256;   // MI355X / gfx950
 
-// The launch of an attention call: tiles of 16 * nb rows, workgroups, and whether tiles are cut.
+// The launch of an attention call: rows of a tile, workgroups, and whether tiles are cut.
 struct AttnPlan {
-  int nb, wgs;
+  int rows, wgs;
   bool whole;
 };
 // A cache of at most so many positions a sequence is read in a few steps: its tiles are not cut over workgroups,
 // which saves the second launch that joins them.
 constexpr int kWholeCapacity = 256;
-AttnPlan attn_plan(const pa::PagedCache& c, int64_t heads_q, int64_t max_new) {
+AttnPlan attn_plan(const pa::PagedCache& c, int64_t d, int64_t heads_q, int64_t max_new) {
   const int64_t group = heads_q / c.heads;
   const int64_t new_tokens = !c.cu ? c.per_seq : max_new > 0 ? std::min<int64_t>(max_new, c.tokens) : c.tokens;
-  const int64_t rows = new_tokens * group;
-  const int nb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t most = new_tokens * group;   // rows of a sequence and key/value head
+  const int rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : pa::chunk_rows_of((int)d);
   // As many workgroups as are resident at once, or fewer where the work's bound is below their least share.
-  const pa::TileShape t = pa::make_tiles((int)group, 16 * nb);
+  const pa::TileShape t = pa::make_tiles((int)group, rows);
   const double tiles = (double)c.tokens / t.tokens + c.seqs;
   const double units = tiles * c.heads * t.splits * ((double)pa::kTileCost + c.capacity);
-  const int resident = kCUs * pa::few_waves(nb);
+  const int resident = kCUs * (rows > 64 ? pa::chunk_wgs((int)d) : pa::few_waves(rows / 16));
   const int wgs = (int)std::max(1.0, std::min<double>(resident, units / pa::kMinUnits + 1));
-  return {nb, wgs, c.capacity <= kWholeCapacity};
+  return {rows, wgs, c.capacity <= kWholeCapacity};
 }
 
-template <typename T, typename C, int D, int NB>
-hipError_t launch_few(const pa::PagedCache& c, const pa::RowsQ& a, const AttnPlan& plan, int causal, void* workspace,
-                      hipStream_t stream) {
-  const pa::AttnWork w{pa::make_tiles(a.group, 16 * NB), pa::kMinUnits, plan.whole, causal, pa::kLog2e / sqrtf((float)D),
+template <typename T, int D, int ROWS, typename Kernel>
+hipError_t launch_attn(Kernel kernel, int threads, const pa::PagedCache& c, const pa::RowsQ& a, const AttnPlan& plan,
+                       int causal, void* workspace, hipStream_t stream) {
+  const pa::AttnWork w{pa::make_tiles(a.group, ROWS), pa::kMinUnits, plan.whole, causal, pa::kLog2e / sqrtf((float)D),
                        static_cast<pa::PartRecord*>(workspace),
                        reinterpret_cast<float*>(static_cast<char*>(workspace) + pa::attn_record_bytes(plan.wgs))};
-  hipLaunchKernelGGL((pa::paged_attn_few<T, C, D, NB>), dim3((unsigned)plan.wgs), dim3(256), 0, stream, c, a, w);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)plan.wgs), dim3(threads), 0, stream, c, a, w);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || plan.whole) return e;
-  hipLaunchKernelGGL((pa::paged_attn_join<T, D, 16 * NB>), dim3((unsigned)plan.wgs, NB), dim3(256), 0, stream, c, a, w, plan.wgs);
+  hipLaunchKernelGGL((pa::paged_attn_join<T, D, ROWS>), dim3((unsigned)plan.wgs, ROWS > 64 ? ROWS / 32 : ROWS / 16), dim3(256), 0,
+                     stream, c, a, w, plan.wgs);
   return hipGetLastError();
 }
 
@@ -180,8 +181,8 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
   if (!apart(o_token_stride, tokens, o_head_stride, heads_q) && !apart(o_head_stride, heads_q, o_token_stride, tokens))
     return fail(PA_ERR_INVALID, "%s: out's rows must not overlap", name);
   if (max_new < 0) return fail(PA_ERR_INVALID, "%s: max_new must not be negative", name);
-  const AttnPlan plan = attn_plan(c, heads_q, max_new);
-  if (workspace_bytes < pa::attn_workspace(plan.wgs, 16 * plan.nb, (int)cache->d) || !workspace || !aligned16(workspace))
+  const AttnPlan plan = attn_plan(c, cache->d, heads_q, max_new);
+  if (workspace_bytes < pa::attn_workspace(plan.wgs, plan.rows, (int)cache->d) || !workspace || !aligned16(workspace))
     return fail(PA_ERR_INVALID, "%s: the workspace is too small, null or not 16-byte aligned", name);
   const pa::RowsQ a{q, o, q_token_stride, q_head_stride, o_token_stride, o_head_stride, (int)(heads_q / cache->heads),
                     (int)heads_q};
@@ -190,9 +191,13 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
     typedef decltype(t) T;
     typedef decltype(ct) C;
     constexpr int D = decltype(dim)::value;
-    return plan.nb == 1 ? launch_few<T, C, D, 1>(c, a, plan, causal, workspace, st)
-         : plan.nb == 2 ? launch_few<T, C, D, 2>(c, a, plan, causal, workspace, st)
-                        : launch_few<T, C, D, 4>(c, a, plan, causal, workspace, st);
+    constexpr int CR = pa::chunk_rows_of(D);
+    switch (plan.rows) {
+      case 16: return launch_attn<T, D, 16>(pa::paged_attn_few<T, C, D, 1>, 256, c, a, plan, causal, workspace, st);
+      case 32: return launch_attn<T, D, 32>(pa::paged_attn_few<T, C, D, 2>, 256, c, a, plan, causal, workspace, st);
+      case 64: return launch_attn<T, D, 64>(pa::paged_attn_few<T, C, D, 4>, 256, c, a, plan, causal, workspace, st);
+      default: return launch_attn<T, D, CR>(pa::paged_attn_chunk<T, C, D, CR>, 2 * CR, c, a, plan, causal, workspace, st);
+    }
   });
   return hip_status(e, name);
 }
@@ -205,8 +210,8 @@ int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t 
   if (int rc = check_tokens(name, tokens, cu_seqlens, &c)) return rc;
   if (heads_q <= 0 || heads_q > (1 << 16) || heads_q % cache->heads != 0 || max_new < 0)
     return fail(PA_ERR_INVALID, "%s: the query heads must be a multiple of the cache's heads, max_new not negative", name);
-  const AttnPlan plan = attn_plan(c, heads_q, max_new);
-  return pa::attn_workspace(plan.wgs, 16 * plan.nb, (int)cache->d);
+  const AttnPlan plan = attn_plan(c, cache->d, heads_q, max_new);
+  return pa::attn_workspace(plan.wgs, plan.rows, (int)cache->d);
 }
 
 }  // extern "C"
