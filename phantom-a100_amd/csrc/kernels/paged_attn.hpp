@@ -706,25 +706,29 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         for (int db = 0; db < NDB; ++db) o[db] *= f;
       }
     };
-    auto exponentiate = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int par, bool clean, int t, uint64_t present) {
+    auto exponentiate = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS]) {
+      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) pf[b * 2 + r / 8][r % 8] = from_f32<T>(exp2_fast(fmaf(s[b][r], w.scale_log2, neg_m)));
+    };
+    // 8 bits: l takes P, the product P times the values' scales.
+    auto exponentiate8 = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int par, bool clean, int t, uint64_t present) {
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
       const float unit = kUnits ? 1.f / vref : 1.f;
-      Bits v;
-      if constexpr (k8) v = clean ? Bits{~0u, ~0u} : visible(t, present);
+      const Bits v = clean ? Bits{{~0u, ~0u}} : visible(t, present);
 #pragma unroll
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          f32x4 x;
-          if constexpr (k8) x = *reinterpret_cast<const f32x4*>(&vs_lds[par][32 * b + 8 * q4 + 4 * hi]);
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&vs_lds[par][32 * b + 8 * q4 + 4 * hi]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float p = exp2_fast(k8 ? s[b][4 * q4 + r] + neg_m : fmaf(s[b][4 * q4 + r], w.scale_log2, neg_m));
-            if constexpr (k8) {
-              l += p;
-              p *= kUnits ? x[r] * unit : x[r];
-              if (!clean) p = v.b[b] & 1u << (8 * q4 + r) ? p : 0.f;   // (0 x a scale that is not finite)
-            }
+            float p = exp2_fast(s[b][4 * q4 + r] + neg_m);
+            l += p;
+            p *= kUnits ? x[r] * unit : x[r];
+            if (!clean) p = v.b[b] & 1u << (8 * q4 + r) ? p : 0.f;   // (0 x a scale that is not finite)
             pf[b * 2 + q4 / 2][(q4 % 2) * 4 + r] = from_f32<T>(p);
           }
         }
@@ -741,14 +745,13 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           o[db] = mfma32x32x16(__builtin_bit_cast(V8, x), pf[i], o[db]);
         }
     };
-    // l of the lane's keys from the rounded P (8 bits: from P before its scale, in exponentiate). Not by a product
+    // l of the lane's keys from the rounded P. Not by a product
     // with a constant operand: its zeros would carry one row's NaN into another's sum.
     auto row_sum = [&](const V8 (&pf)[PV_STEPS]) {
-      if constexpr (!k8)
 #pragma unroll
-        for (int i = 0; i < PV_STEPS; ++i)
+      for (int i = 0; i < PV_STEPS; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) l = add_pair(__builtin_bit_cast(u32x4, pf[i])[j], l, static_cast<T*>(nullptr));
+        for (int j = 0; j < 4; ++j) l = add_pair(__builtin_bit_cast(u32x4, pf[i])[j], l, static_cast<T*>(nullptr));
     };
     // Whether the tile's values in LDS are all finite.
     auto values_finite = [&](const unsigned char* vs) {
@@ -766,17 +769,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     chunk_rows(row, rows);
     chunk_rows(row1, rows1);
     u32x4 kx[CPT], vx[CPT];
-    float ksx = 0.f, vsx = 0.f;
+    float scale_x = 0.f;
     if constexpr (k8) {
-      u32x4 k1[CPT];
       to_regs(c.k, rows, kx);
       to_regs(c.v, rows, vx);
-      to_regs(c.k, rows1, k1);
-      if (wave == 0) ks_lds[0][lane] = load_scale(c.k_scale, row) * w.scale_log2, ks_lds[1][lane] = load_scale(c.k_scale, row1) * w.scale_log2;
-      store_v_scale(0, row, load_scale(c.v_scale, row));
+      if (wave == 0) ks_lds[0][lane] = row >= 0 ? load_scale(c.k_scale, row) * w.scale_log2 : 0.f;
+      if (wave == 1) store_v_scale(0, row, load_scale(c.v_scale, row));
       widen(kx, k_stage(even), false);
       widen(vx, v_stage(even), true);
-      widen(k1, k_stage(odd), false);
     } else {
       to_lds(c.k, rows, k_stage(even), false);
       to_lds(c.v, rows, v_stage(even), true);
@@ -787,13 +787,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     f32x16 sa[NKB], sb[NKB];
     const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
     auto is_clean = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= wave_all; };
-    if (wave_tiles > 0) {
-      qk(sa, k_stage(even));
-      scale_scores(sa, 0);
-      if (!is_clean(0, present)) mask(sa, 0, present);
-      raise(row_max(sa));
+    if constexpr (!k8) {
+      if (wave_tiles > 0) {
+        qk(sa, k_stage(even));
+        if (!is_clean(0, present)) mask(sa, 0, present);
+        raise(row_max(sa));
+      }
+      __syncthreads();   // iteration 0 replaces K(0)
     }
-    __syncthreads();   // iteration 0 replaces K(0)
 
     auto iteration = [&](auto par, int t, f32x16 (&s)[NKB], f32x16 (&sn)[NKB]) {
       constexpr int P = decltype(par)::value;
@@ -806,19 +807,80 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       int rows2[CPT];
       chunk_rows(row2, rows2);
       if (t + 1 < nt) {
-        if constexpr (k8) {
-          to_regs(c.k, rows2, kx);
-          to_regs(c.v, rows1, vx);
-          if (wave == 0) ksx = load_scale(c.k_scale, row2);
-          if (wave == 1) vsx = load_scale(c.v_scale, row1);
-        } else {
-          to_lds(c.k, rows2, k_stage(cur), false);
-          to_lds(c.v, rows1, v_stage(nxt), true);
-        }
+        to_lds(c.k, rows2, k_stage(cur), false);
+        to_lds(c.v, rows1, v_stage(nxt), true);
       }
       if (t < wave_tiles) {
         V8 pf[PV_STEPS];
+        const bool clean = is_clean(t, present), more = t + 1 < wave_tiles;
+        // Phase A: S(t+1) with P(t). (Past the wave's last tile the product is of what the stage holds, and unused.)
+        __builtin_amdgcn_s_setprio(2);
+        qk(sn, k_stage(nxt));
+        exponentiate(s, pf);
+#pragma unroll
+        for (int i = 0; i < PV_STEPS; ++i) asm volatile("" : "+v"(pf[i]));   // (not to be moved past the branches below)
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
+#pragma unroll
+        for (int i = 0; i < NKB * QK_STEPS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedValu, 96 / (NKB * QK_STEPS), 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
+        if (more && !is_clean(t + 1, present1)) mask(sn, t + 1, present1);
+        if (!clean && skip_from == INT32_MAX && !values_finite(v_stage(cur))) skip_from = t;
+        // Phase B: O += V(t) P(t) with the row sums of P(t) and the row maxima of S(t+1).
+        float mx;
+        if (clean || skip_from == INT32_MAX) {
+          pv(pf, v_stage(cur));
+          row_sum(pf);
+          mx = row_max(sn);
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 4, 0);
+#pragma unroll
+          for (int i = 0; i < PV_STEPS * NDB; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedValu, 48 / (PV_STEPS * NDB), 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        } else {
+          row_sum(pf);
+          mx = row_max(sn);
+        }
+        if (!more) mx = -INFINITY;
+        raise(mx);
+      }
+      present = present1, present1 = present2;
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) rows1[i] = rows2[i];
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    };
+    // 8 bits: K(t+1) and V(t+1) come through registers; tile by tile, the other waves' MFMAs beside this one's VALU
+    // (with S(t+1) ahead as above, D = 128 spills 60 to 220 registers).
+    auto iteration8 = [&](auto par, int t) {
+      constexpr int P = decltype(par)::value;
+      const std::integral_constant<int, P> cur{};
+      const std::integral_constant<int, 1 - P> nxt{};
+      const int row_t1 = row1;
+      const bool fetch = t + 1 < nt;
+      if (fetch) {
+        to_regs(c.k, rows1, kx);
+        to_regs(c.v, rows1, vx);
+        if (wave == 0) scale_x = load_scale(c.k_scale, row_t1);
+        if (wave == 1) scale_x = load_scale(c.v_scale, row_t1);
+      }
+      row1 = find_row(t + 2, page);
+      page = load_page(t + 3);
+      chunk_rows(row1, rows1);
+      if (t < wave_tiles) {
+        V8 pf[PV_STEPS];
         const bool clean = is_clean(t, present);
+        qk(sa, k_stage(cur));
+        scale_scores(sa, P);
+        if (!clean) mask(sa, t, present);
+        raise(row_max(sa));
         if constexpr (kUnits) {
           const float top = uniform_f(top_lds[P]);
           if (top > vref) {
@@ -828,40 +890,26 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
             for (int db = 0; db < NDB; ++db) o[db] *= f;
           }
         }
-        // Phase A: S(t+1) with P(t). (Past the last tile the product is of what the stage holds, and unused.)
-        __builtin_amdgcn_s_setprio(2);
-        qk(sn, k_stage(nxt));
-        exponentiate(s, pf, P, clean, t, present);
-        __builtin_amdgcn_s_setprio(0);
-        const bool more = t + 1 < wave_tiles;
-        if (more) {
-          scale_scores(sn, 1 - P);
-          if (!is_clean(t + 1, present1)) mask(sn, t + 1, present1);
-        }
-        // Phase B: O += V(t) P(t) with the row maxima of S(t+1).
+        exponentiate8(sa, pf, P, clean, t, present);
         if (!clean && skip_from == INT32_MAX && !values_finite(v_stage(cur))) skip_from = t;
         if (clean || skip_from == INT32_MAX) pv(pf, v_stage(cur));
-        row_sum(pf);
-        if (more) raise(row_max(sn));
       }
-      if constexpr (k8) {
-        if (t + 1 < nt) {
-          widen(kx, k_stage(cur), false);
-          widen(vx, v_stage(nxt), true);
-          if (wave == 0) ks_lds[P][lane] = row2 >= 0 ? ksx * w.scale_log2 : 0.f;
-          store_v_scale(1 - P, row1, vsx);
-        }
+      present = present1, present1 = __builtin_amdgcn_ballot_w64(row1 >= 0);
+      if (fetch) {
+        widen(kx, k_stage(nxt), false);
+        widen(vx, v_stage(nxt), true);
+        if (wave == 0) ks_lds[1 - P][lane] = row_t1 >= 0 ? scale_x * w.scale_log2 : 0.f;
+        store_v_scale(1 - P, row_t1, scale_x);
       }
-      present = present1, present1 = present2, row1 = row2;
-#pragma unroll
-      for (int i = 0; i < CPT; ++i) rows1[i] = rows2[i];
-      __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
     };
     for (int t = 0; t < nt; t += 2) {
-      iteration(even, t, sa, sb);
-      if (t + 1 < nt) iteration(odd, t + 1, sb, sa);
+      if constexpr (k8) iteration8(even, t); else iteration(even, t, sa, sb);
+      if (t + 1 < nt) {
+        if constexpr (k8) iteration8(odd, t + 1); else iteration(odd, t + 1, sb, sa);
+      }
     }
+
 
     // ---- P . V of the tiles left out, over the visible pairs alone: scores again, all in fp32
     if (skip_from < wave_tiles) {
@@ -945,34 +993,78 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 }
 
 // Joins the parts of the tile that workgroup blockIdx.x of the attention kernel began and did not end: its own
-// and those of the workgroups after it, up to the one that ends the tile. 16 threads a row.
+// and those of the workgroups after it, up to the one that ends the tile. 16 threads a row. What bounds it is
+// the latency of its loads, so that no load waits for another but the records: the parts' number comes from
+// 64 records at once, their weights by lane, and their rows four parts at a time.
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedCache c, RowsQ a, AttnWork w, int wgs) {
-  constexpr int EL = D / 16;
-  const PartRecord rec = w.records[blockIdx.x];
+  constexpr int EL = D / 16, MOST = 64;
+  __shared__ float weight[16][MOST];
+  const int first = (int)blockIdx.x, lane = (int)threadIdx.x % kWave;
+  const PartRecord rec = w.records[first];
   if (!(rec.flags & kPartBegins)) return;
+  int n = 1;   // parts
+  for (int at = first + 1; at < wgs; at += kWave) {
+    const int flags = at + lane < wgs ? w.records[at + lane].flags : kPartEnds;
+    const uint64_t ends = __builtin_amdgcn_ballot_w64((flags & kPartEnds) != 0);
+    n = at - first + (ends ? __builtin_ctzll(ends) + 1 : kWave);
+    if (ends) break;
+  }
+  n = min(n, wgs - first);
   const SeqRows s = load_seq(c, rec.seq);
-  const int part = (int)threadIdx.x % 16;
-  for (int r = (int)blockIdx.y * 16 + (int)threadIdx.x / 16; r < ROWS; r += (int)gridDim.y * 16) {
+  const int part = (int)threadIdx.x % 16, tr = (int)threadIdx.x / 16;
+  for (int r0 = (int)blockIdx.y * 16; r0 < ROWS; r0 += (int)gridDim.y * 16) {
+    const int r = r0 + tr;
     int token, hq;
-    if (!tile_row(w.tiles, s, rec.head, rec.tile, r, token, hq)) continue;
+    const bool mine = tile_row(w.tiles, s, rec.head, rec.tile, r, token, hq);
     float m = -INFINITY, sum = 0.f, x[EL] = {};
-    for (int i = (int)blockIdx.x; i < wgs; ++i) {
-      const int slot = i == (int)blockIdx.x ? 1 : 0;
-      const float* st = part_stats(w, wgs, i, slot, ROWS, D);
-      const float* from = part_rows(w, i, slot, ROWS, D) + r * D + part * EL;
-      const float mi = st[r], mn = fmaxf(m, mi);
-      const float f = m == -INFINITY ? 0.f : exp2_fast(m - mn), fi = mi == -INFINITY ? 0.f : exp2_fast(mi - mn);
-      sum = sum * f + st[ROWS + r] * fi;
+    for (int p0 = 0; p0 < n; p0 += MOST) {
+      float mi[MOST / 16], li[MOST / 16], top = -INFINITY, add = 0.f;
 #pragma unroll
-      for (int e = 0; e < EL; e += 4) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(from + e);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[e + j] = (f > 0.f ? x[e + j] * f : 0.f) + (fi > 0.f ? y[j] * fi : 0.f);
+      for (int k = 0; k < MOST / 16; ++k) {
+        const int i = p0 + 16 * k + part;
+        mi[k] = -INFINITY, li[k] = 0.f;
+        if (mine && i < n) {
+          const float* st = part_stats(w, wgs, first + i, i == 0 ? 1 : 0, ROWS, D);
+          mi[k] = st[r], li[k] = st[ROWS + r];
+        }
       }
+#pragma unroll
+      for (int k = 0; k < MOST / 16; ++k) top = fmaxf(top, mi[k]);
+      top = fmaxf(top, dpp_move<0xB1>(top));
+      top = fmaxf(top, dpp_move<0x4E>(top));
+      top = fmaxf(top, dpp_move<0x141>(top));
+      top = fmaxf(top, dpp_move<0x140>(top));
+      const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : exp2_fast(m - mn);
+#pragma unroll
+      for (int k = 0; k < MOST / 16; ++k) {
+        const float e = mi[k] == -INFINITY ? 0.f : exp2_fast(mi[k] - mn);
+        weight[tr][16 * k + part] = e;
+        add = fmaf(e, li[k], add);
+      }
+      add += dpp_move<0xB1>(add);
+      add += dpp_move<0x4E>(add);
+      add += dpp_move<0x141>(add);
+      add += dpp_move<0x140>(add);
+      sum = sum * f + add;
       m = mn;
-      if (i != (int)blockIdx.x && (w.records[i].flags & kPartEnds)) break;
+#pragma unroll
+      for (int e = 0; e < EL; ++e) x[e] = f > 0.f ? x[e] * f : 0.f;
+      // (A row's weights are written and read by the same wave, in order.)
+      if (mine)
+#pragma unroll 4
+        for (int i = 0; i < min(MOST, n - p0); ++i) {
+          const float wi = weight[tr][i];
+          const float* from = part_rows(w, first + p0 + i, p0 + i == 0 ? 1 : 0, ROWS, D) + r * D + part * EL;
+#pragma unroll
+          for (int e = 0; e < EL; e += 4) {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(from + e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[e + j] = fmaf(wi, wi > 0.f ? y[j] : 0.f, x[e + j]);
+          }
+        }
     }
+    if (!mine) continue;
     typedef T TE __attribute__((ext_vector_type(EL)));
     TE y;
 #pragma unroll

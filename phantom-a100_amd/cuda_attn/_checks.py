@@ -153,6 +153,37 @@ def check_paged(name: str, rows, k_cache, v_cache, page_table, lengths, k_scale,
         _fail(f"{name}: k_scale and v_scale are for 8-bit caches")
 
 
+def paged_ok(rows, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale) -> bool:
+    """Whether a call passes check_paged and check_rows, each property read once: a small call is bound by this
+    host path. Anything that this does not accept goes through those checks for its message."""
+    shape, dtype, device = k_cache.shape, k_cache.dtype, k_cache.device
+    table = page_table.shape
+    if not (len(shape) == 4 and shape[3] in TC_HEAD_DIMS and k_cache.is_cuda and k_cache.is_contiguous()
+            and v_cache.shape == shape and v_cache.dtype is dtype and v_cache.device == device and v_cache.is_contiguous()
+            and 0 not in shape and len(table) == 2 and 0 not in table and page_table.dtype is torch.int32
+            and page_table.stride(1) == 1 and page_table.device == device and lengths.dtype is torch.int32
+            and lengths.shape == table[:1] and lengths.device == device and lengths.is_contiguous()
+            and (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0):
+        return False
+    if dtype in EIGHT_BIT:
+        for s in (k_scale, v_scale):
+            if not (s is not None and s.shape == shape[:3] and s.dtype is torch.float32 and s.device == device and s.is_contiguous()):
+                return False
+    elif k_scale is not None or v_scale is not None:
+        return False
+    if rows is None:
+        return dtype in TC_DTYPES or dtype in EIGHT_BIT
+    x, strides = rows.shape, rows.stride()
+    if not (len(x) == 3 and x[2] == shape[3] and 0 not in x and strides[2] == 1 and (strides[0] | strides[1]) % 8 == 0
+            and rows.device == device and rows.data_ptr() % 16 == 0 and rows.dtype in TC_DTYPES
+            and (dtype is rows.dtype or dtype in EIGHT_BIT)):
+        return False
+    if cu_seqlens is None:
+        return x[0] % table[0] == 0
+    return (cu_seqlens.dtype is torch.int32 and cu_seqlens.shape == (table[0] + 1,) and cu_seqlens.device == device
+            and cu_seqlens.is_contiguous())
+
+
 def check_rows(name: str, x, k_cache, lengths, cu_seqlens) -> None:
     """A tensor of new tokens, (tokens, heads, d)."""
     if x.dim() != 3 or x.shape[2] != k_cache.shape[3]:
@@ -171,8 +202,13 @@ def check_rows(name: str, x, k_cache, lengths, cu_seqlens) -> None:
 
 
 def check_same_rows(name: str, k, v, k_cache) -> None:
+    """v against k, which has been checked."""
     if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.shape[1] != k_cache.shape[1]:
         _fail(f"{name}: k and v must share shape, dtype and device and have the cache's heads")
+    strides = v.stride()
+    if strides[2] != 1 or strides[0] % 8 or strides[1] % 8:
+        _fail(f"{name}: rows must be contiguous, at strides of whole 16-byte steps")
+    check_aligned(name, v)
 
 
 def check_query_heads(name: str, q, k_cache) -> None:

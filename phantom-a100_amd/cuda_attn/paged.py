@@ -23,6 +23,8 @@ replayed. Whatever they hold, no access leaves the tensors. Rows behind the last
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _checks, _native
@@ -31,13 +33,23 @@ _DTYPE_CODE = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_B
                torch.int8: _native.DTYPE_I8, torch.float8_e4m3fn: _native.DTYPE_E4M3}
 
 
+_pack = struct.Struct("PPPPPPqqqqqqqi4x").pack   # pa_paged_cache, several times faster than its fields one by one
+
+
 def _cache_args(k_cache, v_cache, page_table, lengths, k_scale, v_scale):
     pages, heads, page_size, d = k_cache.shape
-    return _native.PagedCacheArgs(
-        k_cache.data_ptr(), v_cache.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
-        None if v_scale is None else v_scale.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-        pages, page_size, heads, d, page_table.shape[0], page_table.shape[1], page_table.stride(0),
-        _DTYPE_CODE[k_cache.dtype])
+    seqs, cols = page_table.shape
+    return _native.PagedCacheArgs.from_buffer_copy(_pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
+        0 if v_scale is None else v_scale.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+        pages, page_size, heads, d, seqs, cols, page_table.stride(0), _DTYPE_CODE[k_cache.dtype]))
+
+
+def _check(name, rows, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale):
+    if not _checks.paged_ok(rows, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale):
+        _checks.check_paged(name, rows, k_cache, v_cache, page_table, lengths, k_scale, v_scale)
+        if rows is not None:
+            _checks.check_rows(name, rows, k_cache, lengths, cu_seqlens)
 
 
 def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -51,13 +63,12 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     call must be distinct (no page shared by two sequences where both write)."""
     from . import _call, _stream_ptr
 
-    _checks.check_paged("cache_write", k, k_cache, v_cache, page_table, lengths, k_scale, v_scale)
-    _checks.check_rows("cache_write", k, k_cache, lengths, cu_seqlens)
-    _checks.check_rows("cache_write", v, k_cache, lengths, cu_seqlens)
+    _check("cache_write", k, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale)
     _checks.check_same_rows("cache_write", k, v, k_cache)
+    ks, vs = k.stride(), v.stride()
     cache = _cache_args(k_cache, v_cache, page_table, lengths, k_scale, v_scale)
     _call("pa_cache_write", "cache_write", k.device, cache, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], k.shape[0],
-          k.stride(0), k.stride(1), v.stride(0), v.stride(1), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+          ks[0], ks[1], vs[0], vs[1], None if cu_seqlens is None else cu_seqlens.data_ptr(),
           _stream_ptr(k.device))
 
 
@@ -71,7 +82,7 @@ def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     from . import _call, _stream_ptr
 
     dtype = _checks.read_dtype("cache_read", k_cache, dtype)
-    _checks.check_paged("cache_read", None, k_cache, v_cache, page_table, lengths, k_scale, v_scale)
+    _check("cache_read", None, k_cache, v_cache, page_table, lengths, None, k_scale, v_scale)
     b, (_, heads, page_size, d) = page_table.shape[0], k_cache.shape
     n = page_table.shape[1] * page_size if max_len is None else max_len
     _checks.check_max_len("cache_read", n)
@@ -97,11 +108,10 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     a new tensor are not set."""
     from . import _call, _stream_ptr
 
-    _checks.check_paged("paged_attn", q, k_cache, v_cache, page_table, lengths, k_scale, v_scale)
-    _checks.check_rows("paged_attn", q, k_cache, lengths, cu_seqlens)
+    _check("paged_attn", q, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale)
     _checks.check_query_heads("paged_attn", q, k_cache)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q)
     else:
         _checks.check_out("paged_attn", q, out)
     bound = 0 if max_new is None else _checks.check_max_new("paged_attn", max_new)
@@ -113,7 +123,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     if need < 0:
         _native.check(need, "paged_attn")
     workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    qs, os = q.stride(), out.stride()
     _call("pa_paged_attn_fwd", "paged_attn", q.device, cache, q.data_ptr(), out.data_ptr(), code, tokens, heads_q,
-          q.stride(0), q.stride(1), out.stride(0), out.stride(1), cu, bound, 1 if causal else 0, workspace.data_ptr(),
+          qs[0], qs[1], os[0], os[1], cu, bound, 1 if causal else 0, workspace.data_ptr(),
           need, _stream_ptr(q.device))
     return out

@@ -213,3 +213,39 @@ def test_oracle_codes():
     assert scale[0] == 2 and scale[1] == 0 and math.isnan(scale[2]) and scale[3] == 0
     codes, scale = po.quantise(x, torch.float8_e4m3fn)
     assert codes.float()[0].tolist() == [1.75, -3.5, 0.875, 448.0] and scale[0] == torch.tensor(254.0) / 448
+
+
+@pytest.mark.parametrize("change", [
+    {}, {"k_cache": torch.zeros(5, 2, 64, 16, dtype=torch.float16).transpose(2, 3)}, {"v_cache": torch.zeros(5, 2, 16, 64)},
+    {"v_cache": torch.zeros(4, 2, 16, 64, dtype=torch.float16)}, {"page_table": torch.zeros(3, 2, dtype=torch.int64)},
+    {"page_table": torch.zeros(2, 3, dtype=torch.int32).t()}, {"lengths": torch.zeros(2, dtype=torch.int32)},
+    {"lengths": torch.zeros(6, dtype=torch.int32)[::2]}, {"k_scale": torch.zeros(5, 2, 16)}, {"rows": torch.zeros(6, 4, 64)},
+    {"rows": torch.zeros(6, 4, 68, dtype=torch.float16)[..., :64]}, {"rows": torch.zeros(7, 4, 64, dtype=torch.float16)}])
+def test_one_pass_acceptance_agrees_with_the_checks(change, monkeypatch):
+    """paged_ok accepts what the checks one by one accept (on CPU tensors that say they are on the GPU), nothing else."""
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+    t = tensors()
+    t.update(change)
+    t = {n: x if x is None else x.as_subclass(OnGpu) for n, x in t.items()}
+
+    def one_by_one():
+        try:
+            _checks.check_paged("paged_attn", **t)
+            _checks.check_rows("paged_attn", t["rows"], t["k_cache"], t["lengths"], None)
+        except RuntimeError:
+            return False
+        return True
+    ok = _checks.paged_ok(t["rows"], t["k_cache"], t["v_cache"], t["page_table"], t["lengths"], None, t["k_scale"], t["v_scale"])
+    assert ok == one_by_one() == (not change)
+
+
+def test_packed_arguments_are_the_structure():
+    from cuda_attn import paged as pg
+    t = tensors(cache=torch.int8)
+    got = pg._cache_args(t["k_cache"], t["v_cache"], t["page_table"], t["lengths"], t["k_scale"], t["v_scale"])
+    assert (got.k, got.v, got.k_scale, got.v_scale) == tuple(t[n].data_ptr() for n in ("k_cache", "v_cache", "k_scale", "v_scale"))
+    assert (got.page_table, got.lengths) == (t["page_table"].data_ptr(), t["lengths"].data_ptr())
+    assert (got.pages, got.page_size, got.heads, got.d, got.seqs, got.table_cols, got.table_stride, got.dtype) == \
+        (5, 16, 2, 64, 3, 2, 2, _native.DTYPE_I8)
+    assert pg._cache_args(t["k_cache"], t["v_cache"], t["page_table"], t["lengths"], None, None).k_scale is None
