@@ -45,12 +45,24 @@ __device__ __forceinline__ float* part_stats(const AttnWork& w, int wgs, int wg,
   return w.parts + (int64_t)wgs * 2 * rows * d + ((int64_t)wg * 2 + slot) * 2 * rows;
 }
 
-// Row r of a tile: its new token among the sequence's and its query head; false if the tile has no such row.
-__device__ __forceinline__ bool tile_row(const TileShape& t, const SeqRows& s, int head, int tile, int r, int& token, int& hq) {
-  const int in_tile = r / t.heads, g = head % t.splits * t.heads + r % t.heads;
-  token = tile * t.tokens + in_tile;
-  hq = head / t.splits * t.group + g;
-  return in_tile < t.tokens && token < s.count && g < t.group;
+// Row r of a tile, whichever tile it is: its token and its head among the tile's.
+struct InTile {
+  int token, head;
+};
+__device__ __forceinline__ InTile in_tile(const TileShape& t, int r) { return {r / t.heads, r % t.heads}; }
+// The key/value head and the part of its group that a tile's `head` stands for.
+__device__ __forceinline__ void split_head(const TileShape& t, int head, int& kv_head, int& part) {
+  kv_head = t.splits == 1 ? head : head / t.splits;
+  part = t.splits == 1 ? 0 : head % t.splits;
+}
+// The row's new token among the sequence's and its query head; false if the tile has no such row.
+__device__ __forceinline__ bool tile_row(const TileShape& t, const SeqRows& s, int head, int tile, InTile r, int& token, int& hq) {
+  int kv_head, part;
+  split_head(t, head, kv_head, part);
+  const int g = part * t.heads + r.head;
+  token = tile * t.tokens + r.token;
+  hq = kv_head * t.group + g;
+  return r.token < t.tokens && token < s.count && g < t.group;
 }
 
 // Wave-uniform values in scalar registers: the walk and its branches are the same in every lane, which the
@@ -160,6 +172,10 @@ __device__ __forceinline__ float add_pair(unsigned x, float c, bf16*) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), bf16x2{(bf16)1.f, (bf16)1.f}, c, false);
 }
 
+// Maxima that pass a NaN on: fmaxf first quiets each operand, an instruction apiece. (A row with a NaN score is NaN,
+// whatever its reference.)
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // x over the lanes of equal lane % 16.
 __device__ __forceinline__ float groups_max(float x) { x = fmaxf(x, partner16(x)); return fmaxf(x, partner32(x)); }
 __device__ __forceinline__ float groups_sum(float x) { x += partner16(x); return x + partner32(x); }
@@ -219,16 +235,20 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
   int w_base = v_at(w_row, w_chunk), r_base = v_at(4 * g + lq / 4, lq % 4 / 2) + 8 * (lq % 2);
   auto v_write = [&](int i) { return i * RPL * RB + (w_base ^ (RPL == 4 && CR == 16 && i % 2 ? 128 : 0)); };
 
+  InTile in_row[NB], out_row[NB];   // of the lane's columns, and of the rows that the thread joins
+#pragma unroll
+  for (int b = 0; b < NB; ++b) in_row[b] = in_tile(w.tiles, 16 * b + lq), out_row[b] = in_tile(w.tiles, 16 * b + tid / 16);
   while (active && uniform((int)walk.next([&](int s) { return uniform(load_seq(c, s)); }, sg)) != 0) {
     sg = {uniform(sg.rows), uniform(sg.seq), uniform(sg.head), uniform(sg.tile), uniform(sg.from), uniform(sg.to), uniform(sg.steps)};
-    const int kv_head = sg.head / w.tiles.splits;
+    int kv_head, head_part;
+    split_head(w.tiles, sg.head, kv_head, head_part);
     // ---- the tile's queries
     u32x4 qf[NB][KK];
     int seen[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       int token, hq;
-      const bool mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, 16 * b + lq, token, hq);
+      const bool mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, in_row[b], token, hq);
       seen[b] = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
       const T* qp = static_cast<const T*>(a.q) + (mine ? (int64_t)(sg.rows.first + token) * a.q_token + hq * a.q_head : 0);
 #pragma unroll
@@ -244,7 +264,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         int token, hq;
-        if (tile_row(w.tiles, sg.rows, sg.head, sg.tile, 16 * b + lq, token, hq)) lo = min(lo, seen[b]), hi = max(hi, seen[b]);
+        if (tile_row(w.tiles, sg.rows, sg.head, sg.tile, in_row[b], token, hq)) lo = min(lo, seen[b]), hi = max(hi, seen[b]);
       }
 #pragma unroll
       for (int d = 1; d < 16; d *= 2) lo = min(lo, __shfl_xor(lo, d)), hi = max(hi, __shfl_xor(hi, d));
@@ -481,7 +501,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
         }
       }
       int token, hq;
-      if (tile_row(w.tiles, sg.rows, sg.head, sg.tile, 16 * b + q, token, hq)) {
+      if (tile_row(w.tiles, sg.rows, sg.head, sg.tile, out_row[b], token, hq)) {
         if (done) {
           typedef T TE __attribute__((ext_vector_type(EL)));
           TE y;
@@ -508,8 +528,9 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 //
 // A tile has BM rows, 32 for each wave; its keys go past in tiles of 64 that all waves share in LDS, and what
 // bounds the kernel is the matrix core beside the exponentials. Both products as in fa_mfma.hpp, transposed on
-// 32x32x16 MFMAs with a query per lane, and its two-stage pipeline: while tile t's scores become P(t) the
-// matrix core takes S(t+1), and while it takes O += V(t) P(t) the scores of t+1 get their row maxima. K(t+2)
+// 32x32x16 MFMAs with a query per lane, and its two-stage pipeline over the tiles that every row
+// sees whole: the matrix core takes S(t+1) beside half of the exponentials of P(t), and O += V(t) P(t) beside
+// half of those of P(t+1). K(t+2)
 // and V(t+1) arrive meanwhile: 16-bit rows straight into LDS from 64-bit addresses, a row per page lookup;
 // 8-bit rows through registers, widened to 16 bits (exact) once for all waves. A key's scale multiplies its
 // scores, a value's scale its P before the one rounding of P to the type.
@@ -517,12 +538,13 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 // A value that is not finite must not reach rows that do not see it: a wave looks at the values of a tile that
 // some row sees and another does not, leaves a tile with such a value out of P . V, and adds it at the end in
 // fp32 over the visible pairs.
-__device__ __attribute__((aligned(16))) const unsigned char kZeroChunk[16] = {};
-
 constexpr int chunk_rows_of(int d) { return d == 128 ? 256 : 128; }
 constexpr int chunk_wgs(int d) { return d == 128 ? 1 : 2; }   // workgroups on a CU
 
-template <typename T, typename C, int D, int BM>
+// WIDE: caches of 4 GiB and more. A load to LDS from a 64-bit address is an instruction of the flat kind, after
+// which the compiler waits for all LDS reads instead of the oldest; from a buffer, whose offsets have 32 bits, it is not.
+constexpr uint32_t kPastBuffer = 0xffffe000u;
+template <typename T, typename C, int D, int BM, bool WIDE>
 __global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(2)))
 paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   typedef typename vec8<T>::type V8;
@@ -552,17 +574,29 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   // The swizzles reach chunk bits that the step and the dim block do not, so those enter by XOR.
   const int v_row = hi * 4 + i16 / 4, v_cl = 2 * (g16 % 2) + (i16 % 4) / 2;
   int k_base = lq * RB + ((hi ^ k_swz<CR>(lq)) * 16), v_base = v_row * RB + ((v_cl ^ v_swz<CR>(v_row)) * 16) + 8 * (i16 % 2);
+  const uint32_t cache_bytes = (uint32_t)min((uint64_t)c.pages * c.heads * c.page_size * CB, (uint64_t)kPastBuffer);
+  const rsrc_t k_rs = make_rsrc(c.k, cache_bytes), v_rs = make_rsrc(c.v, cache_bytes);
+
   PartRecord rec = {0, 0, 0, 0};
   WorkWalk walk;
   int wg;
   const bool active = start_walk<THREADS>(c, w, true, walk_lds, wg, walk);
   Segment sg;
+  const InTile in_row = in_tile(w.tiles, 32 * wave + lq);
   while (active && uniform((int)walk.next([&](int s) { return uniform(load_seq(c, s)); }, sg)) != 0) {
     sg = {uniform(sg.rows), uniform(sg.seq), uniform(sg.head), uniform(sg.tile), uniform(sg.from), uniform(sg.to), uniform(sg.steps)};
-    const int kv_head = sg.head / w.tiles.splits;
-    int token, hq;
-    const bool mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, 32 * wave + lq, token, hq);
-    const int seen = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
+    int kv_head, head_part;
+    split_head(w.tiles, sg.head, kv_head, head_part);
+    // The lane's row. Found again for each use, not held over the loops.
+    int token, hq, seen;
+    bool mine;
+    auto find_mine = [&]() {
+      InTile r = in_row;
+      asm volatile("" : "+v"(r.token), "+v"(r.head));
+      mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, r, token, hq);
+      seen = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
+    };
+    find_mine();
     V8 qf[QK_STEPS];
     {
       const T* qp = static_cast<const T*>(a.q) + (mine ? (int64_t)(sg.rows.first + token) * a.q_token + hq * a.q_head : 0) + 8 * hi;
@@ -589,27 +623,31 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     auto find_row = [&](int t, int page) {
       const int key = key_begin + t * BN + lane;
       const uint32_t at = ((uint32_t)page * c.heads + kv_head) * c.page_size + (key - page_of((uint32_t)key, c.div) * c.page_size);
-      return key < key_end && (unsigned)page < (unsigned)c.pages ? (int)at : -1;
+      return (key < key_end) & ((unsigned)page < (unsigned)c.pages) ? (int)at : -1;
     };
-    // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row.
-    auto to_lds = [&](const void* cache, const int (&rows)[CPT], unsigned char* stage, bool is_v) {
+    // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row (loads
+    // are 32 rows apart, so the swizzle is the same).
+    static_assert(k8 || THREADS / LPR == 32, "loads 32 rows apart");
+    const int k_off = (tid % LPR ^ k_swz<CR>(tid / LPR)) * 16, v_off = (tid % LPR ^ v_swz<CR>(tid / LPR)) * 16;
+    auto to_lds = [&](const void* cache, rsrc_t rs, const int (&rows)[CPT], unsigned char* stage, bool is_v) {
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
-        const int slot = i * THREADS + tid, r = slot / CR, pc = slot % CR;
-        const int off = (pc ^ (is_v ? v_swz<CR>(r) : k_swz<CR>(r))) * 16;
-        const unsigned char* p = rows[i] < 0 ? kZeroChunk : static_cast<const unsigned char*>(cache) + (int64_t)rows[i] * CB + off;
-        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)p,
-                                         (__attribute__((address_space(3))) void*)(stage + (i * THREADS + wave * kWave) * 16), 16, 0, 0);
+        unsigned off = is_v ? v_off : k_off;
+        asm("" : "+v"(off));   // (not to be added to the base once for all loads: that spills)
+        unsigned char* to = stage + (i * THREADS + wave * kWave) * 16;
+        if constexpr (WIDE) {
+          const unsigned char* p = static_cast<const unsigned char*>(cache) + ((uint64_t)(unsigned)rows[i] * CB + off);
+          __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+        } else {
+          load16_to_lds(rs, to, (unsigned)rows[i] + off, 0);
+        }
       }
     };
     // 8-bit rows: load, then widen and store.
     auto to_regs = [&](const void* cache, const int (&rows)[CPT], u32x4 (&x)[CPT]) {
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) {
-        const unsigned char* p = rows[i] < 0 ? kZeroChunk
-                                             : static_cast<const unsigned char*>(cache) + (int64_t)rows[i] * CB + (i * THREADS + tid) % LPR * 16;
-        x[i] = *reinterpret_cast<const u32x4*>(p);
-      }
+      for (int i = 0; i < CPT; ++i)
+        x[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(cache) + (uint64_t)(unsigned)rows[i] * CB + tid % LPR * 16);
     };
     auto widen = [&](const u32x4 (&x)[CPT], unsigned char* stage, bool is_v) {
       if constexpr (k8)
@@ -623,7 +661,17 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         *reinterpret_cast<u32x4*>(stage + r * RB + (((ch + 1) ^ sw) * 16)) = hi16;
       }
     };
-    auto chunk_rows = [&](int row, int (&rows)[CPT]) {
+    auto present_of = [&](int row) -> uint64_t { return __builtin_amdgcn_ballot_w64(row >= 0); };
+    // The row that each of the thread's loads reads; where loads are from a buffer, its byte offset, past the
+    // buffer's end (which loads as zeros) for an absent key. Elsewhere an absent key takes the row of the tile's
+    // first present one: its scores are masked, and its P is 0, which a finite value leaves without effect.
+    auto chunk_rows = [&](int row, uint64_t pres, int (&rows)[CPT]) {
+      if constexpr (k8 || WIDE) {
+        const int first = max(__builtin_amdgcn_readlane(row, __builtin_ctzll(pres | 1ull << 63)), 0);
+        row = row < 0 ? first : row;
+      } else {
+        row = row < 0 ? (int)kPastBuffer : (int)((unsigned)row * CB);
+      }
 #pragma unroll
       for (int i = 0; i < CPT; ++i) rows[i] = __shfl(row, (i * THREADS + tid) / LPR);
     };
@@ -647,14 +695,17 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
     for (int db = 0; db < NDB; ++db) o[db] = f32x16{};
 
+    // (The operands' addresses are made from their base each time: hoisted out of the loops, they spill.)
     auto qk = [&](f32x16 (&s)[NKB], const unsigned char* ks) {
+      int kb = k_base;
+      asm("" : "+v"(kb));
 #pragma unroll
       for (int b = 0; b < NKB; ++b) s[b] = f32x16{};
 #pragma unroll
       for (int kk = 0; kk < QK_STEPS; ++kk)
 #pragma unroll
         for (int b = 0; b < NKB; ++b)
-          s[b] = mfma32x32x16(*reinterpret_cast<const V8*>(ks + b * 32 * RB + (k_base ^ (32 * kk))), qf[kk], s[b]);
+          s[b] = mfma32x32x16(*reinterpret_cast<const V8*>(ks + b * 32 * RB + (kb ^ (32 * kk))), qf[kk], s[b]);
     };
     // Keys' scales (8 bits; with log2(e)/sqrt(d), so that scores are in the exponent's units).
     auto scale_scores = [&](f32x16 (&s)[NKB], int par) {
@@ -693,18 +744,20 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-      return half_max(mx) * (k8 ? 1.f : w.scale_log2);
+        for (int r = 0; r < 16; r += 2) mx = max_nan(mx, max_nan(s[b][r], s[b][r + 1]));
+      return max_nan(mx, partner32(mx)) * (k8 ? 1.f : w.scale_log2);
     };
-    auto raise = [&](float mx) {   // the reference maximum, where some row's grew past 2^8
+    auto raise = [&](float mx) {   // the reference maximum, where some row's grew past 2^8: whether it did
       const float m_new = fmaxf(m_run, mx);
-      if (__builtin_amdgcn_ballot_w64(m_new > m_run + kLazyLog2) != 0) {
+      const bool up = __builtin_amdgcn_ballot_w64(m_new > m_run + kLazyLog2) != 0;
+      if (up) {
         const float f = m_new > m_run ? exp2_fast(m_run - m_new) : 1.f;   // (m_run = -inf: 0)
         m_run = m_new;
         l *= f;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) o[db] *= f;
       }
+      return up;
     };
     auto exponentiate = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS]) {
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
@@ -734,11 +787,13 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         }
     };
     auto pv = [&](const V8 (&pf)[PV_STEPS], const unsigned char* vs) {
+      int vb = v_base;
+      asm("" : "+v"(vb));
 #pragma unroll
       for (int i = 0; i < PV_STEPS; ++i)
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
-          const unsigned char* p0 = vs + i * 16 * RB + (v_base ^ (64 * db));
+          const unsigned char* p0 = vs + i * 16 * RB + (vb ^ (64 * db));
           const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p0));
           const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p0 + 8 * RB));
           const i16x8 x = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
@@ -760,127 +815,204 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       for (int i = 0; i < TILE_BYTES / 16 / kWave; ++i) top = max_bits(top, *reinterpret_cast<const u32x4*>(vs + (i * kWave + lane) * 16));
       return __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= kInfBits<T>) == 0;
     };
-    // ---- the first tiles: K(0), V(0), K(1)
-    int page = load_page(0), page1 = load_page(1);
-    int row = find_row(0, page), row1 = find_row(1, page1);
-    page = load_page(2);
-    uint64_t present = __builtin_amdgcn_ballot_w64(row >= 0), present1 = __builtin_amdgcn_ballot_w64(row1 >= 0);
-    int rows[CPT], rows1[CPT];
-    chunk_rows(row, rows);
-    chunk_rows(row1, rows1);
-    u32x4 kx[CPT], vx[CPT];
-    float scale_x = 0.f;
-    if constexpr (k8) {
-      to_regs(c.k, rows, kx);
-      to_regs(c.v, rows, vx);
-      if (wave == 0) ks_lds[0][lane] = row >= 0 ? load_scale(c.k_scale, row) * w.scale_log2 : 0.f;
-      if (wave == 1) store_v_scale(0, row, load_scale(c.v_scale, row));
-      widen(kx, k_stage(even), false);
-      widen(vx, v_stage(even), true);
-    } else {
-      to_lds(c.k, rows, k_stage(even), false);
-      to_lds(c.v, rows, v_stage(even), true);
-      to_lds(c.k, rows1, k_stage(odd), false);
+    const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
+    auto is_clean = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= wave_all; };
+
+    // ---- the first tiles: K(0), V(0), K(1). At a tile t: rows1, row1 and present1 are tile t + 1's, rows2, row2 and
+    // present2 tile t + 2's, page holds tile t + 3's entries.
+    int page = load_page(0), page1 = load_page(1), page2 = load_page(2);
+    int row = find_row(0, page), row1 = find_row(1, page1), row2 = find_row(2, page2);
+    page = load_page(3);
+    uint64_t present = present_of(row), present1 = present_of(row1), present2 = present_of(row2);
+    int rows1[CPT], rows2[CPT];
+    {
+      int rows[CPT];
+      chunk_rows(row, present, rows);
+      chunk_rows(row1, present1, rows1);
+      chunk_rows(row2, present2, rows2);
+      if constexpr (k8) {
+        u32x4 kx[CPT], vx[CPT];
+        to_regs(c.k, rows, kx);
+        to_regs(c.v, rows, vx);
+        if (wave == 0) ks_lds[0][lane] = row >= 0 ? load_scale(c.k_scale, row) * w.scale_log2 : 0.f;
+        if (wave == 1) store_v_scale(0, row, load_scale(c.v_scale, row));
+        widen(kx, k_stage(even), false);
+        widen(vx, v_stage(even), true);
+      } else {
+        to_lds(c.k, k_rs, rows, k_stage(even), false);
+        to_lds(c.v, v_rs, rows, v_stage(even), true);
+        to_lds(c.k, k_rs, rows1, k_stage(odd), false);
+      }
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    f32x16 sa[NKB], sb[NKB];
-    const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
-    auto is_clean = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= wave_all; };
+
+    // ---- the leading tiles that every row sees whole, in the two-stage pipeline (16-bit rows)
+    int t0 = 0;   // tiles done
     if constexpr (!k8) {
-      if (wave_tiles > 0) {
+      const int tile_all = keys_seen(sg.rows, sg.tile * w.tiles.tokens, c.capacity, w.causal);   // the first row's keys
+      auto whole_tile = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= tile_all; };
+      constexpr int HALF = PV_STEPS / 2;
+      // P of scores e and e + 1 (e even; 16-key step e / 8).
+      auto exp_pair = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int e, float neg_m) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = e; k < e + 2; ++k)
+          pf[k / 8][k % 8] = from_f32<T>(exp2_fast(fmaf(s[k / 16][k % 16], w.scale_log2, neg_m)));
+      };
+      auto neg_ref = [&]() { return m_run == -INFINITY ? 0.f : -m_run; };
+      auto exp_first = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS]) __attribute__((always_inline)) {
+        const float neg_m = neg_ref();
+#pragma unroll
+        for (int e = 0; e < HALF * 8; e += 2) exp_pair(s, pf, e, neg_m);
+      };
+      f32x16 sa[NKB], sb[NKB];
+      V8 pa[PV_STEPS], pb[PV_STEPS];
+      if (whole_tile(0, present) && whole_tile(1, present1)) {
         qk(sa, k_stage(even));
-        if (!is_clean(0, present)) mask(sa, 0, present);
         raise(row_max(sa));
+        exp_first(sa, pa);
+        __syncthreads();   // iteration 0 replaces K(0)
+        auto iteration = [&](auto par, int t, f32x16 (&s)[NKB], f32x16 (&sn)[NKB], V8 (&pf)[PV_STEPS], V8 (&pn)[PV_STEPS]) __attribute__((always_inline)) {
+          constexpr int P = decltype(par)::value;
+          const std::integral_constant<int, P> cur{};
+          const std::integral_constant<int, 1 - P> nxt{};
+          // V(t+1) over V(t-1), K(t+2) over K(t); the rows of tile t + 3 are found inside phase A.
+          to_lds(c.v, v_rs, rows1, v_stage(nxt), true);
+          to_lds(c.k, k_rs, rows2, k_stage(cur), false);
+#pragma unroll
+          for (int i = 0; i < CPT; ++i) rows1[i] = rows2[i];
+          uint64_t present3 = 0;
+          int row3 = 0;
+          // The phases are laid out by hand, one MFMA and its share of the VALU work after another (the compiler's
+          // own order, and its scheduling groups, put the MFMAs first and the exponentials behind them).
+          // Phase A: S(t+1) with the second half of P(t).
+          __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_s_setprio(2);
+          {
+            constexpr int N = NKB * QK_STEPS, PER = HALF * 8 / 2 / N;   // MFMAs; pairs of exponentials for each (D = 128: 1/2)
+            const unsigned char* ks = k_stage(nxt);
+            int kb = k_base;
+            asm("" : "+v"(kb));
+            auto operand = [&](int i) { return *reinterpret_cast<const V8*>(ks + i % NKB * 32 * RB + (kb ^ (32 * (i / NKB)))); };
+            const float neg_m = neg_ref();
+            V8 ahead[2] = {operand(0), operand(1)};
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const V8 x = ahead[i % 2];
+              if (i + 2 < N) ahead[i % 2] = operand(i + 2);
+              sn[i % NKB] = mfma32x32x16(x, qf[i / NKB], i < NKB ? f32x16{} : sn[i % NKB]);
+              if constexpr (PER > 0) {
+#pragma unroll
+                for (int k = 0; k < PER; ++k) exp_pair(s, pf, HALF * 8 + 2 * (i * PER + k), neg_m);
+              } else if (i % 2) {
+                exp_pair(s, pf, HALF * 8 + i - 1, neg_m);
+              }
+              if (i == N / 4) {
+                row3 = find_row(t + 3, page);
+                present3 = present_of(row3);
+                page = load_page(t + 4);
+              }
+              if (i == N / 2) chunk_rows(row3, present3, rows2);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+          __builtin_amdgcn_s_setprio(0);
+          // Phase B: O += V(t) P(t) with the row sums of P(t), the row maxima of S(t+1) and the first half of P(t+1)
+          // against the reference as it is; where that is raised after all, the half is taken again.
+          float mx = -INFINITY;
+          {
+            constexpr int N = PV_STEPS * NDB, PER = HALF * 8 / 2 / N;
+            const unsigned char* vs = v_stage(cur);
+            int vb = v_base;
+            asm("" : "+v"(vb));
+            auto operand = [&](int i) {
+              const unsigned char* p = vs + i / NDB * 16 * RB + (vb ^ (64 * (i % NDB)));
+              const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p));
+              const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<i16x4>)(p + 8 * RB));
+              const i16x8 x = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+              return __builtin_bit_cast(V8, x);
+            };
+            const float neg_m = neg_ref();
+            V8 ahead[2] = {operand(0), operand(1)};
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const V8 x = ahead[i % 2];
+              if (i + 2 < N) ahead[i % 2] = operand(i + 2);
+              o[i % NDB] = mfma32x32x16(x, pf[i / NDB], o[i % NDB]);
+              if constexpr (PER > 0) {
+#pragma unroll
+                for (int k = 0; k < PER; ++k) exp_pair(sn, pn, 2 * (i * PER + k), neg_m);
+              } else if (i % 2) {
+                exp_pair(sn, pn, i - 1, neg_m);
+              }
+#pragma unroll
+              for (int k = 4 * PV_STEPS / N * i; k < 4 * PV_STEPS / N * (i + 1); ++k)
+                l = add_pair(__builtin_bit_cast(u32x4, pf[k / 4])[k % 4], l, static_cast<T*>(nullptr));
+#pragma unroll
+              for (int k = 16 * NKB / N * i; k < 16 * NKB / N * (i + 1); k += 2) mx = max_nan(mx, max_nan(sn[k / 16][k % 16], sn[k / 16][k % 16 + 1]));
+              __builtin_amdgcn_sched_barrier(0);
+            }
+            mx = max_nan(mx, partner32(mx)) * w.scale_log2;
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) asm volatile("" : "+v"(pn[i]));   // (not to be moved into the branches below)
+          }
+          if (raise(mx)) exp_first(sn, pn);
+          present = present1, present1 = present2, present2 = present3;
+          __builtin_amdgcn_s_waitcnt(0);
+          __syncthreads();
+        };
+        // (present, present1: tiles t0 and t0 + 1)
+        while (true) {
+          iteration(even, t0, sa, sb, pa, pb);
+          ++t0;
+          if (!whole_tile(t0 + 1, present1)) break;
+          iteration(odd, t0, sb, sa, pb, pa);
+          ++t0;
+          if (!whole_tile(t0 + 1, present1)) break;
+        }
       }
-      __syncthreads();   // iteration 0 replaces K(0)
     }
 
-    auto iteration = [&](auto par, int t, f32x16 (&s)[NKB], f32x16 (&sn)[NKB]) {
-      constexpr int P = decltype(par)::value;
-      const std::integral_constant<int, P> cur{};
-      const std::integral_constant<int, 1 - P> nxt{};
-      // Loads: K(t+2) over K(t), V(t+1) over V(t-1).
-      const int row2 = find_row(t + 2, page);
-      const uint64_t present2 = __builtin_amdgcn_ballot_w64(row2 >= 0);
-      page = load_page(t + 3);
-      int rows2[CPT];
-      chunk_rows(row2, rows2);
-      if (t + 1 < nt) {
-        to_lds(c.k, rows2, k_stage(cur), false);
-        to_lds(c.v, rows1, v_stage(nxt), true);
-      }
-      if (t < wave_tiles) {
-        V8 pf[PV_STEPS];
-        const bool clean = is_clean(t, present), more = t + 1 < wave_tiles;
-        // Phase A: S(t+1) with P(t). (Past the wave's last tile the product is of what the stage holds, and unused.)
-        __builtin_amdgcn_s_setprio(2);
-        qk(sn, k_stage(nxt));
-        exponentiate(s, pf);
-#pragma unroll
-        for (int i = 0; i < PV_STEPS; ++i) asm volatile("" : "+v"(pf[i]));   // (not to be moved past the branches below)
-        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
-#pragma unroll
-        for (int i = 0; i < NKB * QK_STEPS; ++i) {
-          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(kSchedValu, 96 / (NKB * QK_STEPS), 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(0);
-        if (more && !is_clean(t + 1, present1)) mask(sn, t + 1, present1);
-        if (!clean && skip_from == INT32_MAX && !values_finite(v_stage(cur))) skip_from = t;
-        // Phase B: O += V(t) P(t) with the row sums of P(t) and the row maxima of S(t+1).
-        float mx;
-        if (clean || skip_from == INT32_MAX) {
-          pv(pf, v_stage(cur));
-          row_sum(pf);
-          mx = row_max(sn);
-          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 4, 0);
-#pragma unroll
-          for (int i = 0; i < PV_STEPS * NDB; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(kSchedValu, 48 / (PV_STEPS * NDB), 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+    find_mine();
+    // ---- the other tiles, one by one (the other waves' MFMAs beside this one's VALU): the masked ones, and all
+    // 8-bit ones. K(t+1) and V(t+1) arrive meanwhile, 8-bit rows through registers.
+#pragma unroll 1
+    for (int t = t0; t < nt; ++t) {
+      const int P = t & 1;
+      unsigned char* const k_cur = P ? k_lds1 : k_lds0;
+      unsigned char* const v_cur = P ? v_lds1 : v_lds0;
+      unsigned char* const k_nxt = P ? k_lds0 : k_lds1;
+      unsigned char* const v_nxt = P ? v_lds0 : v_lds1;
+      const int row_nxt = row1;
+      const bool fetch = t + 1 < nt;
+      u32x4 kx[CPT], vx[CPT];
+      float scale_x = 0.f;
+      if (fetch) {
+        if constexpr (k8) {
+          to_regs(c.k, rows1, kx);
+          to_regs(c.v, rows1, vx);
+          if (wave == 0) scale_x = load_scale(c.k_scale, row_nxt);
+          if (wave == 1) scale_x = load_scale(c.v_scale, row_nxt);
         } else {
-          row_sum(pf);
-          mx = row_max(sn);
+          to_lds(c.k, k_rs, rows1, k_nxt, false);
+          to_lds(c.v, v_rs, rows1, v_nxt, true);
         }
-        if (!more) mx = -INFINITY;
-        raise(mx);
       }
-      present = present1, present1 = present2;
+      row1 = row2;
+      row2 = find_row(t + 3, page);
+      page = load_page(t + 4);
+      const uint64_t present3 = present_of(row2);
 #pragma unroll
       for (int i = 0; i < CPT; ++i) rows1[i] = rows2[i];
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-    };
-    // 8 bits: K(t+1) and V(t+1) come through registers; tile by tile, the other waves' MFMAs beside this one's VALU
-    // (with S(t+1) ahead as above, D = 128 spills 60 to 220 registers).
-    auto iteration8 = [&](auto par, int t) {
-      constexpr int P = decltype(par)::value;
-      const std::integral_constant<int, P> cur{};
-      const std::integral_constant<int, 1 - P> nxt{};
-      const int row_t1 = row1;
-      const bool fetch = t + 1 < nt;
-      if (fetch) {
-        to_regs(c.k, rows1, kx);
-        to_regs(c.v, rows1, vx);
-        if (wave == 0) scale_x = load_scale(c.k_scale, row_t1);
-        if (wave == 1) scale_x = load_scale(c.v_scale, row_t1);
-      }
-      row1 = find_row(t + 2, page);
-      page = load_page(t + 3);
-      chunk_rows(row1, rows1);
+      chunk_rows(row2, present3, rows2);
       if (t < wave_tiles) {
+        f32x16 s[NKB];
         V8 pf[PV_STEPS];
         const bool clean = is_clean(t, present);
-        qk(sa, k_stage(cur));
-        scale_scores(sa, P);
-        if (!clean) mask(sa, t, present);
-        raise(row_max(sa));
+        qk(s, k_cur);
+        scale_scores(s, P);
+        if (!clean) mask(s, t, present);
+        raise(row_max(s));
         if constexpr (kUnits) {
           const float top = uniform_f(top_lds[P]);
           if (top > vref) {
@@ -890,26 +1022,24 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
             for (int db = 0; db < NDB; ++db) o[db] *= f;
           }
         }
-        exponentiate8(sa, pf, P, clean, t, present);
-        if (!clean && skip_from == INT32_MAX && !values_finite(v_stage(cur))) skip_from = t;
-        if (clean || skip_from == INT32_MAX) pv(pf, v_stage(cur));
+        if constexpr (k8) exponentiate8(s, pf, P, clean, t, present); else exponentiate(s, pf);
+        if (!clean && skip_from == INT32_MAX && !values_finite(v_cur)) skip_from = t;
+        if (clean || skip_from == INT32_MAX) pv(pf, v_cur);
+        if constexpr (!k8) row_sum(pf);
       }
-      present = present1, present1 = __builtin_amdgcn_ballot_w64(row1 >= 0);
-      if (fetch) {
-        widen(kx, k_stage(nxt), false);
-        widen(vx, v_stage(nxt), true);
-        if (wave == 0) ks_lds[1 - P][lane] = row_t1 >= 0 ? scale_x * w.scale_log2 : 0.f;
-        store_v_scale(1 - P, row_t1, scale_x);
+      present = present1, present1 = present2, present2 = present3;
+      if constexpr (k8) {
+        if (fetch) {
+          widen(kx, k_nxt, false);
+          widen(vx, v_nxt, true);
+          if (wave == 0) ks_lds[1 - P][lane] = row_nxt >= 0 ? scale_x * w.scale_log2 : 0.f;
+          store_v_scale(1 - P, row_nxt, scale_x);
+        }
+      } else {
+        __builtin_amdgcn_s_waitcnt(0);
       }
       __syncthreads();
-    };
-    for (int t = 0; t < nt; t += 2) {
-      if constexpr (k8) iteration8(even, t); else iteration(even, t, sa, sb);
-      if (t + 1 < nt) {
-        if constexpr (k8) iteration8(odd, t + 1); else iteration(odd, t + 1, sb, sa);
-      }
     }
-
 
     // ---- P . V of the tiles left out, over the visible pairs alone: scores again, all in fp32
     if (skip_from < wave_tiles) {
@@ -947,6 +1077,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       }
     }
 
+    find_mine();
     // ---- the wave's 32 rows: done, or a part for the join. (The stages are free: every wave passed the last barrier.)
     const bool done = sg.from == 0 && sg.to == sg.steps;
     const int slot = sg.from == 0 ? 1 : 0;
@@ -1016,7 +1147,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedCache c, RowsQ a, At
   for (int r0 = (int)blockIdx.y * 16; r0 < ROWS; r0 += (int)gridDim.y * 16) {
     const int r = r0 + tr;
     int token, hq;
-    const bool mine = tile_row(w.tiles, s, rec.head, rec.tile, r, token, hq);
+    const bool mine = tile_row(w.tiles, s, rec.head, rec.tile, in_tile(w.tiles, r), token, hq);
     float m = -INFINITY, sum = 0.f, x[EL] = {};
     for (int p0 = 0; p0 < n; p0 += MOST) {
       float mi[MOST / 16], li[MOST / 16], top = -INFINITY, add = 0.f;

@@ -110,7 +110,7 @@ hipError_t launch_attn(Kernel kernel, int threads, const pa::PagedCache& c, cons
                        reinterpret_cast<float*>(static_cast<char*>(workspace) + pa::attn_record_bytes(plan.wgs))};
   hipLaunchKernelGGL(kernel, dim3((unsigned)plan.wgs), dim3(threads), 0, stream, c, a, w);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || plan.whole) return e;
-  hipLaunchKernelGGL((pa::paged_attn_join<T, D, ROWS>), dim3((unsigned)plan.wgs, ROWS > 64 ? ROWS / 32 : ROWS / 16), dim3(256), 0,
+  hipLaunchKernelGGL((pa::paged_attn_join<T, D, ROWS>), dim3((unsigned)plan.wgs, ROWS / 16), dim3(256), 0,
                      stream, c, a, w, plan.wgs);
   return hipGetLastError();
 }
@@ -196,8 +196,14 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
       case 16: return launch_attn<T, D, 16>(pa::paged_attn_few<T, C, D, 1>, 256, c, a, plan, causal, workspace, st);
       case 32: return launch_attn<T, D, 32>(pa::paged_attn_few<T, C, D, 2>, 256, c, a, plan, causal, workspace, st);
       case 64: return launch_attn<T, D, 64>(pa::paged_attn_few<T, C, D, 4>, 256, c, a, plan, causal, workspace, st);
-      default: return launch_attn<T, D, CR>(pa::paged_attn_chunk<T, C, D, CR>, 2 * CR, c, a, plan, causal, workspace, st);
+      default: break;
     }
+    if constexpr (!pa::cache_type<C>::k8bit) {
+      const uint64_t bytes = (uint64_t)c.pages * c.heads * c.page_size * D * sizeof(T);
+      if (bytes > pa::kPastBuffer)
+        return launch_attn<T, D, CR>(pa::paged_attn_chunk<T, C, D, CR, true>, 2 * CR, c, a, plan, causal, workspace, st);
+    }
+    return launch_attn<T, D, CR>(pa::paged_attn_chunk<T, C, D, CR, false>, 2 * CR, c, a, plan, causal, workspace, st);
   });
   return hip_status(e, name);
 }

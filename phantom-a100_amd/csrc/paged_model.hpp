@@ -97,42 +97,55 @@ struct Segment {
   SeqRows rows;
   int seq, head, tile, from, to, steps;
 };
-// The segments of units [at, end), from sequence `seq` (whose units begin at `begin`) on. load(s) gives a
-// sequence's rows. whole: tiles are not cut, one belongs to the workgroup whose units hold its first.
+// The segments of units [at, end). Starts at sequence `seq`, whose units begin at `begin`; load(s) gives a
+// sequence's rows. The first segment is searched for, each next one follows from the last without a division.
+// whole: tiles are not cut, one belongs to the workgroup whose units hold its first.
 struct WorkWalk {
   TileShape tiles;
   int seqs, heads, capacity;   // heads: key/value heads times splits
   bool causal, whole;
-  int64_t at, end, begin;
+  int64_t at, end, begin;      // begin: of the current tile (before the first segment, of the sequence)
   int seq;
+  int head = 0, tile = -1, count = 0;   // the current tile, and the sequence's tiles; -1: before the first
+  SeqRows rows = {0, 0, 0};
 
   template <typename Load>
-  __host__ __device__ bool next(Load load, Segment& out) {
-    while (at < end && seq < seqs) {
-      const SeqRows s = load(seq);
-      const int n = tiles_of(s, tiles);
-      const int64_t per_head = tiles_cost(s, tiles, causal, n), all = per_head * heads;
-      if (at >= begin + all) {
-        begin += all;
-        ++seq;
-        continue;
+  __host__ __device__ __forceinline__ bool next(Load load, Segment& out) {
+    while (at < end) {
+      if (tile < 0) {
+        rows = load(seq);
+        count = tiles_of(rows, tiles);
+        if (count == 0) return false;   // (no sequence holds `at`)
+        const int64_t per_head = tiles_cost(rows, tiles, causal, count), r = at - begin;
+        head = (int)(r / per_head);
+        const int64_t in_head = r - head * per_head;
+        tile = 0;   // the last tile that begins at or before in_head
+        for (int hi = count - 1; tile < hi;) {
+          const int mid = tile + (hi - tile + 1) / 2;
+          if (tiles_cost(rows, tiles, causal, mid) <= in_head) tile = mid; else hi = mid - 1;
+        }
+        begin += head * per_head + tiles_cost(rows, tiles, causal, tile);
+      } else if (++tile == count) {
+        tile = 0;
+        if (++head == heads) {
+          head = 0;
+          do {
+            if (++seq >= seqs) return false;
+            rows = load(seq);
+            count = tiles_of(rows, tiles);
+          } while (count == 0);
+        }
       }
-      const int64_t r = at - begin;
-      const int head = (int)(r / per_head);
-      const int64_t in_head = r - head * per_head;
-      int tile = 0;   // the last tile that begins at or before in_head
-      for (int hi = n - 1; tile < hi;) {
-        const int mid = tile + (hi - tile + 1) / 2;
-        if (tiles_cost(s, tiles, causal, mid) <= in_head) tile = mid; else hi = mid - 1;
-      }
-      const int64_t t0 = begin + head * per_head + tiles_cost(s, tiles, causal, tile);
-      const int64_t t1 = begin + head * per_head + tiles_cost(s, tiles, causal, tile + 1);
-      const int steps = tile_steps(s, tiles, tile, capacity, causal);
+      const int64_t t0 = begin, last = (int64_t)(tile + 1) * tiles.tokens;
+      const int before = rows.length - rows.count;
+      const int64_t t1 = t0 + kTileCost + (causal ? (before > 0 ? before : 0) + (last < rows.count ? last : rows.count) : rows.length);
+      const int steps = tile_steps(rows, tiles, tile, capacity, causal);
       const int64_t from = at == t0 ? 0 : whole ? steps : (at - t0) / kStep;
       const int64_t to = end >= t1 || whole ? steps : (end - t0) / kStep;
       at = t1 < end ? t1 : end;
+      begin = t1;
       if (from < to && from < steps) {
-        out = {s, seq, head, tile, (int)from, (int)(to < steps ? to : steps), steps};
+        out = {rows, seq, head, tile, (int)from, (int)(to < steps ? to : steps), steps};
         return true;
       }
     }
