@@ -561,7 +561,10 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   __shared__ __attribute__((aligned(1024))) unsigned char v_lds0[TILE_BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char k_lds1[TILE_BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char v_lds1[TILE_BYTES];
-  __shared__ __attribute__((aligned(16))) float ks_lds[2][BN], vs_lds[2][BN], top_lds[2];
+  // 8 bits: rows as they are, each thread's own, on their way to the stages; and four tiles' scales.
+  constexpr int RAW = k8 && !WIDE ? BN * CB : 16, SLOTS = k8 ? 4 : 1;
+  __shared__ __attribute__((aligned(1024))) unsigned char k_raw0[RAW], k_raw1[RAW], v_raw0[RAW], v_raw1[RAW];
+  __shared__ __attribute__((aligned(256))) float ks_lds[SLOTS][BN], vs_lds[SLOTS][BN];
   __shared__ int64_t walk_lds[10];
   const std::integral_constant<int, 0> even{};
   const std::integral_constant<int, 1> odd{};
@@ -576,6 +579,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   int k_base = lq * RB + ((hi ^ k_swz<CR>(lq)) * 16), v_base = v_row * RB + ((v_cl ^ v_swz<CR>(v_row)) * 16) + 8 * (i16 % 2);
   const uint32_t cache_bytes = (uint32_t)min((uint64_t)c.pages * c.heads * c.page_size * CB, (uint64_t)kPastBuffer);
   const rsrc_t k_rs = make_rsrc(c.k, cache_bytes), v_rs = make_rsrc(c.v, cache_bytes);
+  const uint32_t scale_bytes = k8 ? (uint32_t)min((uint64_t)c.pages * c.heads * c.page_size * 4, (uint64_t)kPastBuffer) : 0;
+  const rsrc_t ks_rs = make_rsrc(k8 ? c.k_scale : nullptr, scale_bytes), vs_rs = make_rsrc(k8 ? c.v_scale : nullptr, scale_bytes);
 
   PartRecord rec = {0, 0, 0, 0};
   WorkWalk walk;
@@ -643,12 +648,16 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         }
       }
     };
-    // 8-bit rows: load, then widen and store.
-    auto to_regs = [&](const void* cache, const int (&rows)[CPT], u32x4 (&x)[CPT]) {
-#pragma unroll
-      for (int i = 0; i < CPT; ++i)
-        x[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(cache) + (uint64_t)(unsigned)rows[i] * CB + tid % LPR * 16);
+    // 8-bit rows: through registers, or into the thread's 16 bytes of a raw buffer; then widened and stored.
+    static_assert(!k8 || CPT == 1, "one load of 8-bit rows a thread");
+    auto to_regs = [&](const void* cache, rsrc_t rs, const int (&rows)[CPT], u32x4 (&x)[CPT]) {
+      if constexpr (WIDE) x[0] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(cache) + (uint64_t)(unsigned)rows[0] * CB + tid % LPR * 16);
+      else x[0] = load16(rs, (unsigned)rows[0] + tid % LPR * 16);
     };
+    auto to_raw = [&](rsrc_t rs, const int (&rows)[CPT], unsigned char* raw) {
+      load16_to_lds(rs, raw + wave * kWave * 16, (unsigned)rows[0] + tid % LPR * 16, 0);
+    };
+    auto from_raw = [&](const unsigned char* raw, u32x4 (&x)[CPT]) { x[0] = *reinterpret_cast<const u32x4*>(raw + tid * 16); };
     auto widen = [&](const u32x4 (&x)[CPT], unsigned char* stage, bool is_v) {
       if constexpr (k8)
 #pragma unroll
@@ -666,7 +675,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     // buffer's end (which loads as zeros) for an absent key. Elsewhere an absent key takes the row of the tile's
     // first present one: its scores are masked, and its P is 0, which a finite value leaves without effect.
     auto chunk_rows = [&](int row, uint64_t pres, int (&rows)[CPT]) {
-      if constexpr (k8 || WIDE) {
+      if constexpr (WIDE) {
         const int first = max(__builtin_amdgcn_readlane(row, __builtin_ctzll(pres | 1ull << 63)), 0);
         row = row < 0 ? first : row;
       } else {
@@ -675,18 +684,19 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
       for (int i = 0; i < CPT; ++i) rows[i] = __shfl(row, (i * THREADS + tid) / LPR);
     };
-    // A tile's scales by lane = key (wave 0 the keys', wave 1 the values').
-    auto load_scale = [&](const float* scales, int row) { return scales[max(row, 0)]; };
-    auto store_v_scale = [&](int par, int row, float x) {
-      if (wave == 1) {
-        vs_lds[par][lane] = row >= 0 ? x : 0.f;
-        if constexpr (kUnits) {
-          const float top = wave_allreduce(row >= 0 && fabsf(x) < INFINITY ? fabsf(x) : 0.f, MaxOp{});
-          if (lane == 0) top_lds[par] = top;
-        }
-      }
+    // A tile's scales by lane = key, into its slot: wave 0 the keys', wave 1 the values'. Absent keys get zeros.
+    auto load_scale = [&](int row) {
+      const float x = wave < 2 && row >= 0 ? (wave ? c.v_scale : c.k_scale)[row] : 0.f;
+      return x;
     };
-
+    auto store_scale = [&](int t, float x) {
+      if (wave < 2) (wave ? vs_lds : ks_lds)[t % SLOTS][lane] = x;
+    };
+    auto scales_to_lds = [&](int t, int row) {   // (4 bytes a lane)
+      if (wave < 2)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wave ? vs_rs : ks_rs, (__attribute__((address_space(3))) void*)&(wave ? vs_lds : ks_lds)[t % SLOTS][0],
+                                                 4, row < 0 ? kPastBuffer : (unsigned)row * 4, 0, 0, 0);
+    };
     // The wave's first tile that is not clean and has a value that is not finite: from there on, tiles that are
     // not clean leave P . V out, and take_visible adds it at the end.
     int skip_from = INT32_MAX;
@@ -707,14 +717,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         for (int b = 0; b < NKB; ++b)
           s[b] = mfma32x32x16(*reinterpret_cast<const V8*>(ks + b * 32 * RB + (kb ^ (32 * kk))), qf[kk], s[b]);
     };
-    // Keys' scales (8 bits; with log2(e)/sqrt(d), so that scores are in the exponent's units).
-    auto scale_scores = [&](f32x16 (&s)[NKB], int par) {
+    // Keys' scales.
+    auto scale_scores = [&](f32x16 (&s)[NKB], int t) {
       if constexpr (k8)
 #pragma unroll
         for (int b = 0; b < NKB; ++b)
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(&ks_lds[par][32 * b + 8 * q4 + 4 * hi]);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&ks_lds[t % SLOTS][32 * b + 8 * q4 + 4 * hi]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[b][4 * q4 + r] *= x[r];
           }
@@ -745,7 +755,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; r += 2) mx = max_nan(mx, max_nan(s[b][r], s[b][r + 1]));
-      return max_nan(mx, partner32(mx)) * (k8 ? 1.f : w.scale_log2);
+      return max_nan(mx, partner32(mx)) * w.scale_log2;
     };
     auto raise = [&](float mx) {   // the reference maximum, where some row's grew past 2^8: whether it did
       const float m_new = fmaxf(m_run, mx);
@@ -766,25 +776,36 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) pf[b * 2 + r / 8][r % 8] = from_f32<T>(exp2_fast(fmaf(s[b][r], w.scale_log2, neg_m)));
     };
-    // 8 bits: l takes P, the product P times the values' scales.
-    auto exponentiate8 = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int par, bool clean, int t, uint64_t present) {
+    // 8 bits: l takes P, the product P times the values' scales (in fp16 in units of vref, the largest scale so
+    // far, in which O is held: P times a scale must stay in the type's range).
+    auto exponentiate8 = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t, auto masked, const Bits& v) __attribute__((always_inline)) {
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
       const float unit = kUnits ? 1.f / vref : 1.f;
-      const Bits v = clean ? Bits{{~0u, ~0u}} : visible(t, present);
 #pragma unroll
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(&vs_lds[par][32 * b + 8 * q4 + 4 * hi]);
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&vs_lds[t % SLOTS][32 * b + 8 * q4 + 4 * hi]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float p = exp2_fast(s[b][4 * q4 + r] + neg_m);
+            float p = exp2_fast(fmaf(s[b][4 * q4 + r], w.scale_log2, neg_m));
             l += p;
             p *= kUnits ? x[r] * unit : x[r];
-            if (!clean) p = v.b[b] & 1u << (8 * q4 + r) ? p : 0.f;   // (0 x a scale that is not finite)
+            if constexpr (decltype(masked)::value) p = v.b[b] & 1u << (8 * q4 + r) ? p : 0.f;   // (0 x a scale that is not finite)
             pf[b * 2 + q4 / 2][(q4 % 2) * 4 + r] = from_f32<T>(p);
           }
         }
+    };
+    auto raise_units = [&](int t) {   // vref, where tile t has a larger scale: whether it did
+      if constexpr (!kUnits) return false;
+      const float x = fabsf(vs_lds[t % SLOTS][lane]);
+      const float top = uniform_f(wave_allreduce(x < INFINITY ? x : 0.f, MaxOp{}));
+      if (top <= vref) return false;
+      const float f = vref / top;
+      vref = top;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) o[db] *= f;
+      return true;
     };
     auto pv = [&](const V8 (&pf)[PV_STEPS], const unsigned char* vs) {
       int vb = v_base;
@@ -818,78 +839,128 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
     auto is_clean = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= wave_all; };
 
-    // ---- the first tiles: K(0), V(0), K(1). At a tile t: rows1, row1 and present1 are tile t + 1's, rows2, row2 and
-    // present2 tile t + 2's, page holds tile t + 3's entries.
-    int page = load_page(0), page1 = load_page(1), page2 = load_page(2);
-    int row = find_row(0, page), row1 = find_row(1, page1), row2 = find_row(2, page2);
-    page = load_page(3);
-    uint64_t present = present_of(row), present1 = present_of(row1), present2 = present_of(row2);
-    int rows1[CPT], rows2[CPT];
+    // ---- the first tiles: K(0), V(0), K(1). At a tile t: rows[j] and row[j] are tile t + 1 + j's, present[j] tile
+    // t + j's; page holds tile t + 1 + AHEAD's entries.
+    constexpr int AHEAD = k8 ? 3 : 2;
+    int page, row[AHEAD], rows[AHEAD][CPT];
+    uint64_t present[AHEAD + 1];
+    const int tile_all = keys_seen(sg.rows, sg.tile * w.tiles.tokens, c.capacity, w.causal);   // the first row's keys
+    auto whole_tile = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= tile_all; };
+    auto advance = [&](int next_row, uint64_t next_present) {   // to the next tile (its new rows[AHEAD - 1] apart)
+#pragma unroll
+      for (int j = 0; j + 1 < AHEAD; ++j) {
+        row[j] = row[j + 1];
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) rows[j][i] = rows[j + 1][i];
+      }
+      row[AHEAD - 1] = next_row;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) present[j] = present[j + 1];
+      present[AHEAD] = next_present;
+    };
+    bool pipelined;
     {
-      int rows[CPT];
-      chunk_rows(row, present, rows);
-      chunk_rows(row1, present1, rows1);
-      chunk_rows(row2, present2, rows2);
+      int pages[AHEAD + 1], row0, rows0[CPT];
+#pragma unroll
+      for (int j = 0; j <= AHEAD; ++j) pages[j] = load_page(j);
+      page = load_page(AHEAD + 1);
+      row0 = find_row(0, pages[0]);
+      present[0] = present_of(row0);
+      chunk_rows(row0, present[0], rows0);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        row[j] = find_row(j + 1, pages[j + 1]);
+        present[j + 1] = present_of(row[j]);
+        chunk_rows(row[j], present[j + 1], rows[j]);
+      }
+      pipelined = !(k8 && WIDE) && whole_tile(0, present[0]) && whole_tile(1, present[1]);
       if constexpr (k8) {
-        u32x4 kx[CPT], vx[CPT];
-        to_regs(c.k, rows, kx);
-        to_regs(c.v, rows, vx);
-        if (wave == 0) ks_lds[0][lane] = row >= 0 ? load_scale(c.k_scale, row) * w.scale_log2 : 0.f;
-        if (wave == 1) store_v_scale(0, row, load_scale(c.v_scale, row));
+        u32x4 kx[CPT], vx[CPT], k1[CPT];
+        to_regs(c.k, k_rs, rows0, kx);
+        to_regs(c.v, v_rs, rows0, vx);
+        const float scale = load_scale(row0);
+        if constexpr (!WIDE) {
+          if (pipelined) {   // K(1), K(2) and V(1) too
+            to_regs(c.k, k_rs, rows[0], k1);
+            scales_to_lds(1, row[0]);
+            to_raw(k_rs, rows[1], k_raw0);
+            to_raw(v_rs, rows[0], v_raw1);
+            widen(k1, k_stage(odd), false);
+          }
+        }
+        store_scale(0, scale);
         widen(kx, k_stage(even), false);
         widen(vx, v_stage(even), true);
       } else {
-        to_lds(c.k, k_rs, rows, k_stage(even), false);
-        to_lds(c.v, v_rs, rows, v_stage(even), true);
-        to_lds(c.k, k_rs, rows1, k_stage(odd), false);
+        to_lds(c.k, k_rs, rows0, k_stage(even), false);
+        to_lds(c.v, v_rs, rows0, v_stage(even), true);
+        to_lds(c.k, k_rs, rows[0], k_stage(odd), false);
       }
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
 
-    // ---- the leading tiles that every row sees whole, in the two-stage pipeline (16-bit rows)
+    // ---- the leading tiles that every row sees whole, in the two-stage pipeline
     int t0 = 0;   // tiles done
-    if constexpr (!k8) {
-      const int tile_all = keys_seen(sg.rows, sg.tile * w.tiles.tokens, c.capacity, w.causal);   // the first row's keys
-      auto whole_tile = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= tile_all; };
+    if constexpr (!(k8 && WIDE)) {
       constexpr int HALF = PV_STEPS / 2;
-      // P of scores e and e + 1 (e even; 16-key step e / 8).
-      auto exp_pair = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int e, float neg_m) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = e; k < e + 2; ++k)
-          pf[k / 8][k % 8] = from_f32<T>(exp2_fast(fmaf(s[k / 16][k % 16], w.scale_log2, neg_m)));
-      };
       auto neg_ref = [&]() { return m_run == -INFINITY ? 0.f : -m_run; };
-      auto exp_first = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS]) __attribute__((always_inline)) {
-        const float neg_m = neg_ref();
+      // P of four scores, e to e + 3 (16-key step e / 8), of tile t; 8 bits: its sum to `sum`.
+      auto exp_quad = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int e, float neg_m, int t, float unit, float& sum) __attribute__((always_inline)) {
+        f32x4 x = {1.f, 1.f, 1.f, 1.f};
+        if constexpr (k8) x = *reinterpret_cast<const f32x4*>(&vs_lds[t % SLOTS][e / 16 * 32 + e % 16 * 2 + 4 * hi]);
 #pragma unroll
-        for (int e = 0; e < HALF * 8; e += 2) exp_pair(s, pf, e, neg_m);
+        for (int k = 0; k < 4; ++k) {
+          float p = exp2_fast(fmaf(s[e / 16][e % 16 + k], w.scale_log2, neg_m));
+          if constexpr (k8) {
+            sum += p;
+            p *= kUnits ? x[k] * unit : x[k];
+          }
+          pf[e / 8][e % 8 + k] = from_f32<T>(p);
+        }
+      };
+      float l_next = 0.f;   // 8 bits: the sum of the first half of P(t + 1)
+      auto exp_first = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t) __attribute__((always_inline)) {
+        const float neg_m = neg_ref(), unit = kUnits ? 1.f / vref : 1.f;
+        l_next = 0.f;
+#pragma unroll
+        for (int e = 0; e < HALF * 8; e += 4) exp_quad(s, pf, e, neg_m, t, unit, l_next);
       };
       f32x16 sa[NKB], sb[NKB];
       V8 pa[PV_STEPS], pb[PV_STEPS];
-      if (whole_tile(0, present) && whole_tile(1, present1)) {
+      if (pipelined) {
         qk(sa, k_stage(even));
+        scale_scores(sa, 0);
         raise(row_max(sa));
-        exp_first(sa, pa);
+        raise_units(0);
+        exp_first(sa, pa, 0);
         __syncthreads();   // iteration 0 replaces K(0)
         auto iteration = [&](auto par, int t, f32x16 (&s)[NKB], f32x16 (&sn)[NKB], V8 (&pf)[PV_STEPS], V8 (&pn)[PV_STEPS]) __attribute__((always_inline)) {
           constexpr int P = decltype(par)::value;
           const std::integral_constant<int, P> cur{};
           const std::integral_constant<int, 1 - P> nxt{};
-          // V(t+1) over V(t-1), K(t+2) over K(t); the rows of tile t + 3 are found inside phase A.
-          to_lds(c.v, v_rs, rows1, v_stage(nxt), true);
-          to_lds(c.k, k_rs, rows2, k_stage(cur), false);
-#pragma unroll
-          for (int i = 0; i < CPT; ++i) rows1[i] = rows2[i];
-          uint64_t present3 = 0;
-          int row3 = 0;
+          // 16 bits: V(t+1) over V(t-1), K(t+2) over K(t). 8 bits: these come out of the raw buffers in phase B, while
+          // V(t+2) and K(t+3) come into the others. The rows of tile t + 1 + AHEAD are found inside phase A.
+          if constexpr (k8) {
+            to_raw(v_rs, rows[1], P ? v_raw1 : v_raw0);
+            to_raw(k_rs, rows[2], P ? k_raw0 : k_raw1);
+            scales_to_lds(t + 2, row[1]);
+            l += l_next;
+            l_next = 0.f;
+          } else {
+            to_lds(c.v, v_rs, rows[0], v_stage(nxt), true);
+            to_lds(c.k, k_rs, rows[1], k_stage(cur), false);
+          }
+          uint64_t present_new = 0;
+          int row_new = 0;
+          const float unit = kUnits ? 1.f / vref : 1.f;
           // The phases are laid out by hand, one MFMA and its share of the VALU work after another (the compiler's
           // own order, and its scheduling groups, put the MFMAs first and the exponentials behind them).
           // Phase A: S(t+1) with the second half of P(t).
           __builtin_amdgcn_sched_barrier(0);
           __builtin_amdgcn_s_setprio(2);
           {
-            constexpr int N = NKB * QK_STEPS, PER = HALF * 8 / 2 / N;   // MFMAs; pairs of exponentials for each (D = 128: 1/2)
+            constexpr int N = NKB * QK_STEPS, EACH = N / 4;   // MFMAs; four exponentials after each EACH of them
             const unsigned char* ks = k_stage(nxt);
             int kb = k_base;
             asm("" : "+v"(kb));
@@ -901,18 +972,16 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
               const V8 x = ahead[i % 2];
               if (i + 2 < N) ahead[i % 2] = operand(i + 2);
               sn[i % NKB] = mfma32x32x16(x, qf[i / NKB], i < NKB ? f32x16{} : sn[i % NKB]);
-              if constexpr (PER > 0) {
-#pragma unroll
-                for (int k = 0; k < PER; ++k) exp_pair(s, pf, HALF * 8 + 2 * (i * PER + k), neg_m);
-              } else if (i % 2) {
-                exp_pair(s, pf, HALF * 8 + i - 1, neg_m);
-              }
+              if (i % EACH == EACH - 1) exp_quad(s, pf, HALF * 8 + i / EACH * 4, neg_m, t, unit, l);
               if (i == N / 4) {
-                row3 = find_row(t + 3, page);
-                present3 = present_of(row3);
-                page = load_page(t + 4);
+                row_new = find_row(t + 1 + AHEAD, page);
+                present_new = present_of(row_new);
+                page = load_page(t + 2 + AHEAD);
               }
-              if (i == N / 2) chunk_rows(row3, present3, rows2);
+              if (i == N / 2) {
+                advance(row_new, present_new);
+                chunk_rows(row_new, present_new, rows[AHEAD - 1]);
+              }
               __builtin_amdgcn_sched_barrier(0);
             }
           }
@@ -921,7 +990,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           // against the reference as it is; where that is raised after all, the half is taken again.
           float mx = -INFINITY;
           {
-            constexpr int N = PV_STEPS * NDB, PER = HALF * 8 / 2 / N;
+            constexpr int N = PV_STEPS * NDB, EACH = N / 4;
+            u32x4 kx[CPT], vx[CPT];
             const unsigned char* vs = v_stage(cur);
             int vb = v_base;
             asm("" : "+v"(vb));
@@ -939,43 +1009,54 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
               const V8 x = ahead[i % 2];
               if (i + 2 < N) ahead[i % 2] = operand(i + 2);
               o[i % NDB] = mfma32x32x16(x, pf[i / NDB], o[i % NDB]);
-              if constexpr (PER > 0) {
 #pragma unroll
-                for (int k = 0; k < PER; ++k) exp_pair(sn, pn, 2 * (i * PER + k), neg_m);
-              } else if (i % 2) {
-                exp_pair(sn, pn, i - 1, neg_m);
+              for (int k = 16 * NKB / N * i; k < 16 * NKB / N * (i + 1); k += 2) {
+                if constexpr (k8) {   // (four scores at a time)
+                  if (k % 4 == 0) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(&ks_lds[(t + 1) % SLOTS][k / 16 * 32 + k % 16 * 2 + 4 * hi]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sn[k / 16][k % 16 + r] *= x[r];
+                  }
+                }
+                mx = max_nan(mx, max_nan(sn[k / 16][k % 16], sn[k / 16][k % 16 + 1]));
               }
+              if (i % EACH == EACH - 1) exp_quad(sn, pn, i / EACH * 4, neg_m, t + 1, unit, l_next);
+              if constexpr (k8) {
+                if (i == 0) from_raw(P ? k_raw1 : k_raw0, kx);
+                if (i == N / 4) widen(kx, k_stage(cur), false);
+                if (i == N / 2) from_raw(P ? v_raw0 : v_raw1, vx);
+                if (i == N / 2 + N / 4) widen(vx, v_stage(nxt), true);
+              } else {
 #pragma unroll
-              for (int k = 4 * PV_STEPS / N * i; k < 4 * PV_STEPS / N * (i + 1); ++k)
-                l = add_pair(__builtin_bit_cast(u32x4, pf[k / 4])[k % 4], l, static_cast<T*>(nullptr));
-#pragma unroll
-              for (int k = 16 * NKB / N * i; k < 16 * NKB / N * (i + 1); k += 2) mx = max_nan(mx, max_nan(sn[k / 16][k % 16], sn[k / 16][k % 16 + 1]));
+                for (int k = 4 * PV_STEPS / N * i; k < 4 * PV_STEPS / N * (i + 1); ++k)
+                  l = add_pair(__builtin_bit_cast(u32x4, pf[k / 4])[k % 4], l, static_cast<T*>(nullptr));
+              }
               __builtin_amdgcn_sched_barrier(0);
             }
             mx = max_nan(mx, partner32(mx)) * w.scale_log2;
 #pragma unroll
             for (int i = 0; i < HALF; ++i) asm volatile("" : "+v"(pn[i]));   // (not to be moved into the branches below)
           }
-          if (raise(mx)) exp_first(sn, pn);
-          present = present1, present1 = present2, present2 = present3;
+          const bool again = raise(mx), units = raise_units(t + 1);
+          if (again || units) exp_first(sn, pn, t + 1);
           __builtin_amdgcn_s_waitcnt(0);
           __syncthreads();
         };
-        // (present, present1: tiles t0 and t0 + 1)
+        // (present[0] and present[1]: tiles t0 and t0 + 1)
         while (true) {
           iteration(even, t0, sa, sb, pa, pb);
           ++t0;
-          if (!whole_tile(t0 + 1, present1)) break;
+          if (!whole_tile(t0 + 1, present[1])) break;
           iteration(odd, t0, sb, sa, pb, pa);
           ++t0;
-          if (!whole_tile(t0 + 1, present1)) break;
+          if (!whole_tile(t0 + 1, present[1])) break;
         }
       }
     }
 
     find_mine();
-    // ---- the other tiles, one by one (the other waves' MFMAs beside this one's VALU): the masked ones, and all
-    // 8-bit ones. K(t+1) and V(t+1) arrive meanwhile, 8-bit rows through registers.
+    // ---- the other tiles, one by one (the other waves' MFMAs beside this one's VALU), the masked ones above all.
+    // K(t+1) and V(t+1) arrive meanwhile, 8-bit rows through registers.
 #pragma unroll 1
     for (int t = t0; t < nt; ++t) {
       const int P = t & 1;
@@ -983,57 +1064,51 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       unsigned char* const v_cur = P ? v_lds1 : v_lds0;
       unsigned char* const k_nxt = P ? k_lds0 : k_lds1;
       unsigned char* const v_nxt = P ? v_lds0 : v_lds1;
-      const int row_nxt = row1;
       const bool fetch = t + 1 < nt;
       u32x4 kx[CPT], vx[CPT];
-      float scale_x = 0.f;
+      float scale = 0.f;
       if (fetch) {
         if constexpr (k8) {
-          to_regs(c.k, rows1, kx);
-          to_regs(c.v, rows1, vx);
-          if (wave == 0) scale_x = load_scale(c.k_scale, row_nxt);
-          if (wave == 1) scale_x = load_scale(c.v_scale, row_nxt);
+          to_regs(c.k, k_rs, rows[0], kx);
+          to_regs(c.v, v_rs, rows[0], vx);
+          scale = load_scale(row[0]);
         } else {
-          to_lds(c.k, k_rs, rows1, k_nxt, false);
-          to_lds(c.v, v_rs, rows1, v_nxt, true);
+          to_lds(c.k, k_rs, rows[0], k_nxt, false);
+          to_lds(c.v, v_rs, rows[0], v_nxt, true);
         }
       }
-      row1 = row2;
-      row2 = find_row(t + 3, page);
-      page = load_page(t + 4);
-      const uint64_t present3 = present_of(row2);
-#pragma unroll
-      for (int i = 0; i < CPT; ++i) rows1[i] = rows2[i];
-      chunk_rows(row2, present3, rows2);
+      const uint64_t pres = present[0];
+      {
+        const int row_new = find_row(t + 1 + AHEAD, page);
+        page = load_page(t + 2 + AHEAD);
+        const uint64_t present_new = present_of(row_new);
+        advance(row_new, present_new);
+        chunk_rows(row_new, present_new, rows[AHEAD - 1]);
+      }
       if (t < wave_tiles) {
         f32x16 s[NKB];
         V8 pf[PV_STEPS];
-        const bool clean = is_clean(t, present);
+        const bool clean = is_clean(t, pres);
         qk(s, k_cur);
-        scale_scores(s, P);
-        if (!clean) mask(s, t, present);
+        scale_scores(s, t);
+        if (!clean) mask(s, t, pres);
         raise(row_max(s));
-        if constexpr (kUnits) {
-          const float top = uniform_f(top_lds[P]);
-          if (top > vref) {
-            const float f = vref / top;
-            vref = top;
-#pragma unroll
-            for (int db = 0; db < NDB; ++db) o[db] *= f;
-          }
+        raise_units(t);
+        if constexpr (k8) {
+          if (clean) exponentiate8(s, pf, t, std::false_type{}, Bits{});
+          else exponentiate8(s, pf, t, std::true_type{}, visible(t, pres));
+        } else {
+          exponentiate(s, pf);
         }
-        if constexpr (k8) exponentiate8(s, pf, P, clean, t, present); else exponentiate(s, pf);
         if (!clean && skip_from == INT32_MAX && !values_finite(v_cur)) skip_from = t;
         if (clean || skip_from == INT32_MAX) pv(pf, v_cur);
         if constexpr (!k8) row_sum(pf);
       }
-      present = present1, present1 = present2, present2 = present3;
       if constexpr (k8) {
         if (fetch) {
           widen(kx, k_nxt, false);
           widen(vx, v_nxt, true);
-          if (wave == 0) ks_lds[1 - P][lane] = row_nxt >= 0 ? scale_x * w.scale_log2 : 0.f;
-          store_v_scale(1 - P, row_nxt, scale_x);
+          store_scale(t + 1, scale);
         }
       } else {
         __builtin_amdgcn_s_waitcnt(0);

@@ -198,11 +198,9 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
       case 64: return launch_attn<T, D, 64>(pa::paged_attn_few<T, C, D, 4>, 256, c, a, plan, causal, workspace, st);
       default: break;
     }
-    if constexpr (!pa::cache_type<C>::k8bit) {
-      const uint64_t bytes = (uint64_t)c.pages * c.heads * c.page_size * D * sizeof(T);
-      if (bytes > pa::kPastBuffer)
-        return launch_attn<T, D, CR>(pa::paged_attn_chunk<T, C, D, CR, true>, 2 * CR, c, a, plan, causal, workspace, st);
-    }
+    const uint64_t cache_rows = (uint64_t)c.pages * c.heads * c.page_size;
+    if (cache_rows * std::max<size_t>(D * sizeof(C), 4) > pa::kPastBuffer)
+      return launch_attn<T, D, CR>(pa::paged_attn_chunk<T, C, D, CR, true>, 2 * CR, c, a, plan, causal, workspace, st);
     return launch_attn<T, D, CR>(pa::paged_attn_chunk<T, C, D, CR, false>, 2 * CR, c, a, plan, causal, workspace, st);
   });
   return hip_status(e, name);
