@@ -1160,38 +1160,63 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       if (sg.from == 0) rec = {sg.seq, sg.head, sg.tile, rec.flags | kPartBegins};
       else rec.flags |= kPartContinues | (sg.to == sg.steps ? kPartEnds : 0);
     }
+    {
+    // Each wave turns its rows round in LDS of its own (a quarter or an eighth of the stages, chunks swizzled by
+    // row), so that whole rows are stored, 16 bytes a lane; a lane's pieces stored as they are cost ~4 us a tile.
+    int ln = (int)threadIdx.x % kWave;   // (offsets made from it are not to be hoisted out of the segments' loop)
+    asm volatile("" : "+v"(ln));
+    const int lq = ln % 32, hi = ln / 32, lane = ln;
     const float sum = half_sum(l);
-    if (mine) {
-      if (done) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        T* to = static_cast<T*>(a.o) + (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head + 4 * hi;
+    const float factor = done ? (sum == 0.f ? 0.f : (kUnits ? vref : 1.f) / sum) : kUnits ? vref : 1.f;
+    constexpr int PASSES = 2;   // fp32 rows: half of the wave's rows at a time
+    unsigned char* const own = (wave % 4 == 0 ? k_lds0 : wave % 4 == 1 ? v_lds0 : wave % 4 == 2 ? k_lds1 : v_lds1) + wave / 4 * (32 * RB);
+    if (done) {
+      const int64_t offset = mine ? (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head : -1;
+      typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            T4 x;
+        for (int q4 = 0; q4 < 4; ++q4) {
+          T4 x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = from_f32<T>(sum == 0.f ? 0.f : o[db][4 * q4 + r] * (kUnits ? inv * vref : inv));
-            *reinterpret_cast<T4*>(to + 32 * db + 8 * q4) = x;
-          }
-      } else {
-        const int r = 32 * wave + lq;
-        float* to = part_rows(w, wg, slot, BM, D) + r * D + 4 * hi;
+          for (int r = 0; r < 4; ++r) x[r] = from_f32<T>(sum == 0.f ? 0.f : o[db][4 * q4 + r] * factor);
+          *reinterpret_cast<T4*>(own + lq * RB + (((4 * db + q4) ^ lq % CR) * 16) + 8 * hi) = x;
+        }
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
+      for (int i = 0; i < 32 * CR / kWave; ++i) {
+        const int r = (i * kWave + lane) / CR, ch = (i * kWave + lane) % CR;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(own + r * RB + ((ch ^ r % CR) * 16));
+        const int64_t at = (int64_t)(unsigned)__shfl((int)offset, r) | (int64_t)__shfl((int)(offset >> 32), r) << 32;
+        if (at >= 0) *reinterpret_cast<u32x4*>(static_cast<T*>(a.o) + at + 8 * ch) = x;
+      }
+    } else {
+      const uint64_t rows_here = __builtin_amdgcn_ballot_w64(mine);
+      float* const to = part_rows(w, wg, slot, BM, D) + 32 * wave * D;
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            f32x4 x;
+      for (int p = 0; p < PASSES; ++p) {
+        if (lq / 16 == p)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = kUnits ? o[db][4 * q4 + e] * vref : o[db][4 * q4 + e];
-            *reinterpret_cast<f32x4*>(to + 32 * db + 8 * q4) = x;
-          }
-        if (hi == 0) {
-          float* st = part_stats(w, (int)gridDim.x, wg, slot, BM, D);
-          st[r] = m_run == -INFINITY && sum != 0.f ? 0.f : m_run, st[BM + r] = sum;
+          for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              f32x4 x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = o[db][4 * q4 + e] * factor;
+              *reinterpret_cast<f32x4*>(own + lq % 16 * (2 * RB) + (((8 * db + 2 * q4 + hi) ^ lq % 16) * 16)) = x;
+            }
+#pragma unroll
+        for (int i = 0; i < 16 * 2 * CR / kWave; ++i) {
+          const int r = (i * kWave + lane) / (2 * CR), ch = (i * kWave + lane) % (2 * CR);
+          const f32x4 x = *reinterpret_cast<const f32x4*>(own + r * (2 * RB) + ((ch ^ r) * 16));
+          if (rows_here >> (16 * p + r) & 1) *reinterpret_cast<f32x4*>(to + (16 * p + r) * D + 4 * ch) = x;
         }
       }
+      if (mine && hi == 0) {
+        const int r = 32 * wave + lq;
+        float* st = part_stats(w, (int)gridDim.x, wg, slot, BM, D);
+        st[r] = m_run == -INFINITY && sum != 0.f ? 0.f : m_run, st[BM + r] = sum;
+      }
+    }
     }
     __syncthreads();   // the next segment's loads replace the stages
   }
