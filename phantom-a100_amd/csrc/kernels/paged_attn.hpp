@@ -565,6 +565,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   constexpr int RAW = k8 && !WIDE ? BN * CB : 16, SLOTS = k8 ? 4 : 1;
   __shared__ __attribute__((aligned(1024))) unsigned char k_raw0[RAW], k_raw1[RAW], v_raw0[RAW], v_raw1[RAW];
   __shared__ __attribute__((aligned(256))) float ks_lds[SLOTS][BN], vs_lds[SLOTS][BN];
+  __shared__ int odd_lds[2][BM / 32];   // of V(t), at t % 2: whether a wave's share has a value that is not finite
   __shared__ int64_t walk_lds[10];
   const std::integral_constant<int, 0> even{};
   const std::integral_constant<int, 1> odd{};
@@ -588,47 +589,61 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   const bool active = start_walk<THREADS>(c, w, true, walk_lds, wg, walk);
   Segment sg;
   const InTile in_row = in_tile(w.tiles, 32 * wave + lq);
-  while (active && uniform((int)walk.next([&](int s) { return uniform(load_seq(c, s)); }, sg)) != 0) {
+  constexpr int AHEAD = k8 ? 3 : 2;
+  int kv_head, key_begin, key_end, wave_all, wave_any;
+  int pages[AHEAD + 1], page;
+  V8 qf[QK_STEPS];
+  // The lane's row. Found again for each use, not held over the loops.
+  int token, hq, seen;
+  bool mine;
+  auto find_mine = [&]() {
+    InTile r = in_row;
+    asm volatile("" : "+v"(r.token), "+v"(r.head));
+    mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, r, token, hq);
+    seen = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
+  };
+  auto load_page = [&](int t) {
+    const int pos = min(key_begin + t * BN + lane, c.capacity - 1);
+    return c.table[sg.seq * c.table_stride + page_of((uint32_t)pos, c.div)];
+  };
+  // The next segment: its queries and first page table entries on their way. (Called before the stores of the one
+  // before it, which they need not wait for.)
+  auto begin_segment = [&]() __attribute__((always_inline)) {
+    if (uniform((int)walk.next([&](int s) { return uniform(load_seq(c, s)); }, sg)) == 0) return false;
     sg = {uniform(sg.rows), uniform(sg.seq), uniform(sg.head), uniform(sg.tile), uniform(sg.from), uniform(sg.to), uniform(sg.steps)};
-    int kv_head, head_part;
+    int head_part;
     split_head(w.tiles, sg.head, kv_head, head_part);
-    // The lane's row. Found again for each use, not held over the loops.
-    int token, hq, seen;
-    bool mine;
-    auto find_mine = [&]() {
-      InTile r = in_row;
-      asm volatile("" : "+v"(r.token), "+v"(r.head));
-      mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, r, token, hq);
-      seen = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
-    };
-    find_mine();
-    V8 qf[QK_STEPS];
-    {
-      const T* qp = static_cast<const T*>(a.q) + (mine ? (int64_t)(sg.rows.first + token) * a.q_token + hq * a.q_head : 0) + 8 * hi;
+    // Keys of the segment's tile: up to the last row's.
+    const int last_token = min((sg.tile + 1) * w.tiles.tokens, sg.rows.count) - 1;
+    key_begin = sg.from * kStep;
+    key_end = min(sg.to * kStep, keys_seen(sg.rows, last_token, c.capacity, w.causal));
 #pragma unroll
-      for (int kk = 0; kk < QK_STEPS; ++kk) {
-        const u32x4 x = mine ? *reinterpret_cast<const u32x4*>(qp + 16 * kk) : u32x4{0, 0, 0, 0};
-        qf[kk] = __builtin_bit_cast(V8, x);
-      }
+    for (int j = 0; j <= AHEAD; ++j) pages[j] = load_page(j);
+    page = load_page(AHEAD + 1);
+    find_mine();
+    const T* qp = static_cast<const T*>(a.q) + (mine ? (int64_t)(sg.rows.first + token) * a.q_token + hq * a.q_head : 0) + 8 * hi;
+#pragma unroll
+    for (int kk = 0; kk < QK_STEPS; ++kk) {
+      const u32x4 x = mine ? *reinterpret_cast<const u32x4*>(qp + 16 * kk) : u32x4{0, 0, 0, 0};
+      qf[kk] = __builtin_bit_cast(V8, x);
     }
     // Keys that all of the wave's rows see, and that some row does (none: the wave has no rows).
     int lo = mine ? seen : INT32_MAX, up = seen;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) lo = min(lo, __shfl_xor(lo, d)), up = max(up, __shfl_xor(up, d));
-    const int wave_all = uniform(lo), wave_any = uniform(up);
-    // Keys of the segment's tile: up to the last row's.
-    const int last_token = min((sg.tile + 1) * w.tiles.tokens, sg.rows.count) - 1;
-    const int key_begin = sg.from * kStep;
-    const int key_end = min(sg.to * kStep, keys_seen(sg.rows, last_token, c.capacity, w.causal));
+    wave_all = uniform(lo), wave_any = uniform(up);
+    return true;
+  };
+  bool more = active && begin_segment();
+  while (more) {
     const int nt = max(1, (key_end - key_begin + BN - 1) / BN);
 
     // ---- tiles of keys: lane l looks up key l; each thread's chunk rows come from there by lane
-    const int* table = c.table + sg.seq * c.table_stride;
-    auto load_page = [&](int t) { return table[page_of((uint32_t)min(key_begin + t * BN + lane, c.capacity - 1), c.div)]; };
     auto find_row = [&](int t, int page) {
       const int key = key_begin + t * BN + lane;
       const uint32_t at = ((uint32_t)page * c.heads + kv_head) * c.page_size + (key - page_of((uint32_t)key, c.div) * c.page_size);
-      return (key < key_end) & ((unsigned)page < (unsigned)c.pages) ? (int)at : -1;
+      const bool there = (key < key_end) & ((unsigned)page < (unsigned)c.pages);
+      return there ? (int)at : -1;
     };
     // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row (loads
     // are 32 rows apart, so the swizzle is the same).
@@ -659,15 +674,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     };
     auto from_raw = [&](const unsigned char* raw, u32x4 (&x)[CPT]) { x[0] = *reinterpret_cast<const u32x4*>(raw + tid * 16); };
     auto widen = [&](const u32x4 (&x)[CPT], unsigned char* stage, bool is_v) {
-      if constexpr (k8)
-#pragma unroll
-      for (int i = 0; i < CPT; ++i) {
-        const int r = (i * THREADS + tid) / LPR, ch = (i * THREADS + tid) % LPR * 2;
-        const int sw = is_v ? v_swz<CR>(r) : k_swz<CR>(r);
+      if constexpr (k8) {
+        int at = tid;
+        asm("" : "+v"(at));   // (addresses made each time, not held)
+        const int r = at / LPR, ch = (at % LPR * 2) ^ (is_v ? v_swz<CR>(r) : k_swz<CR>(r));
         u32x4 lo16, hi16;
-        widen16<C, T>(x[i], lo16, hi16);
-        *reinterpret_cast<u32x4*>(stage + r * RB + ((ch ^ sw) * 16)) = lo16;
-        *reinterpret_cast<u32x4*>(stage + r * RB + (((ch + 1) ^ sw) * 16)) = hi16;
+        widen16<C, T>(x[0], lo16, hi16);
+        *reinterpret_cast<u32x4*>(stage + r * RB + ch * 16) = lo16;
+        *reinterpret_cast<u32x4*>(stage + r * RB + (ch ^ 1) * 16) = hi16;
       }
     };
     auto present_of = [&](int row) -> uint64_t { return __builtin_amdgcn_ballot_w64(row >= 0); };
@@ -778,7 +792,9 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     };
     // 8 bits: l takes P, the product P times the values' scales (in fp16 in units of vref, the largest scale so
     // far, in which O is held: P times a scale must stay in the type's range).
-    auto exponentiate8 = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t, auto masked, const Bits& v) __attribute__((always_inline)) {
+    // (The product with a scale takes 0 for a P of 0 whatever the scale: of a key that the row does not see, it may
+    // not be finite.)
+    auto exponentiate8 = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t) __attribute__((always_inline)) {
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
       const float unit = kUnits ? 1.f / vref : 1.f;
 #pragma unroll
@@ -788,11 +804,9 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           const f32x4 x = *reinterpret_cast<const f32x4*>(&vs_lds[t % SLOTS][32 * b + 8 * q4 + 4 * hi]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float p = exp2_fast(fmaf(s[b][4 * q4 + r], w.scale_log2, neg_m));
+            const float p = exp2_fast(fmaf(s[b][4 * q4 + r], w.scale_log2, neg_m));
             l += p;
-            p *= kUnits ? x[r] * unit : x[r];
-            if constexpr (decltype(masked)::value) p = v.b[b] & 1u << (8 * q4 + r) ? p : 0.f;   // (0 x a scale that is not finite)
-            pf[b * 2 + q4 / 2][(q4 % 2) * 4 + r] = from_f32<T>(p);
+            pf[b * 2 + q4 / 2][(q4 % 2) * 4 + r] = from_f32<T>(p == 0.f ? 0.f : p * (kUnits ? x[r] * unit : x[r]));
           }
         }
     };
@@ -829,20 +843,21 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) l = add_pair(__builtin_bit_cast(u32x4, pf[i])[j], l, static_cast<T*>(nullptr));
     };
-    // Whether the tile's values in LDS are all finite.
-    auto values_finite = [&](const unsigned char* vs) {
+    // A wave's share of V(t) in LDS: whether all of it is finite, for all waves after the next barrier.
+    auto check_values = [&](int t, const unsigned char* vs) {
       u16x2 top = {0, 0};
-#pragma unroll 4
-      for (int i = 0; i < TILE_BYTES / 16 / kWave; ++i) top = max_bits(top, *reinterpret_cast<const u32x4*>(vs + (i * kWave + lane) * 16));
-      return __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= kInfBits<T>) == 0;
+#pragma unroll
+      for (int i = 0; i < TILE_BYTES / 16 / THREADS; ++i) top = max_bits(top, *reinterpret_cast<const u32x4*>(vs + (i * THREADS + tid) * 16));
+      const bool odd_values = __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= kInfBits<T>) != 0;
+      if (lane == 0) odd_lds[t & 1][wave] = odd_values;
     };
+    auto values_finite = [&](int t) { return __builtin_amdgcn_ballot_w64(odd_lds[t & 1][lane % (BM / 32)] != 0) == 0; };
     const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
     auto is_clean = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= wave_all; };
 
     // ---- the first tiles: K(0), V(0), K(1). At a tile t: rows[j] and row[j] are tile t + 1 + j's, present[j] tile
     // t + j's; page holds tile t + 1 + AHEAD's entries.
-    constexpr int AHEAD = k8 ? 3 : 2;
-    int page, row[AHEAD], rows[AHEAD][CPT];
+    int row[AHEAD], rows[AHEAD][CPT];
     uint64_t present[AHEAD + 1];
     const int tile_all = keys_seen(sg.rows, sg.tile * w.tiles.tokens, c.capacity, w.causal);   // the first row's keys
     auto whole_tile = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= tile_all; };
@@ -860,10 +875,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     };
     bool pipelined;
     {
-      int pages[AHEAD + 1], row0, rows0[CPT];
-#pragma unroll
-      for (int j = 0; j <= AHEAD; ++j) pages[j] = load_page(j);
-      page = load_page(AHEAD + 1);
+      int row0, rows0[CPT];
       row0 = find_row(0, pages[0]);
       present[0] = present_of(row0);
       chunk_rows(row0, present[0], rows0);
@@ -1053,6 +1065,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         }
       }
     }
+    check_values(t0, t0 & 1 ? v_lds1 : v_lds0);
+    __syncthreads();
 
     find_mine();
     // ---- the other tiles, one by one (the other waves' MFMAs beside this one's VALU), the masked ones above all.
@@ -1094,13 +1108,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         if (!clean) mask(s, t, pres);
         raise(row_max(s));
         raise_units(t);
-        if constexpr (k8) {
-          if (clean) exponentiate8(s, pf, t, std::false_type{}, Bits{});
-          else exponentiate8(s, pf, t, std::true_type{}, visible(t, pres));
-        } else {
-          exponentiate(s, pf);
-        }
-        if (!clean && skip_from == INT32_MAX && !values_finite(v_cur)) skip_from = t;
+        if constexpr (k8) exponentiate8(s, pf, t); else exponentiate(s, pf);
+        if (!clean && skip_from == INT32_MAX && !values_finite(t)) skip_from = t;
         if (clean || skip_from == INT32_MAX) pv(pf, v_cur);
         if constexpr (!k8) row_sum(pf);
       }
@@ -1110,9 +1119,11 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           widen(vx, v_nxt, true);
           store_scale(t + 1, scale);
         }
+        __syncthreads();
       } else {
         __builtin_amdgcn_s_waitcnt(0);
       }
+      if (fetch) check_values(t + 1, v_nxt);
       __syncthreads();
     }
 
@@ -1154,6 +1165,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 
     find_mine();
     // ---- the wave's 32 rows: done, or a part for the join. (The stages are free: every wave passed the last barrier.)
+    const int64_t offset = mine ? (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head : -1;
+    const bool was_mine = mine;
     const bool done = sg.from == 0 && sg.to == sg.steps;
     const int slot = sg.from == 0 ? 1 : 0;
     if (!done) {
@@ -1161,6 +1174,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       else rec.flags |= kPartContinues | (sg.to == sg.steps ? kPartEnds : 0);
     }
     {
+    more = begin_segment();
     // Each wave turns its rows round in LDS of its own (a quarter or an eighth of the stages, chunks swizzled by
     // row), so that whole rows are stored, 16 bytes a lane; a lane's pieces stored as they are cost ~4 us a tile.
     int ln = (int)threadIdx.x % kWave;   // (offsets made from it are not to be hoisted out of the segments' loop)
@@ -1171,7 +1185,6 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     constexpr int PASSES = 2;   // fp32 rows: half of the wave's rows at a time
     unsigned char* const own = (wave % 4 == 0 ? k_lds0 : wave % 4 == 1 ? v_lds0 : wave % 4 == 2 ? k_lds1 : v_lds1) + wave / 4 * (32 * RB);
     if (done) {
-      const int64_t offset = mine ? (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head : -1;
       typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -1190,7 +1203,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         if (at >= 0) *reinterpret_cast<u32x4*>(static_cast<T*>(a.o) + at + 8 * ch) = x;
       }
     } else {
-      const uint64_t rows_here = __builtin_amdgcn_ballot_w64(mine);
+      const uint64_t rows_here = __builtin_amdgcn_ballot_w64(was_mine);
       float* const to = part_rows(w, wg, slot, BM, D) + 32 * wave * D;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
@@ -1211,7 +1224,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           if (rows_here >> (16 * p + r) & 1) *reinterpret_cast<f32x4*>(to + (16 * p + r) * D + 4 * ch) = x;
         }
       }
-      if (mine && hi == 0) {
+      if (was_mine && hi == 0) {
         const int r = 32 * wave + lq;
         float* st = part_stats(w, (int)gridDim.x, wg, slot, BM, D);
         st[r] = m_run == -INFINITY && sum != 0.f ? 0.f : m_run, st[BM + r] = sum;
