@@ -565,6 +565,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   constexpr int RAW = k8 && !WIDE ? BN * CB : 16, SLOTS = k8 ? 4 : 1;
   __shared__ __attribute__((aligned(1024))) unsigned char k_raw0[RAW], k_raw1[RAW], v_raw0[RAW], v_raw1[RAW];
   __shared__ __attribute__((aligned(256))) float ks_lds[SLOTS][BN], vs_lds[SLOTS][BN];
+  __shared__ float ones_lds[k8 ? BN : 1];
   __shared__ int odd_lds[2][BM / 32];   // of V(t), at t % 2: whether a wave's share has a value that is not finite
   __shared__ int64_t walk_lds[10];
   const std::integral_constant<int, 0> even{};
@@ -583,6 +584,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   const uint32_t scale_bytes = k8 ? (uint32_t)min((uint64_t)c.pages * c.heads * c.page_size * 4, (uint64_t)kPastBuffer) : 0;
   const rsrc_t ks_rs = make_rsrc(k8 ? c.k_scale : nullptr, scale_bytes), vs_rs = make_rsrc(k8 ? c.v_scale : nullptr, scale_bytes);
 
+  if (k8 && tid < BN) ones_lds[tid] = 1.f;   // (before the barriers of start_walk)
   PartRecord rec = {0, 0, 0, 0};
   WorkWalk walk;
   int wg;
@@ -843,13 +845,20 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) l = add_pair(__builtin_bit_cast(u32x4, pf[i])[j], l, static_cast<T*>(nullptr));
     };
-    // A wave's share of V(t) in LDS: whether all of it is finite, for all waves after the next barrier.
+    // The wave's own share of V(t) in LDS, and its scales: whether all of it is finite, for all waves after the next
+    // barrier.
     auto check_values = [&](int t, const unsigned char* vs) {
+      constexpr int N = TILE_BYTES / 16 / THREADS;
       u16x2 top = {0, 0};
 #pragma unroll
-      for (int i = 0; i < TILE_BYTES / 16 / THREADS; ++i) top = max_bits(top, *reinterpret_cast<const u32x4*>(vs + (i * THREADS + tid) * 16));
-      const bool odd_values = __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= kInfBits<T>) != 0;
-      if (lane == 0) odd_lds[t & 1][wave] = odd_values;
+      for (int i = 0; i < N; ++i) {
+        const int at = k8 ? (wave * N + i) * kWave + lane : i * THREADS + tid;
+        top = max_bits(top, *reinterpret_cast<const u32x4*>(vs + at * 16));
+      }
+      bool odd_here = max(top[0], top[1]) >= kInfBits<T>;
+      if constexpr (k8) odd_here = odd_here || !(fabsf(vs_lds[t % SLOTS][lane]) < INFINITY);
+      const bool any = __builtin_amdgcn_ballot_w64(odd_here) != 0;
+      if (lane == 0) odd_lds[t & 1][wave] = any;
     };
     auto values_finite = [&](int t) { return __builtin_amdgcn_ballot_w64(odd_lds[t & 1][lane % (BM / 32)] != 0) == 0; };
     const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
@@ -885,20 +894,18 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         present[j + 1] = present_of(row[j]);
         chunk_rows(row[j], present[j + 1], rows[j]);
       }
-      pipelined = !(k8 && WIDE) && whole_tile(0, present[0]) && whole_tile(1, present[1]);
+      pipelined = !(k8 && WIDE);
       if constexpr (k8) {
         u32x4 kx[CPT], vx[CPT], k1[CPT];
         to_regs(c.k, k_rs, rows0, kx);
         to_regs(c.v, v_rs, rows0, vx);
         const float scale = load_scale(row0);
         if constexpr (!WIDE) {
-          if (pipelined) {   // K(1), K(2) and V(1) too
-            to_regs(c.k, k_rs, rows[0], k1);
-            scales_to_lds(1, row[0]);
-            to_raw(k_rs, rows[1], k_raw0);
-            to_raw(v_rs, rows[0], v_raw1);
-            widen(k1, k_stage(odd), false);
-          }
+          to_regs(c.k, k_rs, rows[0], k1);   // K(1), K(2) and V(1) too
+          scales_to_lds(1, row[0]);
+          to_raw(k_rs, rows[1], k_raw0);
+          to_raw(v_rs, rows[0], v_raw1);
+          widen(k1, k_stage(odd), false);
         }
         store_scale(0, scale);
         widen(kx, k_stage(even), false);
@@ -910,9 +917,15 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       }
     }
     __builtin_amdgcn_s_waitcnt(0);
+    if (!whole_tile(0, present[0])) {
+      if (k8) __syncthreads();   // (the scales are waves 0 and 1's)
+      check_values(0, v_lds0);
+    }
     __syncthreads();
+    // The pipeline takes a tile that every row sees whole, or that has finite values.
+    auto fits = [&](int t, uint64_t pres) { return t < nt && (whole_tile(t, pres) || values_finite(t)); };
 
-    // ---- the leading tiles that every row sees whole, in the two-stage pipeline
+    // ---- the tiles in the two-stage pipeline
     int t0 = 0;   // tiles done
     if constexpr (!(k8 && WIDE)) {
       constexpr int HALF = PV_STEPS / 2;
@@ -940,9 +953,10 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       };
       f32x16 sa[NKB], sb[NKB];
       V8 pa[PV_STEPS], pb[PV_STEPS];
-      if (pipelined) {
+      if (pipelined && fits(0, present[0])) {
         qk(sa, k_stage(even));
         scale_scores(sa, 0);
+        if (!is_clean(0, present[0])) mask(sa, 0, present[0]);
         raise(row_max(sa));
         raise_units(0);
         exp_first(sa, pa, 0);
@@ -997,7 +1011,16 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
               __builtin_amdgcn_sched_barrier(0);
             }
           }
+#pragma unroll
+          for (int i = 0; i < PV_STEPS; ++i) asm volatile("" : "+v"(pf[i]));   // (not to be moved past the branch below)
           __builtin_amdgcn_s_setprio(0);
+          // (present[0] is tile t + 1's by now. 8 bits: masked after the scales, of which phase B then takes ones.)
+          const float* ks_next = ks_lds[(t + 1) % SLOTS];
+          if (!is_clean(t + 1, present[0])) {
+            scale_scores(sn, t + 1);
+            mask(sn, t + 1, present[0]);
+            ks_next = ones_lds;
+          }
           // Phase B: O += V(t) P(t) with the row sums of P(t), the row maxima of S(t+1) and the first half of P(t+1)
           // against the reference as it is; where that is raised after all, the half is taken again.
           float mx = -INFINITY;
@@ -1025,7 +1048,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
               for (int k = 16 * NKB / N * i; k < 16 * NKB / N * (i + 1); k += 2) {
                 if constexpr (k8) {   // (four scores at a time)
                   if (k % 4 == 0) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(&ks_lds[(t + 1) % SLOTS][k / 16 * 32 + k % 16 * 2 + 4 * hi]);
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(ks_next + k / 16 * 32 + k % 16 * 2 + 4 * hi);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) sn[k / 16][k % 16 + r] *= x[r];
                   }
@@ -1052,25 +1075,21 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           const bool again = raise(mx), units = raise_units(t + 1);
           if (again || units) exp_first(sn, pn, t + 1);
           __builtin_amdgcn_s_waitcnt(0);
+          if (t + 1 < nt && !whole_tile(t + 1, present[0])) check_values(t + 1, v_stage(nxt));
           __syncthreads();
         };
-        // (present[0] and present[1]: tiles t0 and t0 + 1)
         while (true) {
           iteration(even, t0, sa, sb, pa, pb);
-          ++t0;
-          if (!whole_tile(t0 + 1, present[1])) break;
+          if (!fits(++t0, present[0])) break;
           iteration(odd, t0, sb, sa, pb, pa);
-          ++t0;
-          if (!whole_tile(t0 + 1, present[1])) break;
+          if (!fits(++t0, present[0])) break;
         }
       }
     }
-    check_values(t0, t0 & 1 ? v_lds1 : v_lds0);
-    __syncthreads();
 
     find_mine();
-    // ---- the other tiles, one by one (the other waves' MFMAs beside this one's VALU), the masked ones above all.
-    // K(t+1) and V(t+1) arrive meanwhile, 8-bit rows through registers.
+    // ---- tiles with a value that is not finite and that a row does not see, and those after them: one by one. K(t+1)
+    // and V(t+1) arrive meanwhile, 8-bit rows through registers. (And 8-bit caches of 4 GiB.)
 #pragma unroll 1
     for (int t = t0; t < nt; ++t) {
       const int P = t & 1;
