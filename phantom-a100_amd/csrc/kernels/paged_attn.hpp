@@ -210,11 +210,19 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
   constexpr int WAVE_BYTES = kStep * RB;
   static_assert(WAVE_BYTES >= D * 16 * 4, "a wave's V rows make room for 16 rows of its O");
   __shared__ __attribute__((aligned(1024))) unsigned char v_lds[WAVES][WAVE_BYTES];
+  // Two blocks of 128 dims in 16 bits have their queries in LDS, in the order of the products: in registers they are
+  // the 32 too many, beside O (64) and the rows on their way (64). (Four
+  // blocks have twice the registers, with one workgroup on a CU.)
+  constexpr bool q_in_lds = NB == 2 && D == 128 && !k8;
+  __shared__ u32x4 q_lds[q_in_lds ? NB * KK : 1][kWave];
   __shared__ float stat_lds[WAVES][2][16];
   __shared__ float scale_lds[WAVES][2][kStep];
   __shared__ int64_t walk_lds[10];
-  const int tid = (int)threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int g = lane / 16, lq = lane % 16;
+  int tid = (int)threadIdx.x, lane = tid % kWave, g = lane / 16, lq = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  // What follows from the lane (addresses, indexes of lanes, comparisons) is computed where it is used, in a few
+  // instructions: hoisted out of the loops it costs 30 to 60 registers, which then go to memory.
+  auto here = [&] { asm volatile("" : "+v"(tid), "+v"(lane), "+v"(g), "+v"(lq)); };
 
   PartRecord rec = {0, 0, 0, 0};
   WorkWalk walk;
@@ -228,9 +236,8 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
     return row * RB + ((chunk ^ (CR == 16 ? 2 * (row & 7) : 2 * ((row >> 1) & 3))) * 16);
   };
 
-  // Its reads and writes by lane: one base each, the rest by constants (a hoisted address for every one costs
-  // 30 registers). A write of load i is i RPL rows below the lane's first, whose swizzle differs where loads
-  // alternate between the halves of 8 rows.
+  // Its reads and writes by lane: one base each, the rest by constants. A write of load i is i RPL rows below the
+  // lane's first, whose swizzle differs where loads alternate between the halves of 8 rows.
   const int w_row = lane / LPR, w_chunk = lane % LPR * (k8 ? 2 : 1);
   int w_base = v_at(w_row, w_chunk), r_base = v_at(4 * g + lq / 4, lq % 4 / 2) + 8 * (lq % 2);
   auto v_write = [&](int i) { return i * RPL * RB + (w_base ^ (RPL == 4 && CR == 16 && i % 2 ? 128 : 0)); };
@@ -242,6 +249,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
     sg = {uniform(sg.rows), uniform(sg.seq), uniform(sg.head), uniform(sg.tile), uniform(sg.from), uniform(sg.to), uniform(sg.steps)};
     int kv_head, head_part;
     split_head(w.tiles, sg.head, kv_head, head_part);
+    here();
     // ---- the tile's queries
     u32x4 qf[NB][KK];
     int seen[NB];
@@ -254,8 +262,15 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         const int dim = k8 ? 64 * (kk / 2) + 16 * g + 8 * (kk % 2) : 32 * kk + 8 * g;
-        qf[b][kk] = mine ? *reinterpret_cast<const u32x4*>(qp + dim) : u32x4{0, 0, 0, 0};
+        if (!q_in_lds || (b * KK + kk) % WAVES == wave)
+          qf[b][kk] = mine ? *reinterpret_cast<const u32x4*>(qp + dim) : u32x4{0, 0, 0, 0};
       }
+    }
+    if constexpr (q_in_lds) {
+#pragma unroll
+      for (int i = 0; i < NB * KK; ++i)
+        if (i % WAVES == wave) q_lds[i][lane] = qf[i / KK][i % KK];
+      __syncthreads();
     }
     int all_seen = seen[0], any_seen = seen[0];   // keys that every row, and that some row, sees
     {
@@ -321,10 +336,17 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       const bool clean = present == 0xffffffffu && key0 + kStep <= all_seen;
       // ---- V to LDS, S^T
       u16x2 top = {0, 0};
+      here();
+      if constexpr (k8) {   // (widened here, not before, where it would take twice the registers)
+#pragma unroll
+        for (int i = 0; i < VL; ++i) asm volatile("" : "+v"(vr[i]));
+#pragma unroll
+        for (int i = 0; i < KL; ++i) asm volatile("" : "+v"(kr[0][i]), "+v"(kr[1][i]));
+      }
       asm volatile("" : "+v"(w_base), "+v"(r_base));
 #pragma unroll
       for (int i = 0; i < VL; ++i) {
-        const int r = i * RPL + w_row;
+        const int r = i * RPL + lane / LPR;
         if (present != 0xffffffffu && !(present >> r & 1)) vr[i] = u32x4{0, 0, 0, 0};
         if constexpr (k8) {
           u32x4 x, y;
@@ -354,7 +376,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
           }
 #pragma unroll
           for (int b = 0; b < NB; ++b)
-            s[b][h] = mfma16x16x32(__builtin_bit_cast(V8, x), __builtin_bit_cast(V8, qf[b][kk]), s[b][h]);
+            s[b][h] = mfma16x16x32(__builtin_bit_cast(V8, x), __builtin_bit_cast(V8, q_in_lds ? q_lds[b * KK + kk][lane] : qf[b][kk]), s[b][h]);
         }
       f32x4 ksc[2], vsc[2];
       if constexpr (k8) {
@@ -445,6 +467,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       } else {
 #pragma unroll 1
         for (int k = 0; k < kStep; ++k) {
+          here();
           const int from = (k % 16) / 4 * 16 + lq, j = k / 16 * 4 + k % 4;
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
@@ -475,6 +498,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      here();
       const float ls = groups_sum(l[b]);
       const float unit = k8 && std::is_same<T, f16>::value ? vref : 1.f;
 #pragma unroll
@@ -539,13 +563,13 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 // some row sees and another does not, leaves a tile with such a value out of P . V, and adds it at the end in
 // fp32 over the visible pairs.
 constexpr int chunk_rows_of(int d) { return d == 128 ? 256 : 128; }
-constexpr int chunk_wgs(int d) { return d == 128 ? 1 : 2; }   // workgroups on a CU
+constexpr int chunk_wgs(int d, bool k8) { return d == 128 ? 1 : k8 ? 2 : 3; }   // workgroups on a CU
 
 // WIDE: caches of 4 GiB and more. A load to LDS from a 64-bit address is an instruction of the flat kind, after
 // which the compiler waits for all LDS reads instead of the oldest; from a buffer, whose offsets have 32 bits, it is not.
 constexpr uint32_t kPastBuffer = 0xffffe000u;
 template <typename T, typename C, int D, int BM, bool WIDE>
-__global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chunk_wgs(D, cache_type<C>::k8bit) * BM / 128)))
 paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;

@@ -88,7 +88,7 @@ struct AttnPlan {
 // A cache of at most so many positions a sequence is read in a few steps: its tiles are not cut over workgroups,
 // which saves the second launch that joins them.
 constexpr int kWholeCapacity = 256;
-AttnPlan attn_plan(const pa::PagedCache& c, int64_t d, int64_t heads_q, int64_t max_new) {
+AttnPlan attn_plan(const pa::PagedCache& c, int64_t d, bool k8, int64_t heads_q, int64_t max_new) {
   const int64_t group = heads_q / c.heads;
   const int64_t new_tokens = !c.cu ? c.per_seq : max_new > 0 ? std::min<int64_t>(max_new, c.tokens) : c.tokens;
   const int64_t most = new_tokens * group;   // rows of a sequence and key/value head
@@ -97,7 +97,7 @@ AttnPlan attn_plan(const pa::PagedCache& c, int64_t d, int64_t heads_q, int64_t 
   const pa::TileShape t = pa::make_tiles((int)group, rows);
   const double tiles = (double)c.tokens / t.tokens + c.seqs;
   const double units = tiles * c.heads * t.splits * ((double)pa::kTileCost + c.capacity);
-  const int resident = kCUs * (rows > 64 ? pa::chunk_wgs((int)d) : pa::few_waves(rows / 16));
+  const int resident = kCUs * (rows > 64 ? pa::chunk_wgs((int)d, k8) : pa::few_waves(rows / 16));
   const int wgs = (int)std::max(1.0, std::min<double>(resident, units / pa::kMinUnits + 1));
   return {rows, wgs, c.capacity <= kWholeCapacity};
 }
@@ -181,7 +181,7 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
   if (!apart(o_token_stride, tokens, o_head_stride, heads_q) && !apart(o_head_stride, heads_q, o_token_stride, tokens))
     return fail(PA_ERR_INVALID, "%s: out's rows must not overlap", name);
   if (max_new < 0) return fail(PA_ERR_INVALID, "%s: max_new must not be negative", name);
-  const AttnPlan plan = attn_plan(c, cache->d, heads_q, max_new);
+  const AttnPlan plan = attn_plan(c, cache->d, is_8bit(cache->dtype), heads_q, max_new);
   if (workspace_bytes < pa::attn_workspace(plan.wgs, plan.rows, (int)cache->d) || !workspace || !aligned16(workspace))
     return fail(PA_ERR_INVALID, "%s: the workspace is too small, null or not 16-byte aligned", name);
   const pa::RowsQ a{q, o, q_token_stride, q_head_stride, o_token_stride, o_head_stride, (int)(heads_q / cache->heads),
@@ -214,7 +214,7 @@ int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t 
   if (int rc = check_tokens(name, tokens, cu_seqlens, &c)) return rc;
   if (heads_q <= 0 || heads_q > (1 << 16) || heads_q % cache->heads != 0 || max_new < 0)
     return fail(PA_ERR_INVALID, "%s: the query heads must be a multiple of the cache's heads, max_new not negative", name);
-  const AttnPlan plan = attn_plan(c, cache->d, heads_q, max_new);
+  const AttnPlan plan = attn_plan(c, cache->d, is_8bit(cache->dtype), heads_q, max_new);
   return pa::attn_workspace(plan.wgs, plan.rows, (int)cache->d);
 }
 

@@ -57,7 +57,10 @@ __host__ __device__ __forceinline__ int keys_seen(const SeqRows& s, int i, int c
 // workgroup whatever the lengths are, cut at steps of kStep keys. What a cut leaves of a tile are partial
 // results, joined afterwards.
 constexpr int kStep = 32;       // keys of a step
-constexpr int kTileCost = 64;   // units a tile costs beside its keys
+// Units a tile costs beside its keys: its queries, its first keys on their way, its result, in the time of keys.
+// Counted as 64, 256 and 512 keys: 24 x 700 tokens over 4096 keys, D = 128, e4m3 595, 530 and 537 us; 64 x 8 over
+// 8192, bf16 580, 536 and (at 512) no less; one over 28672 does not see it.
+constexpr int kTileCost = 256;
 constexpr int kMinUnits = 128;  // least units of a workgroup: a step for each of four waves
 
 struct TileShape {
