@@ -194,9 +194,12 @@ __device__ __forceinline__ float groups_sum(float x) { x += partner16(x); return
 // its P before the one rounding of P to the type.
 // A value that is not finite must reach the rows that see it and no others, and 0 x infinity would be a NaN:
 // a step that has one takes its P.V product in fp32 over the visible pairs instead.
-constexpr int few_waves(int nb) { return nb == 4 ? 1 : 2; }   // workgroups on a CU
+// Workgroups on a CU: two, but for two blocks of 128 dims in 16 bits, whose queries (32 registers), O (64) and rows
+// on their way (64) leave too few of half the registers (64 x 8 tokens over 8192 keys: 226 us, with two 260). One
+// block with one, 16 bits, 256 x 1 over 700: 109 for 95; in 8 bits, 64 x 1 over 8192 and 64 dims, 108 for 81.
+constexpr int few_wgs(int d, bool k8, int nb) { return d == 128 && !k8 && nb == 2 ? 1 : 2; }
 template <typename T, typename C, int D, int NB>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(NB))))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_wgs(D, cache_type<C>::k8bit, NB))))
 paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;
@@ -210,11 +213,6 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
   constexpr int WAVE_BYTES = kStep * RB;
   static_assert(WAVE_BYTES >= D * 16 * 4, "a wave's V rows make room for 16 rows of its O");
   __shared__ __attribute__((aligned(1024))) unsigned char v_lds[WAVES][WAVE_BYTES];
-  // Two blocks of 128 dims in 16 bits have their queries in LDS, in the order of the products: in registers they are
-  // the 32 too many, beside O (64) and the rows on their way (64). (Four
-  // blocks have twice the registers, with one workgroup on a CU.)
-  constexpr bool q_in_lds = NB == 2 && D == 128 && !k8;
-  __shared__ u32x4 q_lds[q_in_lds ? NB * KK : 1][kWave];
   __shared__ float stat_lds[WAVES][2][16];
   __shared__ float scale_lds[WAVES][2][kStep];
   __shared__ int64_t walk_lds[10];
@@ -262,15 +260,8 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         const int dim = k8 ? 64 * (kk / 2) + 16 * g + 8 * (kk % 2) : 32 * kk + 8 * g;
-        if (!q_in_lds || (b * KK + kk) % WAVES == wave)
-          qf[b][kk] = mine ? *reinterpret_cast<const u32x4*>(qp + dim) : u32x4{0, 0, 0, 0};
+        qf[b][kk] = mine ? *reinterpret_cast<const u32x4*>(qp + dim) : u32x4{0, 0, 0, 0};
       }
-    }
-    if constexpr (q_in_lds) {
-#pragma unroll
-      for (int i = 0; i < NB * KK; ++i)
-        if (i % WAVES == wave) q_lds[i][lane] = qf[i / KK][i % KK];
-      __syncthreads();
     }
     int all_seen = seen[0], any_seen = seen[0];   // keys that every row, and that some row, sees
     {
@@ -376,7 +367,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
           }
 #pragma unroll
           for (int b = 0; b < NB; ++b)
-            s[b][h] = mfma16x16x32(__builtin_bit_cast(V8, x), __builtin_bit_cast(V8, q_in_lds ? q_lds[b * KK + kk][lane] : qf[b][kk]), s[b][h]);
+            s[b][h] = mfma16x16x32(__builtin_bit_cast(V8, x), __builtin_bit_cast(V8, qf[b][kk]), s[b][h]);
         }
       f32x4 ksc[2], vsc[2];
       if constexpr (k8) {

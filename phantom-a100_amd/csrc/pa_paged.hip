@@ -92,12 +92,16 @@ AttnPlan attn_plan(const pa::PagedCache& c, int64_t d, bool k8, int64_t heads_q,
   const int64_t group = heads_q / c.heads;
   const int64_t new_tokens = !c.cu ? c.per_seq : max_new > 0 ? std::min<int64_t>(max_new, c.tokens) : c.tokens;
   const int64_t most = new_tokens * group;   // rows of a sequence and key/value head
-  const int rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : pa::chunk_rows_of((int)d);
+  // Few rows in tiles of 16 or 32, up to two of them over the same keys, more in chunks. 64 x 16 tokens of 4 heads
+  // over 8192 keys as two tiles of 32 and as a chunk: 16 bits 325 and 322 us, 8 bits 228 and 378 (64 dims, 16 bits:
+  // 156 and 137); 128 x 16 of 64 dims over 1000 in 8 bits 46 and 55. 17 to 32 rows as two
+  // tiles of 16: 272 for 226. Tiles of 64 were between the two (315, 314), and slower at 128 rows than chunks (434, 308).
+  const int rows = most <= 16 ? 16 : most <= 64 ? 32 : pa::chunk_rows_of((int)d);
   // As many workgroups as are resident at once, or fewer where the work's bound is below their least share.
   const pa::TileShape t = pa::make_tiles((int)group, rows);
   const double tiles = (double)c.tokens / t.tokens + c.seqs;
   const double units = tiles * c.heads * t.splits * ((double)pa::kTileCost + c.capacity);
-  const int resident = kCUs * (rows > 64 ? pa::chunk_wgs((int)d, k8) : pa::few_waves(rows / 16));
+  const int resident = kCUs * (rows > 64 ? pa::chunk_wgs((int)d, k8) : pa::few_wgs((int)d, k8, rows / 16));
   const int wgs = (int)std::max(1.0, std::min<double>(resident, units / pa::kMinUnits + 1));
   return {rows, wgs, c.capacity <= kWholeCapacity};
 }
@@ -195,7 +199,6 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
     switch (plan.rows) {
       case 16: return launch_attn<T, D, 16>(pa::paged_attn_few<T, C, D, 1>, 256, c, a, plan, causal, workspace, st);
       case 32: return launch_attn<T, D, 32>(pa::paged_attn_few<T, C, D, 2>, 256, c, a, plan, causal, workspace, st);
-      case 64: return launch_attn<T, D, 64>(pa::paged_attn_few<T, C, D, 4>, 256, c, a, plan, causal, workspace, st);
       default: break;
     }
     const uint64_t cache_rows = (uint64_t)c.pages * c.heads * c.page_size;
