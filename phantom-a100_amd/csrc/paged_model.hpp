@@ -58,10 +58,12 @@ __host__ __device__ __forceinline__ int keys_seen(const SeqRows& s, int i, int c
 // results, joined afterwards.
 constexpr int kStep = 32;       // keys of a step
 // Units a tile costs beside its keys: its queries, its first keys on their way, its result, in the time of keys.
-// Counted as 64, 256 and 512 keys: 24 x 700 tokens over 4096 keys, D = 128, e4m3 595, 530 and 537 us; 64 x 8 over
-// 8192, bf16 580, 536 and (at 512) no less; one over 28672 does not see it.
+// Counted as 64, 256 and 512 keys: 24 x 700 tokens over 4096 keys, D = 128, e4m3 595, 520 and 531 us; 16 x 16 over
+// 4096, D = 64, int8 37, 34 and 32; 256 x 1 over 1000 144, 126 and 130; one over 1031 does not see it.
 constexpr int kTileCost = 256;
-constexpr int kMinUnits = 128;  // least units of a workgroup: a step for each of four waves
+// Least units of a workgroup: a step for each of four waves. With 64 and 256, 2 x 5 tokens over 4096 take 27 and 22
+// us, 2 x 100 over 900 take 32 and 31 (128: 22 and 27), one over 1031 the same.
+constexpr int kMinUnits = 128;
 
 struct TileShape {
   int group, heads, tokens, splits;   // query heads per key/value head; of a tile; tokens of a tile; tiles that cover the group

@@ -172,6 +172,7 @@ def attn(p: Problem, causal: bool = True):
     inputs' type, A = sum_j p_j |v_j| / l:
       * p rounded once to the type: u A; below fp16's normal range an absolute 2^-25 of each p (and, for 8-bit
         caches, of p times the value's scale over the largest scale): 2^-25 sum_j max|v| / l
+        (max over the finite values: an output that is a number sums no others)
       * the output rounded: u |o|, or half a subnormal fp16 step
       * scores in fp32: d products summed, |ds| <= (d + 8) 2^-24 sum |q k| / sqrt(d); and 2^-20 for the
         exponentials and the sums; twice, for the numerator and the sum l.
@@ -181,6 +182,7 @@ def attn(p: Problem, causal: bool = True):
     out = torch.zeros(p.q.shape, dtype=torch.float64)
     bound = torch.zeros(p.q.shape, dtype=torch.float64)
     claims = torch.zeros(tokens, dtype=torch.long)
+    finite = lambda x: torch.where(torch.isfinite(x), x, torch.zeros((), dtype=x.dtype))  # noqa: E731
     u = HALF_STEP[p.q.dtype]
     for s, (first, count, length) in enumerate(layout(p, tokens)):
         if count == 0:
@@ -209,6 +211,6 @@ def attn(p: Problem, causal: bool = True):
                     a = (w[i, use] @ vh[use].abs()) / l[i]
                     size = (q[i].abs() @ kh[use].abs().t()).max() / math.sqrt(d)
                     es = 2 * ((d + 8) * 2.0 ** -24 * size + 2.0 ** -20)
-                    low = 2.0 ** -25 * use.sum() * vh[use].abs().max() / l[i] if p.q.dtype == torch.float16 else 0.0
+                    low = 2.0 ** -25 * use.sum() * finite(vh[use]).abs().max() / l[i] if p.q.dtype == torch.float16 else 0.0
                     bound[first + i, h] = (2 * u + es) * a + low + u * out[first + i, h].abs() + 2.0 ** -25
     return out, bound, claims == 1

@@ -333,3 +333,133 @@ def test_offsets_past_32_bits():
     assert bool(((got - ref).abs() <= bound).all())
     k, _ = cuda_attn.cache_read(kc, vc, table.cuda(), lengths, max_len=300)
     assert torch.equal(k.double().cpu(), po.read(small, 300)[0])
+
+
+@pytest.mark.parametrize("dtype,cache", [(F16, E4M3), (BF16, I8)], ids=IDS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_8bit_offsets_past_32_bits(dtype, cache, d):
+    """8-bit caches of a little over 4 GiB (chunks of them are read from 64-bit addresses), pages in use at both ends."""
+    page, hkv = 128, 1
+    pages = 2 ** 32 // (page * hkv * d) + 64
+    kc = torch.zeros((pages, hkv, page, d), dtype=torch.int8, device="cuda")
+    vc = torch.zeros_like(kc)
+    scales = {n: torch.zeros((pages, hkv, page), device="cuda") for n in ("k_scale", "v_scale")}
+    p = po.make([(100, 300), (3, 200), (1, 90)], d=d, hq=2, hkv=hkv, page=page, dtype=dtype, cache=cache, stale=0.0)
+    where = torch.tensor([pages - 1, 1, pages - 2, pages // 2, 0, pages - 3, pages - 4, 2], device="cuda")[:p.k_cache.shape[0]]
+    kc[where], vc[where] = p.k_cache.view(torch.int8).cuda(), p.v_cache.view(torch.int8).cuda()
+    kc, vc = kc.view(cache), vc.view(cache)
+    for n in scales:
+        scales[n][where] = p.scales[n].cuda()
+    table = torch.where(p.table >= 0, where.cpu()[p.table.clamp(min=0).long()].to(torch.int32), p.table)
+    cuda_attn.cache_write(p.k.cuda(), p.v.cuda(), kc, vc, table.cuda(), p.lengths.cuda(), p.cu.cuda(), **scales)
+    p.k_cache, p.v_cache, p.scales = po.written(p)
+    assert same(kc.view(torch.int8)[where].view(cache), p.k_cache) and same(scales["v_scale"][where], p.scales["v_scale"])
+    for bad in (False, True):
+        if bad:   # a value that the first of the chunk's rows do not see
+            pg, rw = po.slot(p, 0, 250)
+            p.scales["v_scale"][pg, :, rw] = math.inf
+            scales["v_scale"][where[pg], :, rw] = math.inf
+        ref, bound, mine = po.attn(p)
+        got = cuda_attn.paged_attn(p.q.cuda(), kc, vc, table.cuda(), p.lengths.cuda(), p.cu.cuda(), **scales).double().cpu()
+        sees = torch.zeros(p.q.shape[0], dtype=torch.bool)
+        sees[50:100] = bad
+        assert bool(((got - ref).abs() <= bound)[~sees].all())
+        assert not torch.isfinite(got[sees]).any()
+        many = cuda_attn.paged_attn(p.q[:100].cuda(), kc, vc, table[:1].cuda(), p.lengths[:1].cuda(), causal=False, **scales)
+        assert bool(torch.isfinite(many).all()) != bad
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, I8)], ids=IDS)
+@pytest.mark.parametrize("seqs", [257, 700])
+def test_many_sequences(dtype, cache, seqs):
+    """More sequences than a workgroup has threads, some without new tokens; single tokens and chunks among them."""
+    g = torch.Generator().manual_seed(seqs)
+    r = lambda n: int(torch.randint(n, (1,), generator=g))  # noqa: E731
+    sizes = [(0, r(50)) if i % 7 == 3 else (1, 1 + r(300)) if i % 50 else (40 + r(60), 100 + r(400)) for i in range(seqs)]
+    p = po.make(sizes, d=64, hq=2, hkv=1, dtype=dtype, cache=cache)
+    check_attn(p)
+    check_attn(po.make([(1, 1 + r(90)) for _ in range(seqs)], d=128, hq=2, hkv=1, dtype=dtype, cache=cache, uniform=True))
+
+
+@pytest.mark.parametrize("dtype,cache,what", [(*t, w) for t in TYPES for w in ("inf", "nan")]
+                         + [(F16, E4M3, "code"), (BF16, E4M3, "code")], ids=IDS)
+def test_values_that_are_not_finite_in_chunks(dtype, cache, what):
+    """D = 128, tiles of 256 rows: a value (or its scale, or an e4m3 NaN code) that some rows of a tile see."""
+    seqs = [(150, 400), (90, 513)]
+    p = po.make(seqs, d=128, hq=4, hkv=2, dtype=dtype, cache=cache)
+    seen_from = {0: 330, 1: 460}   # in the middle of a tile of keys, with tiles before and after it
+    for s, pos in seen_from.items():
+        pg, rw = po.slot(p, s, pos)
+        if what == "code":
+            p.v_cache.view(torch.int8)[pg, :, rw, 77] = 0x7f
+        elif p.scales:
+            p.scales["v_scale"][pg, :, rw] = math.inf if what == "inf" else math.nan
+        else:
+            p.v_cache[pg, :, rw, 77] = math.inf if what == "inf" else math.nan
+    ref, bound, _ = po.attn(p)
+    g = p.to("cuda")
+    got = cuda_attn.paged_attn(g.q, *g.cache(), g.cu, **g.scales).double().cpu()
+    sees = torch.cat([torch.arange(n - c, n) >= seen_from[s] for s, (c, n) in enumerate(seqs)])
+    assert bool(((got - ref).abs() <= bound)[~sees].all())
+    if p.scales and what != "code":
+        assert not torch.isfinite(got[sees]).any()
+    else:   # one dim of the rows that see it, as the formula has it
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref))
+        fine = torch.isfinite(ref)
+        assert bool(((got - ref).abs() <= bound)[fine].all())
+
+
+@pytest.mark.parametrize("new", [1, 6, 90])
+def test_shared_pages_and_a_table_with_strides(new):
+    """Two sequences that share a prefix's pages, one that has a page twice; the table is a slice of a wider one."""
+    p = po.make([(new, 200), (new, 230), (new, 190)], d=64, page=16, dtype=BF16)
+    p.table[1, :6] = p.table[0, :6]
+    p.table[2, 3] = p.table[2, 5]
+    check_attn(p)
+    g = p.to("cuda")
+    wide = torch.full((4, 2 * p.table.shape[1] + 3), 2 ** 31 - 1, dtype=torch.int32, device="cuda")
+    wide[:3, 2:2 + p.table.shape[1]] = g.table
+    view = wide[:3, 2:2 + p.table.shape[1]]
+    want = cuda_attn.paged_attn(g.q, *g.cache(), g.cu)
+    assert torch.equal(cuda_attn.paged_attn(g.q, g.k_cache, g.v_cache, view, g.lengths, g.cu), want)
+    for a, b in zip(cuda_attn.cache_read(g.k_cache, g.v_cache, view, g.lengths), cuda_attn.cache_read(*g.cache())):
+        assert torch.equal(a, b)
+    one = g.table[:1].expand(3, -1)   # every sequence the same pages
+    p.table = p.table[:1].expand(3, -1).contiguous()
+    p.lengths[:] = 190
+    ref, bound, _ = po.attn(p)
+    got = cuda_attn.paged_attn(g.q, g.k_cache, g.v_cache, one, p.lengths.cuda(), g.cu).double().cpu()
+    assert bool(((got - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("hq,new", [(300, 1), (300, 2), (520, 3)])
+def test_groups_of_more_heads_than_a_tile_has_rows(hq, new):
+    check_attn(po.make([(new, 70), (new, 130)], d=128, hq=hq, hkv=1, dtype=BF16, cache=E4M3))
+    check_attn(po.make([(new, 70), (new, 330)], d=64, hq=hq, hkv=1, dtype=F16))
+
+
+def test_many_lengths_out_of_range():
+    """Lengths of the largest int for many sequences count as the table's capacity, in the work's division too."""
+    p = po.make([(2, 90)] * 300 + [(40, 60)], d=64, page=16, dtype=F16)
+    p.lengths[:] = 2 ** 31 - 1
+    check_attn(p)
+    check_attn(p, causal=False, max_new=2)
+
+
+@pytest.mark.parametrize("new", [1, 90])
+def test_two_calls_at_once(new):
+    """Calls that overlap on two streams, over one cache: each has a workspace of its own."""
+    p = po.make([(new, 2000), (new, 1500)], d=128, hq=8, hkv=2, dtype=BF16)
+    g = p.to("cuda")
+    other = torch.randn_like(g.q.float()).to(BF16)
+    want = [cuda_attn.paged_attn(q, *g.cache(), g.cu, max_new=new) for q in (g.q, other)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, q in enumerate((g.q, other)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(cuda_attn.paged_attn(q, *g.cache(), g.cu, max_new=new))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])

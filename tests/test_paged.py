@@ -180,6 +180,17 @@ def test_c_entries_refuse_arguments():
     assert lib.pa_cache_read(c, p, p, f16, 2 ** 31, None) == -2
 
 
+def test_c_entries_refuse_more_work_than_they_can_count():
+    """Offsets out of order could give every sequence all tokens: the worst case must fit the kernels' numbers."""
+    lib, p, f16 = _native.lib(), ctypes.c_void_p(256), _native.DTYPE_F16
+    c = native_cache(seqs=2 ** 24, heads=1, pages=1, table_cols=2 ** 25)
+    for got in (lambda: lib.pa_paged_attn_workspace(c, f16, 2 ** 30, 1, p, 0),
+                lambda: lib.pa_paged_attn_fwd(c, p, p, f16, 2 ** 30, 1, 64, 64, 64, 64, p, 0, 1, p, 2 ** 60, None)):
+        assert got() == -2 and "2^62" in _native.last_error()
+    c = native_cache(seqs=4096, heads=8, pages=2 ** 20, table_cols=2 ** 13)   # a large call
+    assert lib.pa_paged_attn_workspace(c, f16, 2 ** 20, 64, p, 0) > 0
+
+
 def test_index_arithmetic(tmp_path):
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not os.path.exists(hipcc):
