@@ -128,7 +128,9 @@ struct RowsIn {
 };
 
 // One row (a new token's key or value of one head) per LPR lanes, 16 bytes a lane. Rows of a wave run over
-// (token, K or V, head): a token's heads are near each other in the inputs.
+// (token, K or V, head): a token's heads are near each other in the inputs. A row's largest magnitude is a maximum
+// over its lanes, without LDS. Small calls are bound by the chain offsets, lengths, page table, store (32 single
+// tokens: WRITE_SMALL), large ones by bytes: 8 x up to 2048 tokens, 16 heads, D = 64, f16 (WRITE_BYTES).
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(256) cache_write_rows(PagedCache c, RowsIn kin, RowsIn vin) {
   constexpr int LPR = D / 8, RPW = kWave / LPR;
@@ -137,6 +139,8 @@ __global__ void __launch_bounds__(256) cache_write_rows(PagedCache c, RowsIn kin
   const int64_t row0 = wave * RPW, rows = (int64_t)c.tokens * 2 * c.heads;
   int seq = 0, tok = 0, h = 0;
   bool is_v = false, mine = false;
+  typedef typename vec8<T>::type V8;
+  V8 x;
   // The rows of a wave lie in a few tokens: find each token's sequence with the whole wave.
   {
     const int64_t row = min(row0 + lane / LPR, rows - 1);
@@ -145,6 +149,9 @@ __global__ void __launch_bounds__(256) cache_write_rows(PagedCache c, RowsIn kin
     is_v = rest >= c.heads;
     h = is_v ? rest - c.heads : rest;
     mine = row0 + lane / LPR < rows;
+    // (Every row may be read, also one that no sequence has: on its way before its place is known.)
+    const RowsIn& in = is_v ? vin : kin;
+    x = *reinterpret_cast<const V8*>(static_cast<const T*>(in.p) + tok * in.token + h * in.head + 8 * sub);
     int last = -1;
 #pragma unroll
     for (int r = 0; r < RPW; ++r) {
@@ -160,9 +167,6 @@ __global__ void __launch_bounds__(256) cache_write_rows(PagedCache c, RowsIn kin
   if (i < 0 || i >= s.count) return;
   const int pos = new_token_pos(s, i);
   if (pos < 0 || pos >= c.capacity) return;
-  const RowsIn& in = is_v ? vin : kin;
-  typedef typename vec8<T>::type V8;
-  const V8 x = *reinterpret_cast<const V8*>(static_cast<const T*>(in.p) + tok * in.token + h * in.head + 8 * sub);
   const int at = cache_row(c, seq, h, pos);
   if (at < 0) return;
   C* out = static_cast<C*>(is_v ? c.v : c.k) + (int64_t)at * D + 8 * sub;
@@ -194,8 +198,12 @@ __global__ void __launch_bounds__(256) cache_write_rows(PagedCache c, RowsIn kin
 }
 
 // Rows read back as (seqs, heads, n, D), one row per LPR lanes; zeros from a sequence's length on and for
-// absent pages. Grid: x over (sequence, head), y over blocks of rows.
-template <typename T, typename C, int D>
+// absent pages. Grid: x over (sequence, head), y over blocks of rows. Bytes are all it does: 16 sequences of 1 to 8192
+// tokens, 8 heads, D = 128, e4m3 (537 MB of results): 102 us, 6.9 TB/s.
+// STREAM: results past kStreamBytes go by the caches, which could not hold them for a reader: that case took 164 us
+// through them, 32 full sequences 350 for 329. Fewer stay in: 67 MB and a sum over them 31 us, past the caches 33.
+constexpr int64_t kStreamBytes = 256ll << 20;   // the memory-side cache
+template <typename T, typename C, int D, bool STREAM>
 __global__ void __launch_bounds__(256) cache_read_rows(PagedCache c, T* k, T* v, int n) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;
   const int s = (int)blockIdx.x / c.heads, h = (int)blockIdx.x % c.heads;
@@ -215,7 +223,8 @@ __global__ void __launch_bounds__(256) cache_read_rows(PagedCache c, T* k, T* v,
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = from_f32<T>(x[j]);
       }
-      *reinterpret_cast<V8*>((m ? v : k) + to) = o;
+      V8* out = reinterpret_cast<V8*>((m ? v : k) + to);
+      if constexpr (STREAM) __builtin_nontemporal_store(o, out); else *out = o;
     }
   }
 }

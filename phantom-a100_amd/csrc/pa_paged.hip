@@ -168,8 +168,11 @@ int pa_cache_read(const pa_paged_cache* cache, void* k, void* v, int dtype, int6
   const int64_t y = std::min<int64_t>((n + rows_per_block - 1) / rows_per_block, 65535);
   const hipError_t e = with_types(dtype, cache->dtype, cache->d, [&](auto t, auto ct, auto dim) {
     typedef decltype(t) T;
-    hipLaunchKernelGGL((pa::cache_read_rows<T, decltype(ct), decltype(dim)::value>), dim3((unsigned)x, (unsigned)y),
-                       dim3(256), 0, static_cast<hipStream_t>(stream), c, static_cast<T*>(k), static_cast<T*>(v), (int)n);
+    const bool past_caches = x * n >= pa::kStreamBytes / (2 * cache->d * (int64_t)sizeof(T));
+    const auto kernel = past_caches ? pa::cache_read_rows<T, decltype(ct), decltype(dim)::value, true>
+                                  : pa::cache_read_rows<T, decltype(ct), decltype(dim)::value, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)y), dim3(256), 0, static_cast<hipStream_t>(stream), c,
+                       static_cast<T*>(k), static_cast<T*>(v), (int)n);
     return hipGetLastError();
   });
   return hip_status(e, name);
