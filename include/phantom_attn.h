@@ -195,7 +195,8 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
                       void* stream);
 
 /* Bytes of workspace that pa_paged_attn_fwd needs for a call with these arguments; a negative PA_ERR_* code if it
- * refuses them. It depends on sizes alone, not on what the tensors hold. No GPU needed. */
+ * refuses them (PA_ERR_UNSUPPORTED also where sequences, tokens and positions could make 2^62 steps of work). It
+ * depends on sizes alone, not on what the tensors hold. No GPU needed. */
 int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
                                 const int32_t* cu_seqlens, int64_t max_new);
 

@@ -569,7 +569,7 @@ constexpr int chunk_wgs(int d, bool k8) { return d == 128 ? 1 : k8 ? 2 : 3; }   
 
 // WIDE: caches (or their scales) past a buffer's 32-bit offsets. 16-bit rows then come from 64-bit addresses by
 // instructions of the flat kind, after which the compiler waits for all LDS reads instead of the oldest; 8-bit ones
-// are not pipelined at all.
+// are not pipelined at all. The case above takes 2108 us (in buffers 1976), in int8 3129 (2312), with D = 64 2659 (1756).
 constexpr uint32_t kPastBuffer = 0xffffe000u;
 template <typename T, typename C, int D, int BM, bool WIDE>
 __global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chunk_wgs(D, cache_type<C>::k8bit) * BM / 128)))

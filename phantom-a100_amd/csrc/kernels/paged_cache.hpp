@@ -201,9 +201,9 @@ __global__ void __launch_bounds__(256) cache_write_rows(PagedCache c, RowsIn kin
 
 // Rows read back as (seqs, heads, n, D), one row per LPR lanes; zeros from a sequence's length on and for
 // absent pages. Grid: x over (sequence, head), y over blocks of rows. Bytes are all it does: 16 sequences of 1 to 8192
-// tokens, 8 heads, D = 128, e4m3 (537 MB of results): 102 us, 6.9 TB/s.
+// tokens, 8 heads, D = 128, e4m3 (537 MB of results): 148 us, 4.75 TB/s; 102 where the codes are in the memory-side cache.
 // STREAM: results past kStreamBytes go by the caches, which could not hold them for a reader: that case took 164 us
-// through them, 32 full sequences 350 for 329. Fewer stay in: 67 MB and a sum over them 31 us, past the caches 33.
+// through them with the codes in there, 32 full sequences 350 for 329. Fewer stay in: 67 MB and a sum over them 31 us, past the caches 33.
 constexpr int64_t kStreamBytes = 256ll << 20;   // the memory-side cache
 template <typename T, typename C, int D, bool STREAM>
 __global__ void __launch_bounds__(256) cache_read_rows(PagedCache c, T* k, T* v, int n) {
