@@ -123,8 +123,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     if need < 0:
         _native.check(need, "paged_attn")
     workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    qs, os = q.stride(), out.stride()
+    qs, outs = q.stride(), out.stride()
     _call("pa_paged_attn_fwd", "paged_attn", q.device, cache, q.data_ptr(), out.data_ptr(), code, tokens, heads_q,
-          qs[0], qs[1], os[0], os[1], cu, bound, 1 if causal else 0, workspace.data_ptr(),
+          qs[0], qs[1], outs[0], outs[1], cu, bound, 1 if causal else 0, workspace.data_ptr(),
           need, _stream_ptr(q.device))
     return out

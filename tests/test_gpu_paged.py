@@ -409,6 +409,25 @@ def test_values_that_are_not_finite_in_chunks(dtype, cache, what):
         assert bool(((got - ref).abs() <= bound)[fine].all())
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("new,length", [(3, 90), (12, 700), (150, 700)])
+def test_queries_that_are_not_finite(dtype, cache, new, length):
+    """They change their own rows only; in rows that no sequence has they change nothing."""
+    p = po.make([(new, length), (2, 70)], d=128, hq=4, hkv=2, dtype=dtype, cache=cache)
+    p.q[1, 2, 5], p.q[2, 0, 7], p.q[new, 3, 1] = math.nan, math.inf, -math.inf
+    p.q = torch.cat([p.q, torch.full((5, 4, 128), math.nan, dtype=dtype)])
+    ref, bound, mine = po.attn(p)
+    g = p.to("cuda")
+    out = torch.full_like(g.q, 7.0)
+    cuda_attn.paged_attn(g.q, *g.cache(), g.cu, out=out, **g.scales)
+    got = out.double().cpu()
+    assert bool((got[new + 2:] == 7).all())
+    bad = torch.zeros(new + 2, 4, dtype=torch.bool)
+    bad[1, 2] = bad[2, 0] = bad[new, 3] = True
+    assert bool(torch.isnan(got[:new + 2][bad]).all())
+    assert bool(((got - ref).abs() <= bound)[:new + 2][~bad].all())
+
+
 @pytest.mark.parametrize("new", [1, 6, 90])
 def test_shared_pages_and_a_table_with_strides(new):
     """Two sequences that share a prefix's pages, one that has a page twice; the table is a slice of a wider one."""
