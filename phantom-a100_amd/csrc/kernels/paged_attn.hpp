@@ -295,10 +295,11 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
     u32x4 kr[2][KL], vr[VL];
     float ks = 0.f, vs = 0.f;
     const int* table = c.table + sg.seq * c.table_stride;
+    const uint32_t page_rows = c.heads * c.page_size;
     auto load_page = [&](int step) { return table[page_of((uint32_t)min(step * kStep + lane % 32, c.capacity - 1), c.div)]; };
     auto find_row = [&](int step, int page) {
       const int key = step * kStep + lane % 32;
-      const uint32_t at = ((uint32_t)page * c.heads + kv_head) * c.page_size + (key - page_of((uint32_t)key, c.div) * c.page_size);
+      const uint32_t at = (uint32_t)page * page_rows + kv_head * c.page_size + (key - page_of((uint32_t)key, c.div) * c.page_size);
       return key < any_seen && (unsigned)page < (unsigned)c.pages ? (int)at : -1;
     };
     auto load_step = [&](int row) {
@@ -620,7 +621,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   const InTile in_row = in_tile(w.tiles, 32 * wave + lq);
   constexpr int AHEAD = k8 ? 3 : 2;
   int kv_head, key_begin, key_end, wave_all, wave_any;
-  int pages[AHEAD + 1], page;
+  int pages[AHEAD + 1], page, in_page;   // in_page: the row in its page of the key whose entry `page` is
   V8 qf[QK_STEPS];
   // The lane's row. Found again for each use, not held over the loops.
   int token, hq, seen;
@@ -631,9 +632,15 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, r, token, hq);
     seen = mine ? keys_seen(sg.rows, token, c.capacity, w.causal) : 0;
   };
-  auto load_page = [&](int t) {
+  auto load_page = [&](int t, int& rest) {
     const int pos = min(key_begin + t * BN + lane, c.capacity - 1);
-    return c.table[sg.seq * c.table_stride + page_of((uint32_t)pos, c.div)];
+    const int col = (int)page_of((uint32_t)pos, c.div);
+    rest = pos - col * c.page_size;
+    return c.table[sg.seq * c.table_stride + col];
+  };
+  auto in_page_of = [&](int t) {
+    const int key = key_begin + t * BN + lane;
+    return key - (int)page_of((uint32_t)key, c.div) * c.page_size;
   };
   // The next segment: its queries and first page table entries on their way. (Called before the stores of the one
   // before it, which they need not wait for.)
@@ -647,8 +654,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     key_begin = sg.from * kStep;
     key_end = min(sg.to * kStep, keys_seen(sg.rows, last_token, c.capacity, w.causal));
 #pragma unroll
-    for (int j = 0; j <= AHEAD; ++j) pages[j] = load_page(j);
-    page = load_page(AHEAD + 1);
+    for (int j = 0; j <= AHEAD; ++j) pages[j] = load_page(j, in_page);
+    page = load_page(AHEAD + 1, in_page);
     find_mine();
     const T* qp = static_cast<const T*>(a.q) + (mine ? (int64_t)(sg.rows.first + token) * a.q_token + hq * a.q_head : 0) + 8 * hi;
 #pragma unroll
@@ -668,9 +675,10 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     const int nt = max(1, (key_end - key_begin + BN - 1) / BN);
 
     // ---- tiles of keys: lane l looks up key l; each thread's chunk rows come from there by lane
-    auto find_row = [&](int t, int page) {
+    const uint32_t page_rows = c.heads * c.page_size, head_rows = kv_head * c.page_size;
+    auto find_row = [&](int t, int page, int rest) {
       const int key = key_begin + t * BN + lane;
-      const uint32_t at = ((uint32_t)page * c.heads + kv_head) * c.page_size + (key - page_of((uint32_t)key, c.div) * c.page_size);
+      const uint32_t at = (uint32_t)page * page_rows + (head_rows + rest);
       const bool there = (key < key_end) & ((unsigned)page < (unsigned)c.pages);
       return there ? (int)at : -1;
     };
@@ -912,12 +920,12 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     bool pipelined;
     {
       int row0, rows0[CPT];
-      row0 = find_row(0, pages[0]);
+      row0 = find_row(0, pages[0], in_page_of(0));
       present[0] = present_of(row0);
       chunk_rows(row0, present[0], rows0);
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
-        row[j] = find_row(j + 1, pages[j + 1]);
+        row[j] = find_row(j + 1, pages[j + 1], in_page_of(j + 1));
         present[j + 1] = present_of(row[j]);
         chunk_rows(row[j], present[j + 1], rows[j]);
       }
@@ -1028,9 +1036,9 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
               sn[i % NKB] = mfma32x32x16(x, qf[i / NKB], i < NKB ? f32x16{} : sn[i % NKB]);
               if (i % EACH == EACH - 1) exp_quad(s, pf, HALF * 8 + i / EACH * 4, neg_m, t, unit, l);
               if (i == N / 4) {
-                row_new = find_row(t + 1 + AHEAD, page);
+                row_new = find_row(t + 1 + AHEAD, page, in_page);
                 present_new = present_of(row_new);
-                page = load_page(t + 2 + AHEAD);
+                page = load_page(t + 2 + AHEAD, in_page);
               }
               if (i == N / 2) {
                 advance(row_new, present_new);
@@ -1141,8 +1149,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       }
       const uint64_t pres = present[0];
       {
-        const int row_new = find_row(t + 1 + AHEAD, page);
-        page = load_page(t + 2 + AHEAD);
+        const int row_new = find_row(t + 1 + AHEAD, page, in_page);
+        page = load_page(t + 2 + AHEAD, in_page);
         const uint64_t present_new = present_of(row_new);
         advance(row_new, present_new);
         chunk_rows(row_new, present_new, rows[AHEAD - 1]);
@@ -1179,7 +1187,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     if (skip_from < wave_tiles) {
 #pragma unroll 1
       for (int t = skip_from; t < wave_tiles; ++t) {
-        const int row_t = find_row(t, load_page(t));
+        int rest;
+        const int page_t = load_page(t, rest), row_t = find_row(t, page_t, rest);
         const uint64_t present_t = __builtin_amdgcn_ballot_w64(row_t >= 0);
         if (is_clean(t, present_t)) continue;
 #pragma unroll 1
