@@ -558,8 +558,8 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 // does not see whole, each wave looks at its share of the values as they arrive; if one is not finite, the pipeline
 // ends there. The tiles from it on go one by one, those with such a value leave P . V out, and it is added at the
 // end in fp32 over the visible pairs.
-// 4096 tokens at the end of 32768 keys, 32 heads over 8, D = 128, causal: bf16 1.99 ms, 1030 TFLOP/s (the card's
-// large matrix products reach 1290); e4m3 2.26 ms; D = 64 1.30 ms.
+// 4096 tokens at the end of 32768 keys, 32 heads over 8, D = 128, causal: bf16 1.93 to 2.05 ms, 1000 to 1070
+// TFLOP/s (the card's large matrix products reach 1290); e4m3 2.20 ms; D = 64 1.23 ms.
 //
 // Rows of a tile, D = 128, 256 and 128 (one workgroup of 8 waves on a CU, two of 4): that case 2015 and 2183 us, 4 x
 // 2048 120 and 117, 24 x 700 over 4096 456 and 491, 256 x 64 over 640 73 and 85. D = 64 has 128, and as many
