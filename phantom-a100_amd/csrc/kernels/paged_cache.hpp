@@ -51,11 +51,7 @@ struct PagedCache {
 __device__ __forceinline__ SeqRows load_seq(const PagedCache& c, int s) {
   const int begin = c.cu ? c.cu[s] : s * c.per_seq;
   const int end = c.cu ? c.cu[s + 1] : begin + c.per_seq;
-  SeqRows r = seq_rows(begin, end, c.lengths[s], c.tokens);
-  // A longer one has its new tokens past the capacity too, and every key that it sees below it: the same rows and
-  // keys, but the work counted for it stays within what the launcher admits.
-  r.length = min(r.length, c.capacity + r.count);
-  return r;
+  return held_rows(seq_rows(begin, end, c.lengths[s], c.tokens), c.capacity);
 }
 // Cache row of position pos (0 <= pos < capacity) of sequence s for head h, -1 if its page is absent.
 __device__ __forceinline__ int cache_row(const PagedCache& c, int s, int h, int pos) {

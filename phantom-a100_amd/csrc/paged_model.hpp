@@ -8,8 +8,8 @@
 
 namespace pa {
 
-// Sizes the launchers admit: positions, rows of new tokens and page sizes stay below 2^30, so sums of two
-// fit 32 bits; the rows of a cache (pages x heads x page size) stay below 2^31.
+// Sizes the launchers admit: capacities, rows of new tokens and page sizes are at most 2^30, so that one of them and
+// a tile's more fits 31 bits (two of 2^30 do not); the rows of a cache (pages x heads x page size) stay below 2^31.
 constexpr int64_t kPagedMaxPos = 1ll << 30;
 
 // pos / page_size as a multiplication: with L = ceil(log2 d) and magic = floor(2^(31+L) / d) + 1,
@@ -39,6 +39,13 @@ struct SeqRows {
 __host__ __device__ __forceinline__ SeqRows seq_rows(int begin, int end, int length, int tokens) {
   const int b = clamp_int(begin, 0, tokens), e = clamp_int(end, b, tokens);
   return {b, e - b, clamp_int(length, 0, (int)kPagedMaxPos)};
+}
+// The rows as the work is counted and divided by: a longer sequence has its new tokens past the capacity too, and every
+// key that it sees below it, at the length capacity + count: the same rows and keys, but no more work than the launcher
+// admits. (Compared by the difference: both summands may be 2^30.)
+__host__ __device__ __forceinline__ SeqRows held_rows(SeqRows s, int capacity) {
+  if (s.length - s.count > capacity) s.length = capacity + s.count;
+  return s;
 }
 // Position in the cache of the sequence's new token i; below 0 or past the table's columns it has none.
 __host__ __device__ __forceinline__ int new_token_pos(const SeqRows& s, int i) { return s.length - s.count + i; }
