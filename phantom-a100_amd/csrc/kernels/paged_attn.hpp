@@ -180,6 +180,18 @@ __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_el
 __device__ __forceinline__ float groups_max(float x) { x = fmaxf(x, partner16(x)); return fmaxf(x, partner32(x)); }
 __device__ __forceinline__ float groups_sum(float x) { x += partner16(x); return x + partner32(x); }
 
+// fp16 over an 8-bit cache: P times a value's scale goes into a 16-bit product, whatever the scales are, so each row's O
+// is held in a unit of its own, and its P times scale is divided by that. The unit follows what the row itself gives
+// weight: it starts at kUnitLeast, becomes 2^-8 of the row's largest weight P |scale| when that outgrows it by 2^15 (an
+// fp16 reaches 65504), and falls with the row's other sums when its maximum rises. So it never exceeds 2^-8 of the
+// largest weight, what a key loses below fp16's normal range is at most 2^-33 of that, and neither a key that the row
+// does not see nor a large value that it gives no weight costs it bits.
+constexpr float kUnitLeast = 0x1p-100f, kUnitMost = 0x1p120f, kUnitRoom = 0x1p15f;
+// The unit of a row, `unit` so far, whose largest weight is `top`. (One that is not finite makes the row so in any unit.)
+__device__ __forceinline__ float unit_for(float unit, float top) {
+  return top > unit * kUnitRoom && top < INFINITY ? fminf(top * 0x1p-8f, kUnitMost) : fmaxf(unit, kUnitLeast);
+}
+
 // ---- Few rows a tile: single tokens, and the few tokens of one ----
 //
 // A tile has 16 NB rows; its keys go past once, and what bounds the kernel is reading them: 4 D bytes (2 D in 8
@@ -206,6 +218,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_wg
 paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;
+  constexpr bool kUnits = k8 && std::is_same<T, f16>::value;      // each row's O in a unit of its own
   constexpr int WAVES = 4, ROWS = 16 * NB, RB = D * 2;            // RB: bytes of a V row in LDS
   constexpr int CB = k8 ? D : 2 * D;                              // bytes of a cache row
   constexpr int LPR = CB / 16, RPL = kWave / LPR, VL = kStep / RPL;   // V loads: lanes per row, rows per load, loads
@@ -280,12 +293,13 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       all_seen = __builtin_amdgcn_readfirstlane(lo);
       any_seen = __builtin_amdgcn_readfirstlane(hi);
     }
-    float m[NB], l[NB], vref = 1e-30f;
+    float m[NB], l[NB], unit[NB];
     f32x4 o[NB][NDB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       m[b] = -INFINITY;
       l[b] = 0.f;
+      unit[b] = kUnits ? kUnitLeast : 1.f;
 #pragma unroll
       for (int db = 0; db < NDB; ++db) o[b][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -376,18 +390,6 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       f32x4 ksc[2], vsc[2];
       if constexpr (k8) {
         if (lane < 32) scale_lds[wave][0][lane] = ks, scale_lds[wave][1][lane] = vs;
-        if constexpr (std::is_same<T, f16>::value) {
-          // P times a value's scale must stay in fp16's range: O is held in units of vref, the largest scale so far.
-          const float big = wave_allreduce(row >= 0 && fabsf(vs) < INFINITY ? fabsf(vs) : 0.f, MaxOp{});
-          if (big > vref) {
-            const float f = vref / big;
-            vref = big;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int db = 0; db < NDB; ++db) o[b][db] *= f;
-          }
-        }
       }
       // ---- the next step's rows, into the registers that this one's have left
       __builtin_amdgcn_sched_barrier(0);
@@ -398,11 +400,10 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (k8) {
-        const float unit = std::is_same<T, f16>::value ? 1.f / vref : 1.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           ksc[h] = *reinterpret_cast<const f32x4*>(&scale_lds[wave][0][16 * h + 4 * g]) * w.scale_log2;
-          vsc[h] = *reinterpret_cast<const f32x4*>(&scale_lds[wave][1][16 * h + 4 * g]) * unit;
+          vsc[h] = *reinterpret_cast<const f32x4*>(&scale_lds[wave][1][16 * h + 4 * g]);
         }
       }
       // ---- softmax
@@ -432,10 +433,15 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
         if (__builtin_amdgcn_ballot_w64(m_new > m[b]) != 0) {
           const float f = m[b] == -INFINITY ? 0.f : exp2_fast(m[b] + neg_m);
           l[b] *= f;
+          if constexpr (kUnits) {
+            unit[b] *= f;
+          } else {
 #pragma unroll
-          for (int db = 0; db < NDB; ++db) o[b][db] *= f;
+            for (int db = 0; db < NDB; ++db) o[b][db] *= f;
+          }
           m[b] = m_new;
         }
+        float top = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float p = exp2_fast(t[j] + neg_m);
@@ -444,9 +450,23 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
             p *= vsc[j / 4][j % 4];
             if (!clean) p = sees >> j & 1 ? p : 0.f;   // (0 x a scale that is not finite)
           }
+          if constexpr (kUnits) top = fmaxf(top, fabsf(p));
           p32[b][j] = p;
-          pf[b][j] = from_f32<T>(p);
         }
+        if constexpr (kUnits) {
+          const float was = unit[b], now = unit_for(was, groups_max(top));
+          if (__builtin_amdgcn_ballot_w64(now != was) != 0) {
+            const float f = now == was ? 1.f : was / now;
+            unit[b] = now;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) o[b][db] *= f;
+          }
+          const float inv = __builtin_amdgcn_rcpf(now);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p32[b][j] *= inv;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[b][j] = from_f32<T>(p32[b][j]);
       }
       // ---- O^T += V^T . P^T
       if (!odd) {
@@ -495,10 +515,9 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
     for (int b = 0; b < NB; ++b) {
       here();
       const float ls = groups_sum(l[b]);
-      const float unit = k8 && std::is_same<T, f16>::value ? vref : 1.f;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
-        *reinterpret_cast<f32x4*>(vw + lq * (D * 4) + (((4 * db + g) ^ lq) * 16)) = o[b][db] * unit;
+        *reinterpret_cast<f32x4*>(vw + lq * (D * 4) + (((4 * db + g) ^ lq) * 16)) = o[b][db] * unit[b];
       // (Scores that are all NaN leave no maximum and a NaN sum, which must not count as a row that sees nothing.)
       if (lane < 16) stat_lds[wave][0][lane] = m[b] == -INFINITY && ls != 0.f ? 0.f : m[b], stat_lds[wave][1][lane] = ls;
       __syncthreads();
@@ -552,7 +571,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 // of those of P(t+1). K(t+2) and V(t+1) arrive meanwhile, a row per page lookup: 16-bit rows straight into LDS;
 // 8-bit rows into a raw buffer of LDS one tile earlier, each thread its own, and from there widened to 16 bits
 // (exact) once for all waves. A key's scale multiplies its scores, a value's scale its P before the one rounding of
-// P to the type; so fp16 holds O in units of the largest value scale so far, and P times a scale stays in its range.
+// P to the type (fp16: in the row's unit).
 // O and l are rescaled only when some row's maximum outgrew its reference by more than 2^8.
 // A value that is not finite must not reach rows that do not see it (0 x infinity is NaN): of a tile that some row
 // does not see whole, each wave looks at its share of the values as they arrive; if one is not finite, the pipeline
@@ -577,7 +596,7 @@ __global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chu
 paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;
-  constexpr bool kUnits = k8 && std::is_same<T, f16>::value;   // O in units of the largest value scale so far
+  constexpr bool kUnits = k8 && std::is_same<T, f16>::value;   // each row's O in a unit of its own
   constexpr int BN = 64, THREADS = BM * 2, RB = D * 2, CB = k8 ? D : 2 * D, CR = D / 8;
   constexpr int TILE_BYTES = BN * RB;
   constexpr int QK_STEPS = D / 16, NKB = BN / 32, NDB = D / 32, PV_STEPS = BN / 16;
@@ -751,7 +770,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     // The wave's first tile that is not clean and has a value that is not finite: from there on, tiles that are
     // not clean leave P . V out, and take_visible adds it at the end.
     int skip_from = INT32_MAX;
-    float m_run = -INFINITY, vref = 1e-30f, l = 0.f;
+    float m_run = -INFINITY, unit = kUnits ? kUnitLeast : 1.f, l = 0.f;
     f32x16 o[NDB];
 #pragma unroll
     for (int db = 0; db < NDB; ++db) o[db] = f32x16{};
@@ -815,8 +834,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         const float f = m_new > m_run ? exp2_fast(m_run - m_new) : 1.f;   // (m_run = -inf: 0)
         m_run = m_new;
         l *= f;
+        float g = f;
+        if constexpr (kUnits) {   // (the unit falls instead of O, down to its least)
+          const float to = fmaxf(unit * f, kUnitLeast);
+          g = unit * f == to ? 1.f : unit * f / to;
+          unit = to;
+        }
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) o[db] *= f;
+        for (int db = 0; db < NDB; ++db) o[db] *= g;
       }
       return up;
     };
@@ -827,13 +852,13 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) pf[b * 2 + r / 8][r % 8] = from_f32<T>(exp2_fast(fmaf(s[b][r], w.scale_log2, neg_m)));
     };
-    // 8 bits: l takes P, the product P times the values' scales (in fp16 in units of vref, the largest scale so
-    // far, in which O is held: P times a scale must stay in the type's range).
+    // 8 bits: the sum takes P, the product P times the values' scales (in fp16 in the row's unit; `top` takes the largest).
     // (The product with a scale takes 0 for a P of 0 whatever the scale: of a key that the row does not see, it may
     // not be finite.)
-    auto exponentiate8 = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t) __attribute__((always_inline)) {
+    auto exponentiate8 = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t, float& sum, float& top) __attribute__((always_inline)) {
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-      const float unit = kUnits ? 1.f / vref : 1.f;
+      const float inv = kUnits ? __builtin_amdgcn_rcpf(unit) : 1.f;
+      sum = top = 0.f;
 #pragma unroll
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
@@ -841,21 +866,23 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           const f32x4 x = *reinterpret_cast<const f32x4*>(&vs_lds[t % SLOTS][32 * b + 8 * q4 + 4 * hi]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = exp2_fast(fmaf(s[b][4 * q4 + r], w.scale_log2, neg_m));
-            l += p;
-            pf[b * 2 + q4 / 2][(q4 % 2) * 4 + r] = from_f32<T>(p == 0.f ? 0.f : p * (kUnits ? x[r] * unit : x[r]));
+            float p = exp2_fast(fmaf(s[b][4 * q4 + r], w.scale_log2, neg_m));
+            sum += p;
+            p = p == 0.f ? 0.f : p * x[r];
+            if constexpr (kUnits) top = fmaxf(top, fabsf(p)), p *= inv;
+            pf[b * 2 + q4 / 2][(q4 % 2) * 4 + r] = from_f32<T>(p);
           }
         }
     };
-    auto raise_units = [&](int t) {   // vref, where tile t has a larger scale: whether it did
+    // The rows' units, for weights of up to `top` in the lane: whether some changed. scaled: what O was multiplied by.
+    auto raise_units = [&](float top, float& scaled) {
       if constexpr (!kUnits) return false;
-      const float x = fabsf(vs_lds[t % SLOTS][lane]);
-      const float top = uniform_f(wave_allreduce(x < INFINITY ? x : 0.f, MaxOp{}));
-      if (top <= vref) return false;
-      const float f = vref / top;
-      vref = top;
+      const float was = unit, now = unit_for(was, fmaxf(top, partner32(top)));
+      if (__builtin_amdgcn_ballot_w64(now != was) == 0) return false;
+      scaled = now == was ? 1.f : was / now;
+      unit = now;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) o[db] *= f;
+      for (int db = 0; db < NDB; ++db) o[db] *= scaled;
       return true;
     };
     auto pv = [&](const V8 (&pf)[PV_STEPS], const unsigned char* vs) {
@@ -965,9 +992,10 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     if constexpr (!(k8 && WIDE)) {
       constexpr int HALF = PV_STEPS / 2;
       auto neg_ref = [&]() { return m_run == -INFINITY ? 0.f : -m_run; };
-      // P of four scores, e to e + 3 (16-key step e / 8), of tile t; 8 bits: its sum to `sum`. (A masked score gives 0,
-      // and 0 times a scale is 0: a tile with a scale that is not finite and a masked key does not come here.)
-      auto exp_quad = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int e, float neg_m, int t, float unit, float& sum) __attribute__((always_inline)) {
+      // P of four scores, e to e + 3 (16-key step e / 8), of tile t; 8 bits: its sum to `sum`, in fp16 its largest weight
+      // to `top`. (A masked score gives 0, and 0 times a scale is 0: a tile with a scale that is not finite and a masked
+      // key does not come here.)
+      auto exp_quad = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int e, float neg_m, int t, float inv, float& sum, float& top) __attribute__((always_inline)) {
         f32x4 x = {1.f, 1.f, 1.f, 1.f};
         if constexpr (k8) x = *reinterpret_cast<const f32x4*>(&vs_lds[t % SLOTS][e / 16 * 32 + e % 16 * 2 + 4 * hi]);
 #pragma unroll
@@ -975,17 +1003,32 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           float p = exp2_fast(fmaf(s[e / 16][e % 16 + k], w.scale_log2, neg_m));
           if constexpr (k8) {
             sum += p;
-            p *= kUnits ? x[k] * unit : x[k];
+            p *= x[k];
+            if constexpr (kUnits) top = max_nan(top, fabsf(p)), p *= inv;
           }
           pf[e / 8][e % 8 + k] = from_f32<T>(p);
         }
       };
-      float l_next = 0.f;   // 8 bits: the sum of the first half of P(t + 1)
+      auto inverse_unit = [&]() { return kUnits ? __builtin_amdgcn_rcpf(unit) : 1.f; };
+      float l_next = 0.f, top = 0.f;   // 8 bits: the sum of the first half of P(t + 1); its largest weight so far
       auto exp_first = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t) __attribute__((always_inline)) {
-        const float neg_m = neg_ref(), unit = kUnits ? 1.f / vref : 1.f;
-        l_next = 0.f;
+        const float neg_m = neg_ref(), inv = inverse_unit();
+        l_next = top = 0.f;
 #pragma unroll
-        for (int e = 0; e < HALF * 8; e += 4) exp_quad(s, pf, e, neg_m, t, unit, l_next);
+        for (int e = 0; e < HALF * 8; e += 4) exp_quad(s, pf, e, neg_m, t, inv, l_next, top);
+      };
+      // The first half of P(t) after its reference was raised (again) or its unit. (A second time at most: the unit then
+      // has room for the same weights.)
+      auto settle_first = [&](const f32x16 (&s)[NKB], V8 (&pf)[PV_STEPS], int t, bool again) __attribute__((always_inline)) {
+        if constexpr (!kUnits) {
+          if (again) exp_first(s, pf, t);
+        } else {
+          float scaled;
+          do {
+            if (again) exp_first(s, pf, t);
+            again = raise_units(top, scaled);
+          } while (again);
+        }
       };
       f32x16 sa[NKB], sb[NKB];
       V8 pa[PV_STEPS], pb[PV_STEPS];
@@ -994,8 +1037,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         scale_scores(sa, 0);
         if (!is_clean(0, present[0])) mask(sa, 0, present[0]);
         raise(row_max(sa));
-        raise_units(0);
-        exp_first(sa, pa, 0);
+        settle_first(sa, pa, 0, true);
         __syncthreads();   // iteration 0 replaces K(0)
         auto iteration = [&](auto par, int t, f32x16 (&s)[NKB], f32x16 (&sn)[NKB], V8 (&pf)[PV_STEPS], V8 (&pn)[PV_STEPS]) __attribute__((always_inline)) {
           constexpr int P = decltype(par)::value;
@@ -1015,7 +1057,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           }
           uint64_t present_new = 0;
           int row_new = 0;
-          const float unit = kUnits ? 1.f / vref : 1.f;
+          const float inv = inverse_unit();
           // The phases are laid out by hand, one MFMA and its share of the VALU work after another (the compiler's
           // own order, and its scheduling groups, put the MFMAs first and the exponentials behind them).
           // Phase A: S(t+1) with the second half of P(t).
@@ -1034,7 +1076,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
               const V8 x = ahead[i % 2];
               if (i + 2 < N) ahead[i % 2] = operand(i + 2);
               sn[i % NKB] = mfma32x32x16(x, qf[i / NKB], i < NKB ? f32x16{} : sn[i % NKB]);
-              if (i % EACH == EACH - 1) exp_quad(s, pf, HALF * 8 + i / EACH * 4, neg_m, t, unit, l);
+              if (i % EACH == EACH - 1) exp_quad(s, pf, HALF * 8 + i / EACH * 4, neg_m, t, inv, l, top);
               if (i == N / 4) {
                 row_new = find_row(t + 1 + AHEAD, page, in_page);
                 present_new = present_of(row_new);
@@ -1050,6 +1092,19 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
           for (int i = 0; i < PV_STEPS; ++i) asm volatile("" : "+v"(pf[i]));   // (not to be moved past the branch below)
           __builtin_amdgcn_s_setprio(0);
+          if constexpr (kUnits) {
+            // The second half outgrew its row's unit: taken again in the new one, the first half is scaled to it.
+            float scaled;
+            if (raise_units(top, scaled)) {
+              const float neg_m = neg_ref(), inv = inverse_unit();
+              float none = 0.f;
+#pragma unroll
+              for (int e = 0; e < HALF * 8; ++e) pf[e / 8][e % 8] = from_f32<T>(to_f32(pf[e / 8][e % 8]) * scaled);
+#pragma unroll
+              for (int e = HALF * 8; e < 2 * HALF * 8; e += 4) exp_quad(s, pf, e, neg_m, t, inv, none, top);
+            }
+            top = 0.f;
+          }
           // (present[0] is tile t + 1's by now. 8 bits: masked after the scales, of which phase B then takes ones.)
           const float* ks_next = ks_lds[(t + 1) % SLOTS];
           if (!is_clean(t + 1, present[0])) {
@@ -1073,7 +1128,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
               const i16x8 x = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
               return __builtin_bit_cast(V8, x);
             };
-            const float neg_m = neg_ref();
+            const float neg_m = neg_ref(), inv = inverse_unit();
             V8 ahead[2] = {operand(0), operand(1)};
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -1091,7 +1146,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
                 }
                 mx = max_nan(mx, max_nan(sn[k / 16][k % 16], sn[k / 16][k % 16 + 1]));
               }
-              if (i % EACH == EACH - 1) exp_quad(sn, pn, i / EACH * 4, neg_m, t + 1, unit, l_next);
+              if (i % EACH == EACH - 1) exp_quad(sn, pn, i / EACH * 4, neg_m, t + 1, inv, l_next, top);
               if constexpr (k8) {
                 if (i == 0) from_raw(P ? k_raw1 : k_raw0, kx);
                 if (i == N / 4) widen(kx, k_stage(cur), false);
@@ -1108,8 +1163,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
             for (int i = 0; i < HALF; ++i) asm volatile("" : "+v"(pn[i]));   // (not to be moved into the branches below)
           }
-          const bool again = raise(mx), units = raise_units(t + 1);
-          if (again || units) exp_first(sn, pn, t + 1);
+          settle_first(sn, pn, t + 1, raise(mx));
           __builtin_amdgcn_s_waitcnt(0);
           if (t + 1 < nt && !whole_tile(t + 1, present[0])) check_values(t + 1, v_stage(nxt));
           __syncthreads();
@@ -1163,8 +1217,13 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         scale_scores(s, t);
         if (!clean) mask(s, t, pres);
         raise(row_max(s));
-        raise_units(t);
-        if constexpr (k8) exponentiate8(s, pf, t); else exponentiate(s, pf);
+        if constexpr (k8) {
+          float sum, top, scaled;
+          do exponentiate8(s, pf, t, sum, top); while (raise_units(top, scaled));
+          l += sum;
+        } else {
+          exponentiate(s, pf);
+        }
         if (!clean && skip_from == INT32_MAX && !values_finite(t)) skip_from = t;
         if (clean || skip_from == INT32_MAX) pv(pf, v_cur);
         if constexpr (!k8) row_sum(pf);
@@ -1206,7 +1265,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           }
           dot += partner32(dot);
           float p = exp2_fast(fmaf(dot, ks * w.scale_log2, m_run == -INFINITY ? 0.f : -m_run));
-          p = vis ? p * (kUnits ? vs / vref : vs) : 0.f;
+          p = vis ? p * vs : 0.f;
+          if constexpr (kUnits) p *= __builtin_amdgcn_rcpf(unit);
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) {
             cached8(static_cast<const C*>(c.v) + (int64_t)at * D, 8 * i, 1.f, x);
@@ -1238,7 +1298,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     asm volatile("" : "+v"(ln));
     const int lq = ln % 32, hi = ln / 32, lane = ln;
     const float sum = half_sum(l);
-    const float factor = done ? (sum == 0.f ? 0.f : (kUnits ? vref : 1.f) / sum) : kUnits ? vref : 1.f;
+    const float factor = done ? (sum == 0.f ? 0.f : unit / sum) : unit;
     constexpr int PASSES = 2;   // fp32 rows: half of the wave's rows at a time
     unsigned char* const own = (wave % 4 == 0 ? k_lds0 : wave % 4 == 1 ? v_lds0 : wave % 4 == 2 ? k_lds1 : v_lds1) + wave / 4 * (32 * RB);
     if (done) {
