@@ -2,7 +2,8 @@
 //
 // New token i of a sequence of `length` tokens, count of them new, sees the keys at positions up to
 // length - count + i (causal) or all of them: O = sum_j softmax_j(q . k_j / sqrt(D)) v_j. Query head h reads
-// key/value head h / group. A token that sees no key gets zeros.
+// key/value head h / group. A token that sees no key gets zeros; one whose visible scores are all -inf has a softmax of
+// NaN, as the formula has it.
 #pragma once
 
 #include "fa_mfma.hpp"
@@ -175,6 +176,14 @@ __device__ __forceinline__ float add_pair(unsigned x, float c, bf16*) {
 // Maxima that pass a NaN on: fmaxf first quiets each operand, an instruction apiece. (A row with a NaN score is NaN,
 // whatever its reference.)
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Least maximum of a row that sees a key: -inf is for rows that see none. (P is 0 at a score of -inf against it too, and
+// the largest finite score's is at least 1: a sum of 0 is of no key or of scores that are all -inf.)
+constexpr float kLowest = -3.402823466e38f;
+// A row's result x / sum, for a row of maximum m.
+__device__ __forceinline__ float row_result(float x, float m, float sum) {
+  return sum == 0.f ? (m == -INFINITY ? 0.f : NAN) : x / sum;
+}
 
 // x over the lanes of equal lane % 16.
 __device__ __forceinline__ float groups_max(float x) { x = fmaxf(x, partner16(x)); return fmaxf(x, partner32(x)); }
@@ -411,9 +420,10 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       float p32[NB][8];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        float t[8], mx = -INFINITY;
+        float t[8];
         // Keys (of this lane, j = 4 half + r) that the row sees: bit j.
         unsigned sees = 0xff;
+        float mx = kLowest;   // (lowered in the branch: behind it, 64 x 8 tokens over an int8 cache take 313 us for 275)
         if (!clean) {
           sees = 0;
 #pragma unroll
@@ -421,6 +431,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
             const int k = 16 * (j / 4) + 4 * g + j % 4;
             sees |= key0 + k < seen[b] && (present >> k & 1) ? 1u << j : 0u;
           }
+          mx = sees ? kLowest : -INFINITY;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -518,8 +529,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
         *reinterpret_cast<f32x4*>(vw + lq * (D * 4) + (((4 * db + g) ^ lq) * 16)) = o[b][db] * unit[b];
-      // (Scores that are all NaN leave no maximum and a NaN sum, which must not count as a row that sees nothing.)
-      if (lane < 16) stat_lds[wave][0][lane] = m[b] == -INFINITY && ls != 0.f ? 0.f : m[b], stat_lds[wave][1][lane] = ls;
+      if (lane < 16) stat_lds[wave][0][lane] = m[b], stat_lds[wave][1][lane] = ls;
       __syncthreads();
       const int q = tid / 16, part = tid % 16;   // 16 threads a row, D / 16 dims each
       constexpr int EL = D / 16;
@@ -544,7 +554,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
           typedef T TE __attribute__((ext_vector_type(EL)));
           TE y;
 #pragma unroll
-          for (int e = 0; e < EL; ++e) y[e] = from_f32<T>(sum == 0.f ? 0.f : x[e] / sum);
+          for (int e = 0; e < EL; ++e) y[e] = from_f32<T>(row_result(x[e], mx, sum));
           *reinterpret_cast<TE*>(static_cast<T*>(a.o) + (int64_t)(sg.rows.first + token) * a.o_token + hq * a.o_head + part * EL) = y;
         } else {
           float* to = part_rows(w, wg, slot, ROWS, D) + (16 * b + q) * D + part * EL;
@@ -812,15 +822,19 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       }
       return v;
     };
-    auto mask = [&](f32x16 (&s)[NKB], int t, uint64_t present) {
+    auto mask = [&](f32x16 (&s)[NKB], int t, uint64_t present) {   // gives the least of the maximum
       const Bits v = visible(t, present);
+      constexpr unsigned kMine = 0x0f0f0f0fu;   // the lane's keys
+      unsigned any = 0;
 #pragma unroll
-      for (int b = 0; b < NKB; ++b)
+      for (int b = 0; b < NKB; ++b) {
+        any |= v.b[b] & kMine;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = v.b[b] & 1u << (8 * (r / 4) + r % 4) ? s[b][r] : -INFINITY;
+      }
+      return any ? kLowest : -INFINITY;
     };
-    auto row_max = [&](const f32x16 (&s)[NKB]) {
-      float mx = -INFINITY;
+    auto row_max = [&](const f32x16 (&s)[NKB], float mx) {
 #pragma unroll
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
@@ -1035,8 +1049,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       if (pipelined && fits(0, present[0])) {
         qk(sa, k_stage(even));
         scale_scores(sa, 0);
-        if (!is_clean(0, present[0])) mask(sa, 0, present[0]);
-        raise(row_max(sa));
+        raise(row_max(sa, is_clean(0, present[0]) ? kLowest : mask(sa, 0, present[0])));
         settle_first(sa, pa, 0, true);
         __syncthreads();   // iteration 0 replaces K(0)
         auto iteration = [&](auto par, int t, f32x16 (&s)[NKB], f32x16 (&sn)[NKB], V8 (&pf)[PV_STEPS], V8 (&pn)[PV_STEPS]) __attribute__((always_inline)) {
@@ -1107,14 +1120,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
           }
           // (present[0] is tile t + 1's by now. 8 bits: masked after the scales, of which phase B then takes ones.)
           const float* ks_next = ks_lds[(t + 1) % SLOTS];
+          float mx = kLowest;
           if (!is_clean(t + 1, present[0])) {
             scale_scores(sn, t + 1);
-            mask(sn, t + 1, present[0]);
+            mx = mask(sn, t + 1, present[0]);
             ks_next = ones_lds;
           }
           // Phase B: O += V(t) P(t) with the row sums of P(t), the row maxima of S(t+1) and the first half of P(t+1)
           // against the reference as it is; where that is raised after all, the half is taken again.
-          float mx = -INFINITY;
           {
             constexpr int N = PV_STEPS * NDB, EACH = N / 4;
             u32x4 kx[CPT], vx[CPT];
@@ -1215,8 +1228,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         const bool clean = is_clean(t, pres);
         qk(s, k_cur);
         scale_scores(s, t);
-        if (!clean) mask(s, t, pres);
-        raise(row_max(s));
+        raise(row_max(s, clean ? kLowest : mask(s, t, pres)));
         if constexpr (k8) {
           float sum, top, scaled;
           do exponentiate8(s, pf, t, sum, top); while (raise_units(top, scaled));
@@ -1298,7 +1310,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     asm volatile("" : "+v"(ln));
     const int lq = ln % 32, hi = ln / 32, lane = ln;
     const float sum = half_sum(l);
-    const float factor = done ? (sum == 0.f ? 0.f : unit / sum) : unit;
+    const float factor = done ? unit / sum : unit, nothing = m_run == -INFINITY ? 0.f : NAN;
     constexpr int PASSES = 2;   // fp32 rows: half of the wave's rows at a time
     unsigned char* const own = (wave % 4 == 0 ? k_lds0 : wave % 4 == 1 ? v_lds0 : wave % 4 == 2 ? k_lds1 : v_lds1) + wave / 4 * (32 * RB);
     if (done) {
@@ -1309,7 +1321,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         for (int q4 = 0; q4 < 4; ++q4) {
           T4 x;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = from_f32<T>(sum == 0.f ? 0.f : o[db][4 * q4 + r] * factor);
+          for (int r = 0; r < 4; ++r) x[r] = from_f32<T>(sum == 0.f ? nothing : o[db][4 * q4 + r] * factor);
           *reinterpret_cast<T4*>(own + lq * RB + (((4 * db + q4) ^ lq % CR) * 16) + 8 * hi) = x;
         }
 #pragma unroll
@@ -1344,6 +1356,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       if (was_mine && hi == 0) {
         const int r = 32 * wave + lq;
         float* st = part_stats(w, (int)gridDim.x, wg, slot, BM, D);
+        // (Scores that are all NaN leave no maximum and a NaN sum, which must not count as a row that sees nothing.)
         st[r] = m_run == -INFINITY && sum != 0.f ? 0.f : m_run, st[BM + r] = sum;
       }
     }
@@ -1430,7 +1443,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedCache c, RowsQ a, At
     typedef T TE __attribute__((ext_vector_type(EL)));
     TE y;
 #pragma unroll
-    for (int e = 0; e < EL; ++e) y[e] = from_f32<T>(sum == 0.f ? 0.f : x[e] / sum);
+    for (int e = 0; e < EL; ++e) y[e] = from_f32<T>(row_result(x[e], m, sum));
     *reinterpret_cast<TE*>(static_cast<T*>(a.o) + (int64_t)(s.first + token) * a.o_token + hq * a.o_head + part * EL) = y;
   }
 }
