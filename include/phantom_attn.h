@@ -172,7 +172,7 @@ typedef struct pa_paged_cache {
  * code = round(x * (L / amax)) to nearest even in fp32, L = 127 (int8) or 448 (e4m3), amax the row's
  * largest magnitude; a row below 2^-100 is held as zeros, one with an element that is not finite gets a
  * NaN scale. The positions written in one call must be distinct: of two rows for one position either, or
- * parts of both, may remain. */
+ * parts of both, may remain. k and v may be rows of the cache itself, but none that the call writes. */
 int pa_cache_write(const pa_paged_cache* cache, const void* k, const void* v, int dtype, int64_t tokens,
                    int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
                    const int32_t* cu_seqlens, void* stream);
@@ -184,11 +184,11 @@ int pa_cache_read(const pa_paged_cache* cache, void* k, void* v, int dtype, int6
 /* Attention of the new tokens over the cache (which holds them already): new token i of sequence s sees
  * the positions up to its own (causal != 0) or all lengths[s] of them, scores scaled by 1/sqrt(d); a
  * token that sees nothing gets zeros. q and o are [tokens][heads_q][d] with the strides given, heads_q a
- * multiple of the cache's heads (query head h reads head h / (heads_q / heads)); o must not overlap q.
- * Rows behind the last sequence's are left as they are. max_new: an upper bound of the new tokens of a
- * sequence, 0 if unknown; only the choice of the kernel depends on it. workspace:
- * pa_paged_attn_workspace() bytes of device memory, 16-byte aligned, used until the call's kernels end;
- * calls that may overlap need one each. */
+ * multiple of the cache's heads (query head h reads head h / (heads_q / heads)); o must share no memory
+ * with q or anything else that the call reads (its rows may lie between q's). Rows behind the last
+ * sequence's are left as they are. max_new: an upper bound of the new tokens of a sequence, 0 if unknown;
+ * only the choice of the kernel depends on it. workspace: pa_paged_attn_workspace() bytes of device memory,
+ * 16-byte aligned, used until the call's kernels end; calls that may overlap need one each. */
 int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int dtype, int64_t tokens, int64_t heads_q,
                       int64_t q_token_stride, int64_t q_head_stride, int64_t o_token_stride, int64_t o_head_stride,
                       const int32_t* cu_seqlens, int64_t max_new, int causal, void* workspace, int64_t workspace_bytes,

@@ -222,7 +222,29 @@ def _span(t) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
-def check_out(name: str, q, out) -> None:
+def _apart(a, b) -> bool:
+    """Whether no row of a, (tokens, heads, d), shares memory with one of b, of a's shape. Rows of one may lie between
+    those of the other where both have the same strides (slices of one buffer); of unlike strides, a and b must lie
+    apart altogether."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    axes = sorted((n, s, t) for n, s, t in zip(a.shape[:2], a.stride(), b.stride()) if n > 1)
+    if any(s != t for _, s, t in axes):
+        return False
+    # Rows differ by delta + i s0 + j s1 elements, |i| < n0, |j| < n1: for each i the j nearest to none, on either side.
+    delta, d = (b0 - a0) // a.element_size(), a.shape[2]
+    (n0, s0), (n1, s1) = ([(1, 0), (1, 0)] + [(n, s) for n, s, _ in axes])[-2:]
+    for i in range(1 - n0, n0):
+        at = delta + i * s0
+        j = max(1 - n1, min(n1 - 1, -at // s1)) if s1 else 0
+        if abs(at + j * s1) < d or j < n1 - 1 and abs(at + (j + 1) * s1) < d:
+            return False
+    return True
+
+
+def check_out(name: str, q, out, *others) -> None:
+    """out, where a call with queries q writes; `others` are the tensors that it reads beside q (None: none)."""
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         _fail(f"{name}: out must have q's shape, dtype and device")
     if out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8:
@@ -233,9 +255,12 @@ def check_out(name: str, q, out) -> None:
     by_head = (tokens == 1 or ts >= d) and (heads == 1 or hs >= (tokens - 1) * ts + d)
     if not by_token and not by_head:
         _fail(f"{name}: out's rows must not overlap")
-    (a0, a1), (b0, b1) = _span(q), _span(out)
-    if a0 < b1 and b0 < a1:
+    if not _apart(q, out):
         _fail(f"{name}: out must not share memory with q")
+    o0, o1 = _span(out)
+    for t in others:
+        if t is not None and t.data_ptr() < o1 and _span(t)[1] > o0:
+            _fail(f"{name}: out must not share memory with the cache, its scales, the page table, the lengths or the offsets")
 
 
 def check_max_new(name: str, max_new) -> int:

@@ -60,7 +60,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     An 8-bit cache gets codes and scales: scale = amax / L, code = round(x * (L / amax)) to nearest even in
     fp32, with amax the row's largest magnitude and L = 127 (int8) or 448 (float8_e4m3fn). A row below 2**-100
     is held as zeros; one with an element that is not finite gets a NaN scale. The positions written in one
-    call must be distinct (no page shared by two sequences where both write)."""
+    call must be distinct (no page shared by two sequences where both write). k and v may be rows of the cache
+    itself (a page copied to another), but none that the call writes."""
     from . import _call, _stream_ptr
 
     _check("cache_write", k, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale)
@@ -104,8 +105,9 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     1/sqrt(d); query head h reads the cache's head h // (heads_q / heads). A token that sees nothing gets
     zeros. max_new, an upper bound of the new tokens of a sequence, picks the kernel where cu_seqlens hides
     it (a wrong one costs time, not correctness). out: where to write (q's shape and dtype, strides of whole
-    16-byte steps, no memory shared with q); its rows behind the last sequence's stay as they are, those of
-    a new tensor are not set."""
+    16-byte steps, no memory shared with q or the other tensors; with q's own strides its rows may lie between
+    q's, as slices of one buffer do); its rows behind the last sequence's stay as they are, those of a new
+    tensor are not set."""
     from . import _call, _stream_ptr
 
     _check("paged_attn", q, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale)
@@ -113,7 +115,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
     if out is None:
         out = torch.empty_like(q)
     else:
-        _checks.check_out("paged_attn", q, out)
+        _checks.check_out("paged_attn", q, out, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale)
     bound = 0 if max_new is None else _checks.check_max_new("paged_attn", max_new)
     cache = _cache_args(k_cache, v_cache, page_table, lengths, k_scale, v_scale)
     tokens, heads_q, _ = q.shape
