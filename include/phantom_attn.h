@@ -151,7 +151,7 @@ int pa_device_lds_limit(int device, int64_t* bytes);
  * or, with cu_seqlens NULL, tokens / seqs rows each. page_table, lengths and cu_seqlens are int32 on the
  * device and read by the kernels. Whatever they hold, no access leaves the tensors: rows without a
  * position in the table are not written and see no key; offsets are clamped to [0, tokens], and a row that
- * offsets out of order give to two sequences may hold either's result.
+ * offsets out of order give to two sequences is written for the first of them and may hold either's result.
  *
  * dtype is the tensors' (F16 or BF16); the cache's own is the same, or I8 or E4M3 with an fp32 scale for
  * each row in k_scale / v_scale [pages][heads][page_size]: a row stands for code * scale.

@@ -61,17 +61,17 @@ __device__ __forceinline__ int cache_row(const PagedCache& c, int s, int h, int 
   return (page * c.heads + h) * c.page_size + (pos - col * c.page_size);
 }
 
-// The sequence that holds row t, by all lanes of a wave together (t wave-uniform): the number of sequences
-// that end at or before t. One load per 64 sequences, against log2(seqs) dependent ones of a search.
-// seqs if there is none.
+// The first sequence that has row t, by all lanes of a wave together (t wave-uniform): the first offset at or before t
+// whose next one is past it, among 64 offsets a load, against log2(seqs) dependent loads of a search, which offsets out of
+// order would mislead. seqs if none has it.
 __device__ __forceinline__ int find_seq(const PagedCache& c, int t) {
   if (!c.cu) return t / c.per_seq;
-  int n = 0;
-  for (int s0 = 0; s0 < c.seqs; s0 += kWave) {
-    const int s = s0 + (int)threadIdx.x % kWave;
-    n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(s < c.seqs && c.cu[min(s, c.seqs - 1) + 1] <= t));
+  for (int s0 = 0; s0 < c.seqs; s0 += kWave - 1) {
+    const uint64_t begun = __builtin_amdgcn_ballot_w64(c.cu[min(s0 + (int)threadIdx.x % kWave, c.seqs)] <= t);
+    const uint64_t has = begun & ~(begun >> 1) & ~(1ull << (kWave - 1));
+    if (has) return s0 + __builtin_ctzll(has);
   }
-  return n;
+  return c.seqs;
 }
 
 // Eight consecutive elements of a cache row in fp32.
