@@ -958,7 +958,6 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       for (int j = 0; j < AHEAD; ++j) present[j] = present[j + 1];
       present[AHEAD] = next_present;
     };
-    bool pipelined;
     {
       int row0, rows0[CPT];
       row0 = find_row(0, pages[0], in_page_of(0));
@@ -970,7 +969,6 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
         present[j + 1] = present_of(row[j]);
         chunk_rows(row[j], present[j + 1], rows[j]);
       }
-      pipelined = !(k8 && WIDE);
       if constexpr (k8) {
         u32x4 kx[CPT], vx[CPT], k1[CPT];
         to_regs(c.k, k_rs, rows0, kx);
@@ -1046,7 +1044,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       };
       f32x16 sa[NKB], sb[NKB];
       V8 pa[PV_STEPS], pb[PV_STEPS];
-      if (pipelined && fits(0, present[0])) {
+      if (fits(0, present[0])) {
         qk(sa, k_stage(even));
         scale_scores(sa, 0);
         raise(row_max(sa, is_clean(0, present[0]) ? kLowest : mask(sa, 0, present[0])));

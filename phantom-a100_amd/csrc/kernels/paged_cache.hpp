@@ -74,7 +74,7 @@ __device__ __forceinline__ int find_seq(const PagedCache& c, int t) {
   return c.seqs;
 }
 
-// Eight consecutive elements of a cache row in fp32.
+// Eight consecutive elements of a cache row in fp32. (A row in 16 bits has no scale.)
 __device__ __forceinline__ void cached8(const f16* row, int at, float, float (&x)[8]) {
   const f16x8 v = *reinterpret_cast<const f16x8*>(row + at);
 #pragma unroll

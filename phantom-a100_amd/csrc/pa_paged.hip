@@ -12,7 +12,6 @@
 
 namespace {
 
-using pa::device_cus;
 using pa::fail;
 using pa::hip_status;
 
@@ -78,7 +77,7 @@ hipError_t with_types(int dtype, int cache_dtype, int64_t d, F f) {
   return dtype == PA_DTYPE_F16 ? with_cache_type<pa::f16>(cache_dtype, d, f) : with_cache_type<pa::bf16>(cache_dtype, d, f);
 }
 
-constexpr int kCUs = 256;   // MI355X / gfx950
+constexpr int kCUs = 256;   // MI355X / gfx950. (A constant: a workspace's size is asked for without a GPU.)
 
 // The launch of an attention call: rows of a tile, workgroups, and whether tiles are cut.
 struct AttnPlan {
