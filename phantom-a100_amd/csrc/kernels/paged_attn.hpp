@@ -196,7 +196,8 @@ __device__ __forceinline__ float groups_sum(float x) { x += partner16(x); return
 // largest weight, what a key loses below fp16's normal range is at most 2^-33 of that, and neither a key that the row
 // does not see nor a large value that it gives no weight costs it bits.
 constexpr float kUnitLeast = 0x1p-100f, kUnitMost = 0x1p120f, kUnitRoom = 0x1p15f;
-// The unit of a row, `unit` so far, whose largest weight is `top`. (One that is not finite makes the row so in any unit.)
+// The unit of a row, `unit` so far and at least kUnitLeast, whose largest weight is `top`. (One that is not finite makes the
+// row so in any unit.)
 __device__ __forceinline__ float unit_for(float unit, float top) {
   return top > unit * kUnitRoom && top < INFINITY ? fminf(top * 0x1p-8f, kUnitMost) : fmaxf(unit, kUnitLeast);
 }
@@ -465,7 +466,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
           p32[b][j] = p;
         }
         if constexpr (kUnits) {
-          const float was = unit[b], now = unit_for(was, groups_max(top));
+          const float was = unit[b], now = unit_for(fmaxf(was, kUnitLeast), groups_max(top));
           if (__builtin_amdgcn_ballot_w64(now != was) != 0) {
             const float f = now == was ? 1.f : was / now;
             unit[b] = now;

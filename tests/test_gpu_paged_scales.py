@@ -166,3 +166,26 @@ def test_past_32_bit_offsets(d):
     got = cuda_attn.paged_attn(p.q.cuda(), kc, vc, table, p.lengths.cuda(), p.cu.cuda(), **scales).double().cpu()
     rows = [i for i in range(p.q.shape[0]) if i != 99]
     assert bool(((got - ref).abs() <= bound)[rows].all())
+
+
+@pytest.mark.parametrize("kind", list(SEQS))
+@pytest.mark.parametrize("dtype,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("gap", [60.0, 84.0])
+def test_weights_next_to_nothing(kind, dtype, cache, d, gap):
+    """The first key has all the weight and a value of zero; the others' weights times their scales are e^-60 to e^-90,
+    down to fp32's smallest normal numbers. Their sum is zero in 16 bits, and no more than that."""
+    p = po.make(SEQS[kind], d=d, hq=4, hkv=2, dtype=dtype, cache=cache)
+    p.q[..., 0] = 16.0
+    largest = po.LARGEST[cache]
+    for s, (first, count, length) in enumerate(firsts(p)):
+        for pos in range(length):
+            pg, rw = po.slot(p, s, pos)
+            p.k_cache.view(torch.int8)[pg, :, rw] = 0
+            p.k_cache[pg, :, rw, 0] = torch.tensor(largest if pos == 0 else -largest).to(cache)
+            p.scales["k_scale"][pg, :, rw] = gap / 2 * math.sqrt(d) / 16.0 / largest
+            if pos == 0:
+                p.v_cache.view(torch.int8)[pg, :, rw] = 0
+                p.scales["v_scale"][pg, :, rw] = 0.0
+    got = check(p)
+    assert bool((got == 0).all() if dtype == F16 else (got.abs() < 1e-20).all())
