@@ -196,10 +196,11 @@ __device__ __forceinline__ float groups_sum(float x) { x += partner16(x); return
 // largest weight, what a key loses below fp16's normal range is at most 2^-33 of that, and neither a key that the row
 // does not see nor a large value that it gives no weight costs it bits.
 constexpr float kUnitLeast = 0x1p-100f, kUnitMost = 0x1p120f, kUnitRoom = 0x1p15f;
-// The unit of a row, `unit` so far and at least kUnitLeast, whose largest weight is `top`. (One that is not finite makes the
-// row so in any unit.)
+// The unit of a row, `unit` so far and at least kUnitLeast, whose largest weight is `top`. An infinite weight takes the
+// largest unit: the infinity stays one in each dim, and no finite weight becomes another beside it. (A NaN leaves the unit,
+// and makes the row NaN in any.)
 __device__ __forceinline__ float unit_for(float unit, float top) {
-  return top > unit * kUnitRoom && top < INFINITY ? fminf(top * 0x1p-8f, kUnitMost) : fmaxf(unit, kUnitLeast);
+  return top > unit * kUnitRoom ? fminf(top * 0x1p-8f, kUnitMost) : fmaxf(unit, kUnitLeast);
 }
 
 // ---- Few rows a tile: single tokens, and the few tokens of one ----

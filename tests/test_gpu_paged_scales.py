@@ -189,3 +189,25 @@ def test_weights_next_to_nothing(kind, dtype, cache, d, gap):
                 p.scales["v_scale"][pg, :, rw] = 0.0
     got = check(p)
     assert bool((got == 0).all() if dtype == F16 else (got.abs() < 1e-20).all())
+
+
+@pytest.mark.parametrize("kind", list(SEQS))
+@pytest.mark.parametrize("dtype,cache", TYPES + [(BF16, E4M3)], ids=IDS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", [0, 40, -1])
+def test_an_infinite_scale(kind, dtype, cache, d, at):
+    """The rows that see it are infinite by the signs of its codes, NaN where a code is zero; the others are as they were."""
+    p = po.make(SEQS[kind], d=d, hq=4, hkv=2, dtype=dtype, cache=cache)
+    sees = torch.zeros(p.q.shape[0], dtype=torch.bool)
+    for s, (first, count, length) in enumerate(firsts(p)):
+        pos = at % length
+        pg, rw = po.slot(p, s, pos)
+        p.scales["v_scale"][pg, :, rw] = math.inf
+        p.v_cache.view(torch.int8)[pg, :, rw, ::5] = 0
+        sees[first:first + count] = torch.arange(length - count, length) >= pos
+    ref, bound, _ = po.attn(p)
+    got = attend(p).double().cpu()
+    assert bool(torch.isnan(ref[sees][..., ::5]).all()) and bool(torch.isinf(ref[sees]).any())
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), (int(torch.isnan(got).sum()), int(torch.isnan(ref).sum()))
+    inf = torch.isinf(ref)
+    assert torch.equal(got[inf], ref[inf]) and bool(((got - ref).abs() <= bound)[~sees].all())
