@@ -183,7 +183,7 @@ int pa_cache_read(const pa_paged_cache* cache, void* k, void* v, int dtype, int6
 
 /* Attention of the new tokens over the cache (which holds them already): new token i of sequence s sees
  * the positions up to its own (causal != 0) or all lengths[s] of them, scores scaled by 1/sqrt(d); a
- * token that sees nothing gets zeros. q and o are [tokens][heads_q][d] with the strides given, heads_q a
+ * token that sees nothing gets zeros, one whose visible scores are all -inf a NaN. q and o are [tokens][heads_q][d] with the strides given, heads_q a
  * multiple of the cache's heads (query head h reads head h / (heads_q / heads)); o must share no memory
  * with q or anything else that the call reads (its rows may lie between q's). Rows behind the last
  * sequence's are left as they are. max_new: an upper bound of the new tokens of a sequence, 0 if unknown;

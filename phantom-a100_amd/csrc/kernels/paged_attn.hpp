@@ -214,15 +214,20 @@ __device__ __forceinline__ float unit_for(float unit, float top) {
 // S^T leaves lane l with queries l % 16 and keys 4 (l / 16) + r of both halves of the step, which are the
 // k-slots of P^T once V^T is read in that order, so P^T goes from registers to the product.
 // 8-bit rows are widened to 16 bits (exact) on their way; a key's scale multiplies its scores, a value's scale
-// its P before the one rounding of P to the type.
+// its P before the one rounding of P to the type: the operand of a 16-bit product, half a step of each weight (in 32 bits
+// the product would be the fp32 matrix core's, a sixteenth of the rate). Scores, maxima, sums and O are fp32; the sum takes
+// P before its rounding. Errors of the results against 64 bits, beside those of a form that holds P in fp32 too: bf16
+// 0.0017 to 0.0018 of their size and 0.0017, fp16 0.00023 to 0.00024 and 0.00021.
 // A value that is not finite must reach the rows that see it and no others, and 0 x infinity would be a NaN:
 // a step that has one takes its P.V product in fp32 over the visible pairs instead.
 // 64 single tokens over up to 8192 keys, 32 heads over 8, D = 128, bf16: 215 us, 5.5 TB/s; 32 over 16384, 32 over 4,
-// e4m3: 60 us, 5.0 TB/s of codes and scales. One over 1031, which is latency: 11.5 us and 4 of the join.
+// e4m3: 60 us, 5.0 TB/s of codes and scales. One over 1031, which is latency: 9.8 us and 4.5 of the join.
 //
 // Workgroups on a CU: two, but for two blocks of 128 dims in 16 bits, whose queries (32 registers), O (64) and rows
 // on their way (64) leave too few of half the registers (64 x 8 tokens over 8192 keys: 226 us, with two 260). One
-// block with one, 16 bits, 256 x 1 over 700: 109 for 95; in 8 bits, 64 x 1 over 8192 and 64 dims, 108 for 81.
+// block with one, 16 bits, 256 x 1 over 700: 109 for 95; in 8 bits, 64 x 1 over 8192 and 64 dims, 108 for 81. Two blocks
+// of 128 dims in 8 bits fit two workgroups with 16 (bf16) to 29 (fp16) registers in memory, and are faster than one
+// workgroup without: 64 x 8 over 8192, int8, bf16 167 us and 187, fp16 185 and 194; e4m3, fp16 158 and 185.
 constexpr int few_wgs(int d, bool k8, int nb) { return d == 128 && !k8 && nb == 2 ? 1 : 2; }
 template <typename T, typename C, int D, int NB>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_wgs(D, cache_type<C>::k8bit, NB))))
@@ -583,14 +588,18 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 // of those of P(t+1). K(t+2) and V(t+1) arrive meanwhile, a row per page lookup: 16-bit rows straight into LDS;
 // 8-bit rows into a raw buffer of LDS one tile earlier, each thread its own, and from there widened to 16 bits
 // (exact) once for all waves. A key's scale multiplies its scores, a value's scale its P before the one rounding of
-// P to the type (fp16: in the row's unit).
+// P to the type (fp16: in the row's unit), an operand in 16 bits as in the kernel above; in 16 bits the sum takes the
+// rounded P, two weights an instruction, so that numerator and sum are of the same weights. Errors
+// as above: bf16 over e4m3 0.0023 and 0.0017, bf16 0.0019 and 0.0017, fp16 0.00025 and 0.00020.
 // O and l are rescaled only when some row's maximum outgrew its reference by more than 2^8.
 // A value that is not finite must not reach rows that do not see it (0 x infinity is NaN): of a tile that some row
 // does not see whole, each wave looks at its share of the values as they arrive; if one is not finite, the pipeline
 // ends there. The tiles from it on go one by one, those with such a value leave P . V out, and it is added at the
 // end in fp32 over the visible pairs.
-// 4096 tokens at the end of 32768 keys, 32 heads over 8, D = 128, causal: bf16 1.93 to 2.05 ms, 1000 to 1070
-// TFLOP/s (the card's large matrix products reach 1290); e4m3 2.20 ms; D = 64 1.23 ms.
+// 4096 tokens at the end of 32768 keys, 32 heads over 8, D = 128, causal: bf16 1.93 to 2.09 ms, 990 to 1070
+// TFLOP/s (the card's large matrix products reach 1290), fp16 2.03 to 2.07; e4m3 and int8 with bf16 2.24 and 2.33 ms, with
+// fp16, whose units cost three more VALU operations a pair of scores and 9 to 16 registers in memory, 2.51 and 2.58; D = 64
+// 1.28 ms, int8 1.75, with fp16 2.04.
 //
 // Rows of a tile, D = 128, 256 and 128 (one workgroup of 8 waves on a CU, two of 4): that case 2015 and 2183 us, 4 x
 // 2048 120 and 117, 24 x 700 over 4096 456 and 491, 256 x 64 over 640 73 and 85. D = 64 has 128, and as many
@@ -1399,8 +1408,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 // Joins the parts of the tile that workgroup blockIdx.x of the attention kernel began and did not end: its own
 // and those of the workgroups after it, up to the one that ends the tile. 16 threads a row. What bounds it is
 // the latency of its loads, so that no load waits for another but the records: the parts' number comes from
-// 64 records at once, their weights by lane, and their rows four parts at a time. 4 to 5.5 us, beside kernels of 12
-// to 2000.
+// 64 records at once, their weights by lane, and their rows four parts at a time. 4.5 to 6.3 us after tiles of few rows
+// (kernels of 10 to 220 us); after chunks, whose parts are 45 to 67 MB, 14 to 17 (kernels of 74 to 2090).
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedCache c, RowsQ a, AttnWork w, int wgs) {
   constexpr int EL = D / 16, MOST = 64;

@@ -126,8 +126,9 @@ struct RowsIn {
 // One row (a new token's key or value of one head) per LPR lanes, 16 bytes a lane. Rows of a wave run over
 // (token, K or V, head): a token's heads are near each other in the inputs. A row's largest magnitude is a maximum
 // over its lanes, without LDS. Small calls are bound by the chain from offsets over lengths
-// and page table to the store (32 single tokens: 3.2 us), large ones by bytes: 8 x up to 2048 tokens, 16 heads, D = 64,
-// f16, 17.4 us, 4.3 TB/s; 4 x up to 4096, 8 heads, D = 128, bf16 to int8 20.8 us. (Two to eight groups of rows a wave,
+// and page table to the store (32 single tokens: 3.3 us), large ones by bytes: 8 x up to 2048 tokens, 16 heads, D = 64,
+// f16, 17.2 us, 4.3 TB/s; 4 x up to 4096, 8 heads, D = 128, bf16 to int8 21.4 us, 2.8 TB/s: the scales of a page and head
+// come from as many workgroups, each 4 bytes as a write of 32 (25.0 MB written for 20.6). (Two to eight groups of rows a wave,
 // their loads on their way together, are no faster: 18.2 to 24 us and 24 to 27.)
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(256) cache_write_rows(PagedCache c, RowsIn kin, RowsIn vin) {

@@ -103,7 +103,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pa
 
     A token sees the positions up to its own (causal) or all of its sequence's; scores are scaled by
     1/sqrt(d); query head h reads the cache's head h // (heads_q / heads). A token that sees nothing gets
-    zeros. max_new, an upper bound of the new tokens of a sequence, picks the kernel where cu_seqlens hides
+    zeros, one whose visible scores are all -inf a NaN. max_new, an upper bound of the new tokens of a sequence, picks the kernel where cu_seqlens hides
     it (a wrong one costs time, not correctness). out: where to write (q's shape and dtype, strides of whole
     16-byte steps, no memory shared with q or the other tensors; with q's own strides its rows may lie between
     q's, as slices of one buffer do); its rows behind the last sequence's stay as they are, those of a new
