@@ -200,6 +200,72 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
 int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
                                 const int32_t* cu_seqlens, int64_t max_new);
 
+/* ---- Drafted tokens: a step that verifies several tokens of a sequence at once ----
+ *
+ * A sequence's new tokens of such a step are a tree: its token 0, the root, is certain; parents[i] (an index among the
+ * sequence's new tokens, before i; anything else: none) is the token that token i was drafted behind. The new tokens of all
+ * sequences are packed as above, tokens of sequence s being the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1. The first
+ * max_new (at most 1024) of a sequence are its tree. All of this is read by the kernels, and whatever it holds, no access
+ * leaves the tensors. */
+
+/* mask[i], ceil(max_new / 32) words a token: bit j % 32 of word j / 32 is set for j the token itself or one of its
+ * ancestors (tokens behind the tree: none). positions[i]: that of the sequence's first new token, lengths[s] - count, plus
+ * the token's depth. Rows behind the last sequence's are left as they are. cu_seqlens NULL: tokens / seqs each. */
+int pa_draft_tree(const int32_t* parents, const int32_t* lengths, const int32_t* cu_seqlens, int64_t tokens, int64_t seqs,
+                  int64_t max_new, int32_t* mask, int32_t* positions, void* stream);
+
+/* pa_paged_attn_fwd with a mask in the place of `causal`: a new token sees the positions before its sequence's new tokens,
+ * and the new token j whose bit j % 32 of word j / 32 is set in its row mask + i * mask_stride (mask_words words, those past
+ * them 0; any bits, not only a tree's). Workspace: pa_paged_attn_workspace(). */
+int pa_paged_tree_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int dtype, int64_t tokens, int64_t heads_q,
+                           int64_t q_token_stride, int64_t q_head_stride, int64_t o_token_stride, int64_t o_head_stride,
+                           const int32_t* cu_seqlens, int64_t max_new, const int32_t* mask, int64_t mask_words,
+                           int64_t mask_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows to turn: [b][n][heads][d] with the strides given, in elements; the d elements of a row contiguous. out may be in,
+ * with its strides; otherwise they share no memory. */
+typedef struct pa_rope_rows {
+  const void* in;
+  void* out;
+  int64_t in_b, in_n, in_h, out_b, out_n, out_h;
+  int64_t heads;
+} pa_rope_rows;
+
+/* Rotary positions of queries and (k not NULL) keys. dtype: F32, F16 or BF16; d up to 1024. The first 2 * pairs elements of
+ * a row are turned, pair p by positions[..] * freqs[p] (inverse != 0: by its negative): (x, y) becomes
+ * scale * (x cos - y sin, x sin + y cos). Pairs are elements p and p + pairs, or (interleaved != 0) 2 p and 2 p + 1. The
+ * others are copied. positions: int32, or int64 (positions64 != 0), of token (b, n) at b * position_b + n * position_n.
+ * Angles are in 64 bits, right at any 32-bit position. */
+int pa_rope(const pa_rope_rows* q, const pa_rope_rows* k, int dtype, int64_t b, int64_t n, int64_t d, const void* positions,
+            int positions64, int64_t position_b, int64_t position_n, const double* freqs, int64_t pairs, int interleaved,
+            int inverse, float scale, void* stream);
+
+/* Verification of drafted tokens. From each sequence's root on, the drafts behind the current token are tried in order,
+ * and the first one accepted becomes the current token. With p, q the current token's rows of target_probs and draft_probs
+ * [n_tokens][vocab], t the draft's token and u its number in uniform [n_tokens]:
+ *   draft_probs given (each draft a sample of its parent's row): accepted iff u q(t) S(c) < max(p(t) - c q(t), 0), where
+ *     c = 0 and S(0) = 1 at first; after each rejection c grows by S(c), the sum of max(p - c q, 0);
+ *   draft_probs NULL (drafts chosen without chance): accepted iff u m < p(t), m = 1 at first; after each rejection m falls by
+ *     p(t), and t counts as 0.
+ * Then the next token: the first whose sum of weights up to it exceeds u S, u the root's number, S the sum of the weights
+ * max(p - c q, 0) (or of p but for the rejected tokens); p where those are all 0; -1 where p is too. An element of p or q
+ * that is not a positive finite number is 0; a draft whose token is not in [0, vocab) is none. Sums, products and comparisons
+ * are in 64 bits. path [seqs][max_new]: the accepted tokens, root first, as indices among the sequence's new tokens, then
+ * -1; accepted [seqs]: their number, the root's among them; next_tokens [seqs]. A sequence without tokens: -1, 0, -1.
+ * Strides in elements. vocab up to 2^24, seqs up to 65535. workspace: pa_verify_draft_workspace() bytes, 16-byte aligned;
+ * calls that may overlap need one each. */
+int pa_verify_draft(const int64_t* tokens, const int32_t* parents, const float* target_probs, int64_t target_stride,
+                    const float* draft_probs, int64_t draft_stride, const float* uniform, const int32_t* cu_seqlens,
+                    int64_t n_tokens, int64_t seqs, int64_t vocab, int64_t max_new, int32_t* path, int32_t* accepted,
+                    int64_t* next_tokens, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t pa_verify_draft_workspace(int64_t seqs, int64_t vocab);
+
+/* Leaves of a step's new tokens the accepted ones: row path[s * path_stride + j] of sequence s's new tokens becomes row j,
+ * j = 0 .. accepted[s] - 1, keys, values and scales, in place. Paths must ascend (as pa_verify_draft's do); an entry that is
+ * no new token leaves its row as it is. new_lengths[s] = lengths[s] - count + accepted[s]. */
+int pa_cache_keep(const pa_paged_cache* cache, const int32_t* path, int64_t path_width, int64_t path_stride,
+                  const int32_t* accepted, const int32_t* cu_seqlens, int32_t* new_lengths, void* stream);
+
 /* Message for the last nonzero status returned on this thread ("" if none). */
 const char* pa_last_error(void);
 

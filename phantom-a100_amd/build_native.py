@@ -30,7 +30,7 @@ OUT = os.path.join(HERE, "cuda_attn", "libphantom_attn.so")
 # by cuda_attn.
 TILES_OUT = os.path.join(HERE, "cuda_attn", "libphantom_attn_tiles.so")
 RESOURCES = os.path.join(HERE, "cuda_attn", "kernel_resources.json")
-LIBRARIES = {OUT: ["pa_attn.hip", "pa_paged.hip"], TILES_OUT: ["pa_tiles.hip"]}
+LIBRARIES = {OUT: ["pa_attn.hip", "pa_paged.hip", "pa_tree.hip", "pa_draft.hip"], TILES_OUT: ["pa_tiles.hip"]}
 SOURCES = [src for srcs in LIBRARIES.values() for src in srcs]
 ARCH = "gfx950"
 

@@ -34,6 +34,23 @@ struct AttnWork {
   float* parts;        // [workgroup][slot][row][D], then the rows' maxima and sums [workgroup][slot][2][row]
 };
 
+// The same with trees of drafted tokens: beside the keys before its sequence's new tokens, a row sees the new token j
+// whose bit j % 32 is set in word j / 32 of its token's mask row (words past the row: none).
+struct TreeWork : AttnWork {
+  const uint32_t* mask;   // [token][words]
+  int64_t mask_stride;
+  int words;
+};
+template <bool TREE> using WorkOf = std::conditional_t<TREE, TreeWork, AttnWork>;
+// Keys that every row of a sequence sees whatever the masks hold: those before its new tokens.
+__device__ __forceinline__ int keys_before(const SeqRows& s, int capacity) { return clamp_int(s.length - s.count, 0, capacity); }
+// What the row of new token `row` of the packed tensors sees of the 32 keys from `key0` on, bit i for key key0 + i;
+// keys past the sequence's length are not looked at. The keys straddle two words of the mask.
+__device__ __forceinline__ uint32_t tree_bits(const TreeWork& w, const SeqRows& s, int row, int key0) {
+  const uint32_t* m = w.mask + row * w.mask_stride;
+  return mask_window(key0 - (s.length - s.count), w.words, [&](int i) { return m[i]; });
+}
+
 // Workspace of a call: a record and two slots of `rows` rows for each workgroup.
 __host__ __device__ __forceinline__ int64_t attn_record_bytes(int64_t wgs) { return (wgs * sizeof(PartRecord) + 255) / 256 * 256; }
 __host__ __device__ __forceinline__ int64_t attn_workspace(int64_t wgs, int rows, int d) {
@@ -161,9 +178,9 @@ __device__ __forceinline__ u16x2 max_bits(u16x2 acc, u32x4 w) {
   for (int i = 0; i < 4; ++i) acc = __builtin_elementwise_max(acc, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
   return acc;
 }
-template <typename T> constexpr unsigned short kInfBits = 0;
-template <> constexpr unsigned short kInfBits<f16> = 0x7c00;
-template <> constexpr unsigned short kInfBits<bf16> = 0x7f80;
+template <typename T> inline constexpr unsigned short kInfBits = 0;
+template <> inline constexpr unsigned short kInfBits<f16> = 0x7c00;
+template <> inline constexpr unsigned short kInfBits<bf16> = 0x7f80;
 
 // c plus a pair of 16-bit values.
 __device__ __forceinline__ float add_pair(unsigned x, float c, f16*) {
@@ -229,9 +246,9 @@ __device__ __forceinline__ float unit_for(float unit, float top) {
 // of 128 dims in 8 bits fit two workgroups with 16 (bf16) to 29 (fp16) registers in memory, and are faster than one
 // workgroup without: 64 x 8 over 8192, int8, bf16 167 us and 187, fp16 185 and 194; e4m3, fp16 158 and 185.
 constexpr int few_wgs(int d, bool k8, int nb) { return d == 128 && !k8 && nb == 2 ? 1 : 2; }
-template <typename T, typename C, int D, int NB>
+template <typename T, typename C, int D, int NB, bool TREE = false>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_wgs(D, cache_type<C>::k8bit, NB))))
-paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
+paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;
   constexpr bool kUnits = k8 && std::is_same<T, f16>::value;      // each row's O in a unit of its own
@@ -304,6 +321,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
         int token, hq;
         if (tile_row(w.tiles, sg.rows, sg.head, sg.tile, in_row[b], token, hq)) lo = min(lo, seen[b]), hi = max(hi, seen[b]);
       }
+      if constexpr (TREE) lo = keys_before(sg.rows, c.capacity);
 #pragma unroll
       for (int d = 1; d < 16; d *= 2) lo = min(lo, __shfl_xor(lo, d)), hi = max(hi, __shfl_xor(hi, d));
       all_seen = __builtin_amdgcn_readfirstlane(lo);
@@ -359,6 +377,21 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
       const unsigned present = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);   // of the step's 32 keys
       const int key0 = step * kStep;
       const bool clean = present == 0xffffffffu && key0 + kStep <= all_seen;
+      // Keys of the step that the lane's rows may see: those with a page, and a tree's by its mask.
+      unsigned by_mask[NB];
+      if constexpr (TREE)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          by_mask[b] = present;
+          if (!clean) {
+            int token, hq;
+            const bool mine = tile_row(w.tiles, sg.rows, sg.head, sg.tile, in_row[b], token, hq);
+            by_mask[b] &= tree_bits(w, sg.rows, sg.rows.first + (mine ? token : 0), key0);
+          }
+        }
+      auto shown = [&](int b) {
+        if constexpr (TREE) return by_mask[b]; else return present;
+      };
       // ---- V to LDS, S^T
       u16x2 top = {0, 0};
       here();
@@ -436,7 +469,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int k = 16 * (j / 4) + 4 * g + j % 4;
-            sees |= key0 + k < seen[b] && (present >> k & 1) ? 1u << j : 0u;
+            sees |= key0 + k < seen[b] && (shown(b) >> k & 1) ? 1u << j : 0u;
           }
           mx = sees ? kLowest : -INFINITY;
         }
@@ -508,7 +541,7 @@ paged_attn_few(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) p = i == j ? p32[b][i] : p;
             p = __shfl(p, from);
-            if (key0 + k < seen[b] && (present >> k & 1)) {
+            if (key0 + k < seen[b] && (shown(b) >> k & 1)) {
 #pragma unroll
               for (int db = 0; db < NDB; ++db) {
                 typedef T T4 __attribute__((ext_vector_type(4)));
@@ -612,9 +645,9 @@ constexpr int chunk_wgs(int d, bool k8) { return d == 128 ? 1 : k8 ? 2 : 3; }   
 // instructions of the flat kind, after which the compiler waits for all LDS reads instead of the oldest; 8-bit ones
 // are not pipelined at all. The case above takes 2108 us (in buffers 1976), in int8 3129 (2312), with D = 64 2659 (1756).
 constexpr uint32_t kPastBuffer = 0xffffe000u;
-template <typename T, typename C, int D, int BM, bool WIDE>
+template <typename T, typename C, int D, int BM, bool WIDE, bool TREE = false>
 __global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chunk_wgs(D, cache_type<C>::k8bit) * BM / 128)))
-paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
+paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;
   constexpr bool kUnits = k8 && std::is_same<T, f16>::value;   // each row's O in a unit of its own
@@ -704,7 +737,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
       qf[kk] = __builtin_bit_cast(V8, x);
     }
     // Keys that all of the wave's rows see, and that some row does (none: the wave has no rows).
-    int lo = mine ? seen : INT32_MAX, up = seen;
+    int lo = !mine ? INT32_MAX : TREE ? keys_before(sg.rows, c.capacity) : seen, up = seen;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) lo = min(lo, __shfl_xor(lo, d)), up = max(up, __shfl_xor(up, d));
     wave_all = uniform(lo), wave_any = uniform(up);
@@ -825,11 +858,18 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     struct Bits { unsigned b[NKB]; };
     auto visible = [&](int t, uint64_t present) {
       Bits v;
+      int row = 0;
+      if constexpr (TREE) {
+        find_mine();
+        row = sg.rows.first + (mine ? token : 0);
+      }
 #pragma unroll
       for (int b = 0; b < NKB; ++b) {
         const int n = clamp_int(seen - (key_begin + t * BN + 32 * b), 0, 32);
         const unsigned below = n == 32 ? ~0u : (1u << n) - 1;
-        v.b[b] = ((unsigned)(present >> (32 * b)) & below) >> (4 * hi);
+        unsigned shown = (unsigned)(present >> (32 * b)) & below;
+        if constexpr (TREE) shown &= tree_bits(w, sg.rows, row, key_begin + t * BN + 32 * b);
+        v.b[b] = shown >> (4 * hi);
       }
       return v;
     };
@@ -955,7 +995,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
     // t + j's; page holds tile t + 1 + AHEAD's entries.
     int row[AHEAD], rows[AHEAD][CPT];
     uint64_t present[AHEAD + 1];
-    const int tile_all = keys_seen(sg.rows, sg.tile * w.tiles.tokens, c.capacity, w.causal);   // the first row's keys
+    const int tile_all = TREE ? keys_before(sg.rows, c.capacity)   // the first row's keys, which all see
+                              : keys_seen(sg.rows, sg.tile * w.tiles.tokens, c.capacity, w.causal);
     auto whole_tile = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= tile_all; };
     auto advance = [&](int next_row, uint64_t next_present) {   // to the next tile (its new rows[AHEAD - 1] apart)
 #pragma unroll
@@ -1291,7 +1332,8 @@ paged_attn_chunk(PagedCache c, RowsQ a, AttnWork w) {
 #pragma unroll 1
         for (; keys != 0; keys &= keys - 1) {
           const int k = __builtin_ctzll(keys), at = __builtin_amdgcn_readlane(row_t, k);
-          const bool vis = key_begin + t * BN + k < seen;
+          bool vis = key_begin + t * BN + k < seen;
+          if constexpr (TREE) vis = vis && (tree_bits(w, sg.rows, sg.rows.first + (mine ? token : 0), key_begin + t * BN + k) & 1);
           float dot = 0.f, x[8], ks = 1.f, vs = 1.f;
           if constexpr (k8) ks = c.k_scale[at], vs = c.v_scale[at];
 #pragma unroll

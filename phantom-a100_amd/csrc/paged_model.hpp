@@ -55,6 +55,15 @@ __host__ __device__ __forceinline__ int keys_seen(const SeqRows& s, int i, int c
   return clamp_int(causal ? new_token_pos(s, i) + 1 : s.length, 0, capacity);
 }
 
+// 32 bits of a mask over a sequence's new tokens from its bit j0 on, bit i for new token j0 + i: ones before the first (the
+// sequence's earlier keys, which all of them see), zeros past its `words` words. word(i) gives word i.
+template <typename Word>
+__host__ __device__ __forceinline__ uint32_t mask_window(int j0, int words, Word word) {
+  const int i = j0 >> 5;   // (rounded down)
+  const uint32_t lo = i < 0 ? ~0u : i < words ? word(i) : 0u, hi = i + 1 < 0 ? ~0u : i + 1 < words ? word(i + 1) : 0u;
+  return (uint32_t)(((uint64_t)hi << 32 | lo) >> (j0 & 31));
+}
+
 // ---- Work of an attention call, and its division over workgroups ----
 //
 // A tile is up to `rows` query rows that read the same keys: `heads` query heads of one key/value head times

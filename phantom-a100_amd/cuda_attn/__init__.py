@@ -17,6 +17,11 @@ through its C ABI (include/phantom_attn.h); there is no CPU or PyTorch fallback.
 For serving (paged.py): cache_write and cache_read, a paged key/value cache in 16 or 8 bits, and paged_attn,
 the attention of new tokens over it, d=64 or 128, fp16/bf16, query heads in groups per key/value head.
 
+For steps that verify several drafted tokens at once (draft.py): draft_tree, the masks and positions of trees of
+drafts, paged_tree_attn, their attention over the cache, verify_draft, their verification against the target's
+probabilities, and cache_keep, which leaves the accepted ones in the cache. rope (rope.py) turns queries and keys
+to their rotary positions, in these steps and elsewhere.
+
 Extensions over the reference: fused_tc accepts bfloat16 and d=128; the fused entry points take
 `out_dtype=torch.float32` to return fp32 output from fp16/bf16 inputs.
 """
@@ -206,6 +211,8 @@ def reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
 # The paged key/value cache and attention over it (serving): paged.py. Imported here, after the call helpers
 # that it shares.
 from .paged import cache_read, cache_write, paged_attn  # noqa: E402, F401
+from .draft import cache_keep, draft_tree, paged_tree_attn, verify_draft  # noqa: E402, F401
+from .rope import rope, rope_frequencies  # noqa: E402, F401
 
 # Every version, in the order the project builds them.
 KERNELS = {"naive": naive, "tiled": tiled, "fused": fused,

@@ -283,3 +283,154 @@ def read_dtype(name: str, k_cache, dtype) -> torch.dtype:
     if dtype is not None and dtype != k_cache.dtype:
         _fail(f"{name}: dtype must be the cache's own ({k_cache.dtype})")
     return k_cache.dtype
+
+
+# ---------------------------------------------------------------- drafted tokens (draft.py) and rotary positions (rope.py)
+TREE_MAX = 1024
+
+
+def check_vector(name: str, what: str, x, dtype, size, device, *, require_cuda: bool = True) -> None:
+    """A contiguous vector of `size` elements (None: any number of at least one) beside the others of a call."""
+    if (x.dtype is dtype and x.dim() == 1 and (x.shape[0] == size or size is None and x.shape[0] > 0)
+            and x.is_contiguous() and x.device == device and (x.is_cuda or not require_cuda)):
+        return
+    if require_cuda and not x.is_cuda:
+        _fail(f"{name}: inputs must be CUDA tensors")
+    if x.device != device:
+        _fail(f"{name}: inputs must be on the same device")
+    if x.numel() == 0:
+        _fail(f"{name}: inputs must be non-empty")
+    shape = "" if size is None else f" of {size} elements"
+    _fail(f"{name}: {what} must be a contiguous {str(dtype).replace('torch.', '')} vector{shape}")
+
+
+def check_tree(name: str, parents, seqs: int, cu_seqlens, max_new, *, require_cuda: bool = True) -> int:
+    """The new tokens of a call and their trees; the most tokens of a tree."""
+    check_vector(name, "parents", parents, torch.int32, None, parents.device, require_cuda=require_cuda)
+    tokens = parents.shape[0]
+    if seqs < 1:
+        _fail(f"{name}: inputs must be non-empty")
+    if cu_seqlens is None:
+        if tokens % seqs:
+            _fail(f"{name}: without cu_seqlens the tokens must divide evenly over the sequences")
+    else:
+        check_vector(name, "cu_seqlens", cu_seqlens, torch.int32, seqs + 1, parents.device, require_cuda=require_cuda)
+    if max_new is None:
+        most = tokens // seqs if cu_seqlens is None else tokens
+        if cu_seqlens is None and most > TREE_MAX:
+            _fail(f"{name}: a tree has at most {TREE_MAX} tokens")
+        return min(most, TREE_MAX)
+    if isinstance(max_new, bool) or not isinstance(max_new, int) or not 1 <= max_new <= TREE_MAX:
+        _fail(f"{name}: max_new must be a number of tokens from 1 to {TREE_MAX}")
+    return max_new
+
+
+def check_mask(name: str, mask, q) -> None:
+    """A mask of the new tokens of q."""
+    if mask.device != q.device:
+        _fail(f"{name}: inputs must be on the same device")
+    if (mask.dim() != 2 or mask.dtype is not torch.int32 or mask.shape[0] != q.shape[0] or mask.shape[1] < 1
+            or mask.stride(1) != 1 and mask.shape[1] > 1):
+        _fail(f"{name}: mask must be a (tokens, words) int32 tensor with contiguous rows")
+
+
+def check_no_overlap(name: str, out, x, what: str) -> None:
+    (o0, o1), (x0, x1) = _span(out), _span(x)
+    if x0 < o1 and o0 < x1:
+        _fail(f"{name}: out must not share memory with {what}")
+
+
+def check_probs(name: str, what: str, x, tokens: int, device, vocab=None, *, require_cuda: bool = True) -> None:
+    if require_cuda and not x.is_cuda:
+        _fail(f"{name}: inputs must be CUDA tensors")
+    if x.device != device:
+        _fail(f"{name}: inputs must be on the same device")
+    if x.dim() != 2 or x.shape[0] != tokens or x.dtype is not torch.float32 or x.stride(1) != 1 and x.shape[1] > 1:
+        _fail(f"{name}: {what} must be a (tokens, vocab) float32 tensor with contiguous rows")
+    if x.shape[1] < 1:
+        _fail(f"{name}: inputs must be non-empty")
+    if vocab is not None and x.shape[1] != vocab:
+        _fail(f"{name}: target_probs and draft_probs must be of one vocabulary")
+
+
+def check_path(name: str, path, seqs: int, device) -> None:
+    if path.device != device:
+        _fail(f"{name}: inputs must be on the same device")
+    if (path.dim() != 2 or path.shape[0] != seqs or path.shape[1] < 1 or path.dtype is not torch.int32
+            or path.stride(1) != 1 and path.shape[1] > 1):
+        _fail(f"{name}: path must be a (B, columns) int32 tensor with contiguous rows")
+
+
+ROPE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+ROPE_MAX_DIM = 1024
+
+
+def _rows_overlap(x) -> bool:
+    """Whether elements of a tensor may share memory: its axes, by their strides, must each step past all inner ones."""
+    end = 1
+    for stride, size in sorted((s, n) for n, s in zip(x.shape, x.stride()) if n > 1):
+        if stride < end:
+            return True
+        end = stride * (size - 1) + end
+    return False
+
+
+def _tokens_apart(q, k, token: int) -> bool:
+    """Whether q and k, of the same tokens, share no memory: they lie apart, or each token's rows of the one beside those of
+    the other within one stride of the tokens (slices of one projection)."""
+    (q0, q1), (k0, k1) = _span(q), _span(k)
+    if q1 <= k0 or k1 <= q0:
+        return True
+    step = q.stride(token)
+    others = [s for x in (q, k) for i, (n, s) in enumerate(zip(x.shape, x.stride())) if i not in (1, token, x.dim() - 1) and n > 1]
+    if k.stride(token) != step or step < 1 or any(s % step for s in others):
+        return False
+    size = q.element_size()
+    if (k0 - q0) % size:
+        return False
+    wide = [(x.shape[1] - 1) * x.stride(1) + x.shape[-1] for x in (q, k)]
+    at = (k0 - q0) // size % step
+    return at >= wide[0] and at + wide[1] <= step
+
+
+def check_rope(name: str, q, k, positions, freqs, inplace: bool, *, require_cuda: bool = True) -> None:
+    device, dtype, shape = q.device, q.dtype, q.shape
+    for t in (q, k, positions, freqs):
+        if t is None:
+            continue
+        if require_cuda and not t.is_cuda:
+            _fail(f"{name}: inputs must be CUDA tensors")
+        if t.device != device:
+            _fail(f"{name}: inputs must be on the same device")
+    if len(shape) not in (3, 4):
+        _fail(f"{name}: q and k must be shaped (tokens, heads, d) or (B, heads, N, d)")
+    if dtype not in ROPE_DTYPES:
+        _fail(f"{name}: float32, float16 or bfloat16 only")
+    if 0 in shape or k is not None and 0 in k.shape:
+        _fail(f"{name}: inputs must be non-empty")
+    if k is not None:
+        if k.dtype is not dtype:
+            _fail(f"{name}: q and k must share a dtype")
+        if k.dim() != len(shape) or k.shape[0] != shape[0] or k.shape[2:] != shape[2:]:
+            _fail(f"{name}: q and k must have the same tokens and head dimension")
+    if shape[-1] > ROPE_MAX_DIM:
+        _fail(f"{name}: head dimensions up to {ROPE_MAX_DIM}")
+    for x in (q, k):
+        if x is not None and x.stride(-1) != 1 and shape[-1] > 1:
+            _fail(f"{name}: rows must be contiguous")
+    if positions.dtype not in (torch.int32, torch.int64):
+        _fail(f"{name}: positions must be int32 or int64")
+    if len(shape) == 3:
+        fits = positions.shape == shape[:1]
+    else:
+        fits = positions.shape == (shape[2],) or positions.shape == (shape[0], shape[2])
+    if not fits:
+        _fail(f"{name}: positions must be (tokens,), or (N,) or (B, N) for (B, heads, N, d)")
+    if freqs.dim() != 1 or freqs.dtype is not torch.float64 or not freqs.is_contiguous() or not 1 <= freqs.shape[0] <= shape[-1] // 2:
+        _fail(f"{name}: freqs must be a contiguous float64 vector of 1 to d / 2 elements")
+    if inplace:
+        for x in (q, k):
+            if x is not None and _rows_overlap(x):
+                _fail(f"{name}: rows that are written must not overlap")
+        if k is not None and not _tokens_apart(q, k, 0 if len(shape) == 3 else 2):
+            _fail(f"{name}: q and k must not share memory")
