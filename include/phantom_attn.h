@@ -252,13 +252,13 @@ int pa_rope(const pa_rope_rows* q, const pa_rope_rows* k, int dtype, int64_t b, 
  * that is not a positive finite number is 0; a draft whose token is not in [0, vocab) is none. Sums, products and comparisons
  * are in 64 bits. path [seqs][max_new]: the accepted tokens, root first, as indices among the sequence's new tokens, then
  * -1; accepted [seqs]: their number, the root's among them; next_tokens [seqs]. A sequence without tokens: -1, 0, -1.
- * Strides in elements. vocab up to 2^24, seqs up to 65535. workspace: pa_verify_draft_workspace() bytes, 16-byte aligned;
- * calls that may overlap need one each. */
+ * Strides in elements. vocab up to 2^24, seqs up to 65535. workspace: pa_verify_draft_workspace() bytes (drawn: whether
+ * draft_probs are given), 16-byte aligned; calls that may overlap need one each. 0 bytes: it may be NULL. */
 int pa_verify_draft(const int64_t* tokens, const int32_t* parents, const float* target_probs, int64_t target_stride,
                     const float* draft_probs, int64_t draft_stride, const float* uniform, const int32_t* cu_seqlens,
                     int64_t n_tokens, int64_t seqs, int64_t vocab, int64_t max_new, int32_t* path, int32_t* accepted,
                     int64_t* next_tokens, void* workspace, int64_t workspace_bytes, void* stream);
-int64_t pa_verify_draft_workspace(int64_t seqs, int64_t vocab);
+int64_t pa_verify_draft_workspace(int64_t seqs, int64_t vocab, int drawn);
 
 /* Leaves of a step's new tokens the accepted ones: row path[s * path_stride + j] of sequence s's new tokens becomes row j,
  * j = 0 .. accepted[s] - 1, keys, values and scales, in place. Paths must ascend (as pa_verify_draft's do); an entry that is

@@ -63,6 +63,11 @@ __global__ void __launch_bounds__(256) draft_tree_rows(TreeArgs a) {
 // number, S the sum of the weights max(p - c q, 0) (or p without the rejected tokens); if S is 0, p's.
 // Sums, products and comparisons are in 64 bits: the next token lies between sums over the whole vocabulary, and in 32 bits
 // one draw in a hundred would miss it.
+//
+// The weights of a row are summed in runs of 1024 elements, each by a wave, and the next token is looked for among the
+// runs' sums first and in one run then. Short vocabularies go in one workgroup a sequence and one launch, long ones in as
+// many waves as the rows have runs, a launch behind the walk.
+struct VerifyState;
 struct VerifyArgs {
   const int64_t* tokens;
   const int* parents;
@@ -71,40 +76,53 @@ struct VerifyArgs {
   const float* u;
   const int* cu;
   int64_t p_stride, q_stride;
-  int n_tokens, vocab, most, splits;
+  int n_tokens, vocab, most, runs;
   int* path;                 // [seqs][most]
   int* accepted;
   int64_t* next;
-  struct VerifyState* states;   // [seqs]
-  double* sums;              // [seqs][splits]
+  VerifyState* states;       // [seqs]
+  double* sums;              // [seqs][runs]
 };
-// Where a sequence's path ended: the row of probabilities, c, and the sequence's rows.
+// Where a sequence's path ended: its row of probabilities is first + node.
 struct VerifyState {
-  double off;
+  double off;                // c
   int first, tree, node, pad;
 };
-constexpr int kVerifyChunk = 4096;   // elements of a row that a workgroup sums
+constexpr int kRun = 1024, kRunEach = kRun / kWave;
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // four elements of a row, wherever it begins
 
-__device__ __forceinline__ double weight_of(float x) { return x > 0.f && x < INFINITY ? (double)x : 0.0; }
+// An element as it counts, and what is left of it after `off` times q's.
+// (0x180: positive and finite, by v_cmp_class.)
+__device__ __forceinline__ double weight_of(float x) { return __builtin_amdgcn_classf(x, 0x180) ? (double)x : 0.0; }
+__device__ __forceinline__ double left_of(double p, double off, double q) { return fmax(fma(-off, q, p), 0.0); }
 
-// What is left of p after `off` times q. (The product is rounded by itself: p - off q is 0 where the two are equal.)
-__device__ __forceinline__ double left_of(double p, double off, double q) {
-#pragma clang fp contract(off)
-  const double x = p - off * q;
-  return x > 0 ? x : 0.0;
+// x of another lane, by a move of its halves (common.hpp).
+template <typename Move>
+__device__ __forceinline__ double move_halves(double x, Move move) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const unsigned lo = __builtin_bit_cast(unsigned, move(__builtin_bit_cast(float, (unsigned)u)));
+  const unsigned hi = __builtin_bit_cast(unsigned, move(__builtin_bit_cast(float, (unsigned)(u >> 32))));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-
-// The sum of x over the workgroup's threads, the same in all of them and in the same order always. lds: 16 numbers.
+// Sums over 16 lanes that follow each other, and over the wave; the same in all lanes (a tree of the same pairs for each).
+__device__ __forceinline__ double row_sum16(double x) {
+  x += move_halves(x, [](float y) { return dpp_move<0xB1>(y); });
+  x += move_halves(x, [](float y) { return dpp_move<0x4E>(y); });
+  x += move_halves(x, [](float y) { return dpp_move<0x141>(y); });
+  return x + move_halves(x, [](float y) { return dpp_move<0x140>(y); });
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  x = row_sum16(x);
+  x += move_halves(x, [](float y) { return partner16(y); });
+  return x + move_halves(x, [](float y) { return partner32(y); });
+}
+// The sum of x over a workgroup of 1024 threads, the same in all of them and in the same order always. lds: 16 numbers.
 __device__ __forceinline__ double block_sum(double x, double* lds) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
-  const int waves = (int)blockDim.x / kWave;
+  x = wave_sum(x);
   __syncthreads();
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = x;
   __syncthreads();
-  double sum = 0;
-  for (int i = 0; i < waves; ++i) sum += lds[i];
-  return sum;
+  return row_sum16(lds[threadIdx.x % 16]);
 }
 
 // What the walk needs of each draft. 20 KB of LDS.
@@ -113,6 +131,36 @@ struct Drafts {
   int token[kTreeMax];
   float p[kTreeMax], q[kTreeMax], u[kTreeMax];
 };
+
+// S(off) of a row, by a workgroup of 1024 threads, 16 elements a thread and step.
+__device__ __forceinline__ double row_left(const VerifyArgs& a, int64_t row, double off, double* lds) {
+  constexpr int EACH = 4, STEP = EACH * 4096;
+  const float* pr = a.p + row * a.p_stride;
+  const float* qr = a.q + row * a.q_stride;
+  double sum = 0;
+  int v0 = 0;
+  for (; v0 + STEP <= a.vocab; v0 += STEP) {
+    f32x4u p[EACH], q[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int v = v0 + 4 * ((int)threadIdx.x + 1024 * k);
+      p[k] = *reinterpret_cast<const f32x4u*>(pr + v), q[k] = *reinterpret_cast<const f32x4u*>(qr + v);
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += left_of(weight_of(p[k][j]), off, weight_of(q[k][j]));
+  }
+  float p[4 * EACH], q[4 * EACH];   // the rest, all loads on their way together
+#pragma unroll
+  for (int k = 0; k < 4 * EACH; ++k) {
+    const int v = v0 + (int)threadIdx.x + 1024 * k;
+    p[k] = v < a.vocab ? pr[v] : 0.f, q[k] = v < a.vocab ? qr[v] : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < 4 * EACH; ++k) sum += left_of(weight_of(p[k]), off, weight_of(q[k]));
+  return block_sum(sum, lds);
+}
 
 // The walk of one sequence, by all threads of a workgroup alike. path: where the path goes, null if nowhere. Returns the
 // number of accepted tokens.
@@ -161,14 +209,8 @@ __device__ __forceinline__ int verify_walk(const VerifyArgs& a, int s, Drafts& d
       bool yes;
       if constexpr (DRAWN) {
         const double q = weight_of(d.q[child]);
-        double size = 1.0;
-        if (st.off != 0.0) {   // (another draft behind a rejected one)
-          const float* pr = a.p + (r.first + st.node) * a.p_stride;
-          const float* qr = a.q + (r.first + st.node) * a.q_stride;
-          double sum = 0;
-          for (int v = tid; v < a.vocab; v += (int)blockDim.x) sum += left_of(weight_of(pr[v]), st.off, weight_of(qr[v]));
-          size = block_sum(sum, lds);
-        }
+        // (S(0) is 1; another draft behind a rejected one needs a row's sum)
+        const double size = st.off != 0.0 ? row_left(a, r.first + st.node, st.off, lds) : 1.0;
         yes = u * q * size < left_of(p, st.off, q);
         if (!yes) st.off += size;
       } else {
@@ -186,167 +228,209 @@ __device__ __forceinline__ int verify_walk(const VerifyArgs& a, int s, Drafts& d
   }
   return accepted;
 }
-
-// Bits of the tokens from v0 on, a chunk of them, that the drafts behind `node` had. All threads; bits: a chunk's.
-__device__ __forceinline__ void rejected_bits(const VerifyArgs& a, const VerifyState& st, int v0, unsigned* bits) {
-  for (int i = (int)threadIdx.x; i < kVerifyChunk / 32; i += (int)blockDim.x) bits[i] = 0;
-  __syncthreads();
-  for (int i = st.node + 1 + (int)threadIdx.x; i < st.tree; i += (int)blockDim.x)
-    if (a.parents[st.first + i] == st.node) {
-      const int64_t t = a.tokens[st.first + i];
-      if (t >= v0 && t - v0 < kVerifyChunk) atomicOr(&bits[(t - v0) / 32], 1u << (t - v0) % 32);
-    }
-  __syncthreads();
+__device__ __forceinline__ void write_walk(const VerifyArgs& a, int s, int* path, int accepted, const VerifyState& st) {
+  for (int i = accepted + (int)threadIdx.x; i < a.most; i += (int)blockDim.x) path[i] = -1;
+  if (threadIdx.x == 0) a.accepted[s] = accepted, a.states[s] = st;
 }
 
-// A sequence whose drafts were drawn: its walk, which may have to sum rows.
-__global__ void __launch_bounds__(1024) verify_drawn(VerifyArgs a) {
+// Weights of a wave's elements of a run that starts at v0, 16 a lane: element e(k) = kRunEach * lane + k (by_lane) or
+// 4 * lane + 256 * (k / 4) + k % 4. out: bits of the run's tokens that count as 0, null if none do.
+__device__ __forceinline__ int run_element(bool by_lane, int k) {
+  const int lane = (int)threadIdx.x % kWave;
+  return by_lane ? kRunEach * lane + k : 4 * lane + 256 * (k / 4) + k % 4;
+}
+template <bool DRAWN>
+__device__ __forceinline__ void run_weights(const VerifyArgs& a, int64_t row, double off, int v0, bool by_lane, const unsigned* out,
+                                            double (&x)[kRunEach]) {
+  const float* pr = a.p + row * a.p_stride + v0;
+  const float* qr = DRAWN && off != 0.0 ? a.q + row * a.q_stride + v0 : pr;
+  float p[kRunEach], q[kRunEach];
+  if (v0 + kRun <= a.vocab) {
+#pragma unroll
+    for (int k = 0; k < kRunEach; k += 4) {
+      const f32x4u y = *reinterpret_cast<const f32x4u*>(pr + run_element(by_lane, k));
+      const f32x4u z = DRAWN ? *reinterpret_cast<const f32x4u*>(qr + run_element(by_lane, k)) : y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[k + j] = y[j], q[k + j] = z[j];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRunEach; ++k) {
+      const int e = run_element(by_lane, k);
+      p[k] = v0 + e < a.vocab ? pr[e] : 0.f;
+      q[k] = DRAWN && v0 + e < a.vocab ? qr[e] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRunEach; ++k) {
+    double w = weight_of(p[k]);
+    if constexpr (DRAWN) w = off != 0.0 ? left_of(w, off, weight_of(q[k])) : w;
+    if (out) {
+      const int e = run_element(by_lane, k);
+      w = out[e / 32] >> e % 32 & 1 ? 0.0 : w;
+    }
+    x[k] = w;
+  }
+}
+template <bool DRAWN>
+__device__ __forceinline__ double run_sum(const VerifyArgs& a, int64_t row, double off, int v0, const unsigned* out) {
+  double x[kRunEach], sum = 0;
+  run_weights<DRAWN>(a, row, off, v0, false, out, x);
+#pragma unroll
+  for (int k = 0; k < kRunEach; ++k) sum += x[k];
+  return wave_sum(sum);
+}
+// Bits of the tokens of a run from v0 on that the drafts behind the last token had, by one wave (a run's bits are its own).
+__device__ __forceinline__ void rejected_bits(const VerifyArgs& a, const VerifyState& st, int v0, unsigned* bits) {
+  const int lane = (int)threadIdx.x % kWave;
+  if (lane < kRun / 32) bits[lane] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int i = st.node + 1 + lane; i < st.tree; i += kWave)
+    if (a.parents[st.first + i] == st.node) {
+      const int64_t t = a.tokens[st.first + i];
+      if (t >= v0 && t - v0 < kRun) atomicOr(&bits[(t - v0) / 32], 1u << (t - v0) % 32);
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// The next token, by one wave: `sums` are those of the row's runs. Lane l takes the runs l G to (l + 1) G - 1, then 16
+// elements of the run that was found.
+template <bool DRAWN>
+__device__ __forceinline__ int64_t pick_token(const VerifyArgs& a, const VerifyState& st, const double* sums, unsigned* bits) {
+  const int lane = (int)threadIdx.x % kWave;
+  const int64_t row = st.first + st.node;
+  const int group = (a.runs + kWave - 1) / kWave, r0 = lane * group, r1 = min(r0 + group, a.runs);
+  double off = st.off, mine = 0;
+  bool whole = false;   // p as it is
+  for (int r = r0; r < r1; ++r) mine += sums[r];
+  if (!(wave_sum(mine) > 0)) {   // nothing is left of it
+    whole = true;
+    off = 0.0;
+    mine = 0;
+    for (int r = 0; r < a.runs; ++r) {
+      const double sum = run_sum<DRAWN>(a, row, 0.0, r * kRun, nullptr);
+      mine += r >= r0 && r < r1 ? sum : 0.0;
+    }
+  }
+  auto scan = [&](double x) {   // sums up to the lane's
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const double other = __shfl_up(x, d);
+      if (lane >= d) x += other;
+    }
+    return x;
+  };
+  // The first lane with weight whose sum up to it exceeds theta; else (rounding, or u from 1 on) the last with weight.
+  auto choose = [&](double x, double upto, double theta) {
+    const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0), over = __builtin_amdgcn_ballot_w64(x > 0 && upto > theta);
+    return over ? __builtin_ctzll(over) : some ? kWave - 1 - __builtin_clzll(some) : -1;
+  };
+  double upto = scan(mine);
+  double theta = (double)a.u[st.first] * __shfl(upto, kWave - 1);
+  int at = choose(mine, upto, theta);
+  if (at < 0) return -1;
+  theta -= __shfl(upto - mine, at);   // (the lane's own runs)
+  int run = 0;
+  {
+    double sum = 0, before = 0;
+    for (int r = at * group; r < min((at + 1) * group, a.runs); ++r) {
+      const double x = whole ? run_sum<DRAWN>(a, row, 0.0, r * kRun, nullptr) : sums[r];
+      if (x > 0) run = r, before = sum;
+      sum += x;
+      if (x > 0 && sum > theta) break;
+    }
+    theta -= before;
+  }
+  const int v0 = run * kRun;
+  if (!DRAWN && !whole) rejected_bits(a, st, v0, bits);
+  double x[kRunEach];
+  run_weights<DRAWN>(a, row, off, v0, true, !DRAWN && !whole ? bits : nullptr, x);
+  mine = 0;
+#pragma unroll
+  for (int k = 0; k < kRunEach; ++k) mine += x[k];
+  upto = scan(mine);
+  at = choose(mine, upto, theta);
+  double sum = upto - mine;
+  int here = -1, last = -1;
+#pragma unroll
+  for (int k = 0; k < kRunEach; ++k) {
+    sum += x[k];
+    if (x[k] > 0) last = k;
+    if (x[k] > 0 && here < 0 && sum > theta) here = k;
+  }
+  here = __shfl(here < 0 ? last : here, at < 0 ? 0 : at);
+  return at < 0 ? -1 : v0 + kRunEach * at + here;
+}
+
+// The whole of a sequence in one workgroup. Dynamic LDS: the runs' sums.
+template <bool DRAWN>
+__global__ void __launch_bounds__(1024) verify_whole(VerifyArgs a) {
+  extern __shared__ double sums[];
   __shared__ Drafts d;
   __shared__ double lds[16];
-  const int s = (int)blockIdx.x;
+  __shared__ unsigned bits[16][kRun / 32];
+  const int s = (int)blockIdx.x, wave = (int)threadIdx.x / kWave;
   VerifyState st;
   int* path = a.path + (int64_t)s * a.most;
-  const int accepted = verify_walk<true>(a, s, d, lds, path, st);
+  const int accepted = verify_walk<DRAWN>(a, s, d, lds, path, st);
   for (int i = accepted + (int)threadIdx.x; i < a.most; i += 1024) path[i] = -1;
-  if (threadIdx.x == 0) {
-    a.accepted[s] = accepted;
-    a.states[s] = st;
+  if (threadIdx.x == 0) a.accepted[s] = accepted;
+  if (st.tree == 0) {
+    if (threadIdx.x == 0) a.next[s] = -1;
+    return;
+  }
+  for (int r = wave; r < a.runs; r += 16) {
+    if constexpr (!DRAWN) rejected_bits(a, st, r * kRun, bits[wave]);
+    const double sum = run_sum<DRAWN>(a, st.first + st.node, st.off, r * kRun, DRAWN ? nullptr : bits[wave]);
+    if (threadIdx.x % kWave == 0) sums[r] = sum;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int64_t token = pick_token<DRAWN>(a, st, sums, bits[0]);
+    if (threadIdx.x == 0) a.next[s] = token;
   }
 }
 
-// The sum of a chunk of the last row's weights. Where the drafts are no samples, each workgroup walks its sequence by itself
-// (no row has to be summed for it), and that of the first chunk writes the path. Grid: chunks, sequences.
+// The walk alone, of a sequence whose drafts were drawn (it may have to sum rows).
+__global__ void __launch_bounds__(1024) verify_drawn(VerifyArgs a) {
+  __shared__ Drafts d;
+  __shared__ double lds[16];
+  VerifyState st;
+  int* path = a.path + (int64_t)blockIdx.x * a.most;
+  const int accepted = verify_walk<true>(a, (int)blockIdx.x, d, lds, path, st);
+  write_walk(a, (int)blockIdx.x, path, accepted, st);
+}
+
+// The runs' sums of the last row, one a wave. Where the drafts are no samples, each workgroup walks its sequence by itself
+// (no row has to be summed for that), and the first one writes the path. Grid: four runs, sequences.
 template <bool DRAWN>
 __global__ void __launch_bounds__(256) verify_sums(VerifyArgs a) {
   __shared__ Drafts d;
   __shared__ double lds[16];
-  __shared__ unsigned bits[kVerifyChunk / 32];
-  const int s = (int)blockIdx.y, v0 = (int)blockIdx.x * kVerifyChunk;
+  __shared__ unsigned bits[4][kRun / 32];
+  const int s = (int)blockIdx.y, wave = (int)threadIdx.x / kWave, r = (int)blockIdx.x * 4 + wave;
   VerifyState st;
   if constexpr (DRAWN) {
     st = a.states[s];
   } else {
     int* path = blockIdx.x == 0 ? a.path + (int64_t)s * a.most : nullptr;
     const int accepted = verify_walk<false>(a, s, d, lds, path, st);
-    if (path) {
-      for (int i = accepted + (int)threadIdx.x; i < a.most; i += 256) path[i] = -1;
-      if (threadIdx.x == 0) {
-        a.accepted[s] = accepted;
-        a.states[s] = st;
-      }
-    }
+    if (path) write_walk(a, s, path, accepted, st);
   }
-  if (st.tree == 0) return;
-  if constexpr (!DRAWN) rejected_bits(a, st, v0, bits);
-  const int64_t row = st.first + st.node;
-  double sum = 0;
-#pragma unroll
-  for (int k = 0; k < kVerifyChunk / 256; ++k) {
-    const int e = k * 256 + (int)threadIdx.x, v = v0 + e;
-    if (v >= a.vocab) break;
-    double x = weight_of(a.p[row * a.p_stride + v]);
-    if constexpr (DRAWN) {
-      if (st.off != 0.0) x = left_of(x, st.off, weight_of(a.q[row * a.q_stride + v]));
-    } else {
-      x = bits[e / 32] >> e % 32 & 1 ? 0.0 : x;
-    }
-    sum += x;
-  }
-  sum = block_sum(sum, lds);
-  if (threadIdx.x == 0) a.sums[(int64_t)s * a.splits + blockIdx.x] = sum;
+  if (st.tree == 0 || r >= a.runs) return;
+  if constexpr (!DRAWN) rejected_bits(a, st, r * kRun, bits[wave]);
+  const double sum = run_sum<DRAWN>(a, st.first + st.node, st.off, r * kRun, DRAWN ? nullptr : bits[wave]);
+  if (threadIdx.x % kWave == 0) a.sums[(int64_t)s * a.runs + r] = sum;
 }
 
-// The next token of a sequence: the chunk that u S falls into by the chunks' sums, then the element. Dynamic LDS: the
-// chunks' sums.
+// The next token of a sequence, behind the runs' sums.
 template <bool DRAWN>
-__global__ void __launch_bounds__(256) verify_pick(VerifyArgs a) {
-  extern __shared__ double sums[];
-  __shared__ double lds[16];
-  __shared__ double upto[256];
-  __shared__ unsigned bits[kVerifyChunk / 32];
-  __shared__ int found, last;
-  __shared__ double before;
-  const int s = (int)blockIdx.x, tid = (int)threadIdx.x;
+__global__ void __launch_bounds__(kWave) verify_pick(VerifyArgs a) {
+  __shared__ unsigned bits[kRun / 32];
+  const int s = (int)blockIdx.x;
   const VerifyState st = a.states[s];
-  if (st.tree == 0) {
-    if (tid == 0) a.next[s] = -1;
-    return;
-  }
-  const int64_t row = st.first + st.node;
-  const float* pr = a.p + row * a.p_stride;
-  const float* qr = DRAWN ? a.q + row * a.q_stride : nullptr;
-  double off = st.off;
-  bool whole = false;   // p as it is
-  for (int i = tid; i < a.splits; i += 256) sums[i] = a.sums[(int64_t)s * a.splits + i];
-  __syncthreads();
-  double total = 0;
-  for (int i = 0; i < a.splits; ++i) total += sums[i];
-  if (!(total > 0)) {   // nothing is left of p: p itself
-    whole = true;
-    off = 0.0;
-    for (int c = 0; c < a.splits; ++c) {
-      double sum = 0;
-      for (int v = c * kVerifyChunk + tid; v < min(a.vocab, (c + 1) * kVerifyChunk); v += 256) sum += weight_of(pr[v]);
-      sum = block_sum(sum, lds);
-      if (tid == 0) sums[c] = sum;
-    }
-    __syncthreads();
-    total = 0;
-    for (int i = 0; i < a.splits; ++i) total += sums[i];
-    if (!(total > 0)) {
-      if (tid == 0) a.next[s] = -1;
-      return;
-    }
-  }
-  const double theta = (double)a.u[st.first] * total;
-  if (tid == 0) {
-    // The first chunk whose sum up to it exceeds theta; else (rounding, or u from 1 on) the last that has any weight.
-    double sum = 0, at = 0;
-    int chunk = 0;
-    for (int i = 0; i < a.splits; ++i) {
-      if (sums[i] > 0) chunk = i, at = sum;
-      sum += sums[i];
-      if (sums[i] > 0 && sum > theta) break;
-    }
-    found = chunk, before = at;
-  }
-  __syncthreads();
-  const int chunk = found, v0 = chunk * kVerifyChunk;
-  const double rest = theta - before;
-  if (!DRAWN && !whole) rejected_bits(a, st, v0, bits);
-  // Each thread a run of elements.
-  constexpr int RUN = kVerifyChunk / 256;
-  double x[RUN], mine = 0;
-#pragma unroll
-  for (int k = 0; k < RUN; ++k) {
-    const int e = tid * RUN + k, v = v0 + e;
-    double w = v < a.vocab ? weight_of(pr[v]) : 0.0;
-    if (DRAWN) {
-      if (off != 0.0 && v < a.vocab) w = left_of(w, off, weight_of(qr[v]));
-    } else if (!whole) {
-      w = bits[e / 32] >> e % 32 & 1 ? 0.0 : w;
-    }
-    x[k] = w;
-    mine += w;
-  }
-  upto[tid] = mine;
-  if (tid == 0) found = kVerifyChunk, last = -1;
-  __syncthreads();
-  double sum = 0;
-  for (int i = 0; i < tid; ++i) sum += upto[i];
-  int here = kVerifyChunk, latest = -1;
-#pragma unroll
-  for (int k = 0; k < RUN; ++k) {
-    sum += x[k];
-    if (x[k] > 0) {
-      latest = tid * RUN + k;
-      if (sum > rest && here == kVerifyChunk) here = latest;
-    }
-  }
-  if (here < kVerifyChunk) atomicMin(&found, here);
-  if (latest >= 0) atomicMax(&last, latest);
-  __syncthreads();
-  if (tid == 0) a.next[s] = v0 + (found < kVerifyChunk ? found : last);
+  const int64_t token = st.tree == 0 ? -1 : pick_token<DRAWN>(a, st, a.sums + (int64_t)s * a.runs, bits);
+  if (threadIdx.x == 0) a.next[s] = token;
 }
 
 // ---- The accepted tokens' rows ----

@@ -5,6 +5,7 @@
 // halves of the turned part, or (2 p, 2 p + 1), interleaved. Elements behind the turned part pass as they are.
 #pragma once
 
+#include "../paged_model.hpp"
 #include "common.hpp"
 
 namespace pa {
@@ -23,9 +24,14 @@ struct RopeArgs {
   const double* freqs;
   int64_t pos_b, pos_n;
   int64_t tokens;             // b * n
-  int n, d, pairs, pos64, inverse, units;   // units: of a head, each `W` pairs or `W` elements that pass
+  int n, d, pairs, pos64, inverse;
+  int units;                  // of a head: W pairs or up to 2 W elements that pass each; interleaved, W elements (at least 2)
+  int heads, group;           // q's and k's heads, and the tokens that a workgroup takes at a time
+  int heads_outer;            // units follow each other token by token within a head, else head by head within a token
+  PageDiv by_n, by_pairs, by_units, by_inner;   // by_inner: units of a head's tokens, or of a token's heads
   float scale;
 };
+constexpr int kRopeTurns = 1024;   // angles of a group
 
 // cos and sin of n f in fp32. The angle in turns is n f / (2 pi), of which a fraction counts: products and fraction in 64
 // bits with the products' rounding carried along, so that it is right to about 2^-50 of a turn at any 32-bit position (in
@@ -44,46 +50,72 @@ __device__ __forceinline__ float2 rope_turn(double pos, double f, bool inverse, 
   return {cq * scale, (inverse ? -sq : sq) * scale};
 }
 
-// A workgroup takes one token: its angles once, in LDS, for all heads of q and k; then units of W pairs (two loads of W
-// elements), or of W elements that pass, over the threads. A unit is read whole before it is written, by one thread: in
-// and out may be the same rows. W is the widest that sizes, strides and addresses allow.
+// A workgroup takes a few tokens: their angles once, in LDS, for all heads of q and k; then units over the threads, in the
+// order of memory. A unit is read whole before it is written, by one thread: in and out may be the same rows. W is the widest
+// that sizes, strides and addresses allow.
 template <typename T, int W, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rope_rows(RopeArgs a) {
-  typedef T TW __attribute__((ext_vector_type(W)));
-  __shared__ float2 turn[kRopeMaxDim / 2];
-  for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
-    const int64_t b = token / a.n, n = token - b * a.n;
-    const int64_t at = b * a.pos_b + n * a.pos_n;
-    const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[at] : (double)static_cast<const int*>(a.positions)[at];
+  __shared__ float2 turn[kRopeTurns];
+  const int turned = INTERLEAVED && W > 1 ? 2 * a.pairs / W : a.pairs / W, inner = (a.heads_outer ? a.group : a.heads) * a.units;
+  for (int64_t t0 = (int64_t)blockIdx.x * a.group; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.group) {
+    const int here = (int)min((int64_t)a.group, a.tokens - t0);
     __syncthreads();
-    for (int p = (int)threadIdx.x; p < a.pairs; p += 256) turn[p] = rope_turn(pos, a.freqs[p], a.inverse != 0, a.scale);
+    for (int i = (int)threadIdx.x; i < here * a.pairs; i += 256) {
+      const int t = (int)page_of(i, a.by_pairs), token = (int)t0 + t, b = (int)page_of(token, a.by_n);
+      const int64_t at = b * a.pos_b + (token - b * a.n) * a.pos_n;
+      const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.positions)[at] : (double)static_cast<const int*>(a.positions)[at];
+      turn[i] = rope_turn(pos, a.freqs[i - t * a.pairs], a.inverse != 0, a.scale);
+    }
     __syncthreads();
-    const int turned = a.pairs / W, first = a.x[0].heads * a.units, all = first + a.x[1].heads * a.units;
-    for (int i = (int)threadIdx.x; i < all; i += 256) {
-      const RopeRows& x = a.x[i < first ? 0 : 1];
-      const int j = i < first ? i : i - first, h = j / a.units, u = j - h * a.units;
+    const int items = (a.heads_outer ? a.heads : here) * inner;
+    for (int i = (int)threadIdx.x; i < items; i += 256) {
+      const int outer = (int)page_of(i, a.by_inner), rest = i - outer * inner;
+      const int mid = (int)page_of(rest, a.by_units), u = rest - mid * a.units;
+      const int t = a.heads_outer ? mid : outer;
+      int h = a.heads_outer ? outer : mid;
+      if (t >= here) continue;
+      const int token = (int)t0 + t, b = (int)page_of(token, a.by_n), n = token - b * a.n;
+      const RopeRows& x = a.x[h < a.x[0].heads ? 0 : 1];
+      h -= h < a.x[0].heads ? 0 : a.x[0].heads;
       const T* in = static_cast<const T*>(x.in) + b * x.in_b + n * x.in_n + h * x.in_h;
       T* out = static_cast<T*>(x.out) + b * x.out_b + n * x.out_n + h * x.out_h;
-      if (u >= turned) {
-        const int e = 2 * a.pairs + (u - turned) * W;
-        *reinterpret_cast<TW*>(out + e) = *reinterpret_cast<const TW*>(in + e);
-        continue;
-      }
-      const int e0 = INTERLEAVED ? 2 * u * W : u * W, e1 = INTERLEAVED ? e0 + W : e0 + a.pairs;
-      const TW v0 = *reinterpret_cast<const TW*>(in + e0), v1 = *reinterpret_cast<const TW*>(in + e1);
-      TW w0, w1;
+      // Two loads of W elements a lane, each of them side by side over the lanes: the pairs' halves, or halves of what passes;
+      // interleaved: one of W (at least a pair), wherever it lies.
+      constexpr int E = INTERLEAVED && W == 1 ? 2 : W;
+      typedef T TE __attribute__((ext_vector_type(E), aligned(sizeof(T) * W)));
+      if constexpr (INTERLEAVED) {
+        const int e = u * E;
+        if (e + E > a.d) {   // (an odd head's last element)
+          out[e] = in[e];
+          continue;
+        }
+        TE v = *reinterpret_cast<const TE*>(in + e);
+        if (u < turned) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const float2 t = turn[u * W + k];
-        // interleaved: the unit's 2 W elements are x, y, x, y, ...
-        const int xe = INTERLEAVED ? 2 * k : k, ye = INTERLEAVED ? 2 * k + 1 : W + k;
-        const float xv = to_f32(xe < W ? v0[xe % W] : v1[xe % W]), yv = to_f32(ye < W ? v0[ye % W] : v1[ye % W]);
-        const T xo = from_f32<T>(fmaf(xv, t.x, -(yv * t.y))), yo = from_f32<T>(fmaf(xv, t.y, yv * t.x));
-        if (xe < W) w0[xe % W] = xo; else w1[xe % W] = xo;
-        if (ye < W) w0[ye % W] = yo; else w1[ye % W] = yo;
+          for (int k = 0; k < E; k += 2) {
+            const float2 angle = turn[t * a.pairs + (e + k) / 2];
+            const float xv = to_f32(v[k]), yv = to_f32(v[k + 1]);
+            v[k] = from_f32<T>(fmaf(xv, angle.x, -(yv * angle.y))), v[k + 1] = from_f32<T>(fmaf(xv, angle.y, yv * angle.x));
+          }
+        }
+        *reinterpret_cast<TE*>(out + e) = v;
+      } else {
+        const bool turns = u < turned;
+        const int e0 = turns ? u * W : 2 * a.pairs + (u - turned) * W, e1 = e0 + (turns ? a.pairs : (a.units - turned) * W);
+        const bool both = e1 < a.d;
+        TE v0 = *reinterpret_cast<const TE*>(in + e0), v1 = {};
+        if (both) v1 = *reinterpret_cast<const TE*>(in + e1);
+        if (turns) {
+#pragma unroll
+          for (int k = 0; k < W; ++k) {
+            const float2 angle = turn[t * a.pairs + u * W + k];
+            const float xv = to_f32(v0[k]), yv = to_f32(v1[k]);
+            v0[k] = from_f32<T>(fmaf(xv, angle.x, -(yv * angle.y))), v1[k] = from_f32<T>(fmaf(xv, angle.y, yv * angle.x));
+          }
+        }
+        *reinterpret_cast<TE*>(out + e0) = v0;
+        if (both) *reinterpret_cast<TE*>(out + e1) = v1;
       }
-      *reinterpret_cast<TW*>(out + e0) = w0;
-      *reinterpret_cast<TW*>(out + e1) = w1;
     }
   }
 }

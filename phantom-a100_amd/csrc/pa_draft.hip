@@ -15,16 +15,31 @@ using pa::aligned16;
 using pa::fail;
 using pa::hip_status;
 
+// (B, heads, N, d) of 4 x 4096 tokens, 64 heads of 128: with 4096 workgroups or more of four tokens 101 us, with 2048 of
+// eight 122, with one token each 111; packed tokens of 40 heads, 32768 of them, one each 120 us, four 129.
+constexpr int64_t kRopeBlocks = 4096;
 template <typename T, int W>
 hipError_t launch_rope(const pa::RopeArgs& a, bool interleaved, hipStream_t stream) {
-  const unsigned blocks = (unsigned)std::min<int64_t>(a.tokens, 1 << 22);
+  const unsigned blocks = (unsigned)std::min<int64_t>((a.tokens + a.group - 1) / a.group, 1 << 22);
   if (interleaved) hipLaunchKernelGGL((pa::rope_rows<T, W, true>), dim3(blocks), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((pa::rope_rows<T, W, false>), dim3(blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 template <typename T>
 hipError_t launch_rope(pa::RopeArgs a, int width, bool interleaved, hipStream_t stream) {
-  a.units = a.pairs / width + (a.d - 2 * a.pairs) / width;
+  const int wide = interleaved ? std::max(width, 2) : 2 * width;
+  a.units = interleaved ? (a.d + wide - 1) / wide : a.pairs / width + (a.d - 2 * a.pairs + wide - 1) / wide;
+  a.heads = a.x[0].heads + a.x[1].heads;
+  // Tokens of a workgroup at a time: as many as give each thread a unit; where a head's tokens follow each other in memory,
+  // as many as there are threads for their angles, but at least kRopeBlocks workgroups.
+  a.heads_outer = a.x[0].in_h > a.x[0].in_n;
+  const int64_t token_units = (int64_t)a.heads * a.units;
+  const int64_t fill = std::min<int64_t>(256 / token_units, pa::kRopeTurns / a.pairs);
+  const int64_t run = a.heads_outer ? std::min<int64_t>({256 / a.pairs, a.tokens / kRopeBlocks, (1 << 30) / token_units}) : 1;
+  a.group = (int)std::max<int64_t>({fill, run, 1});
+  a.by_n = pa::make_page_div((uint32_t)a.n), a.by_pairs = pa::make_page_div((uint32_t)a.pairs);
+  a.by_units = pa::make_page_div((uint32_t)a.units);
+  a.by_inner = pa::make_page_div((uint32_t)((a.heads_outer ? a.group : a.heads) * a.units));
   switch (width) {
     case 8:
       if constexpr (sizeof(T) == 2) return launch_rope<T, 8>(a, interleaved, stream);
@@ -34,7 +49,12 @@ hipError_t launch_rope(pa::RopeArgs a, int width, bool interleaved, hipStream_t 
   }
 }
 
-int64_t verify_splits(int64_t vocab) { return (vocab + pa::kVerifyChunk - 1) / pa::kVerifyChunk; }
+int64_t verify_runs(int64_t vocab) { return (vocab + pa::kRun - 1) / pa::kRun; }
+// Rows of so many elements go in one workgroup and one launch: up to 32 runs, 64 where drafts were drawn (a third launch
+// saved, of a call that has three). 48 chains of 8 over 32000 and 65537 tokens, in a graph: 9.5 and 13.3 us, in three
+// launches 10.3 and 11.6, and from Python, where a launch costs 2.3 us more, 16 for 21; one chain without, 9.6 and
+// 13.0 for 9.0 and 9.1, from Python 15.5 for 17.8.
+bool verify_in_one(int64_t vocab, bool drawn) { return verify_runs(vocab) <= (drawn ? 64 : 32); }
 int64_t verify_state_bytes(int64_t seqs) { return seqs * (int64_t)sizeof(pa::VerifyState); }
 int check_verify_sizes(const char* name, int64_t seqs, int64_t vocab) {
   if (seqs <= 0 || vocab <= 0) return fail(PA_ERR_INVALID, "%s: inputs must be non-empty", name);
@@ -68,8 +88,8 @@ int pa_rope(const pa_rope_rows* q, const pa_rope_rows* k, int dtype, int64_t b, 
   auto fits = [&](int64_t x, int64_t unit) {
     while (x % (width * unit) != 0) width /= 2;
   };
-  fits(pairs, 1), fits(d, 1);
-  int64_t heads = 0;
+  fits(interleaved ? 2 * pairs : pairs, 1), fits(d, 1);
+
   for (int i = 0; i < 2; ++i) {
     const pa_rope_rows* x = i ? k : q;
     if (!x) continue;
@@ -84,7 +104,7 @@ int pa_rope(const pa_rope_rows* q, const pa_rope_rows* k, int dtype, int64_t b, 
     if (n > 1) fits(x->in_n, 1), fits(x->out_n, 1);
     if (x->heads > 1) fits(x->in_h, 1), fits(x->out_h, 1);
     a.x[i] = pa::RopeRows{x->in, x->out, x->in_b, x->in_n, x->in_h, x->out_b, x->out_n, x->out_h, (int)x->heads};
-    heads += x->heads;
+
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const hipError_t e = dtype == PA_DTYPE_F32   ? launch_rope<float>(a, (int)width, interleaved != 0, st)
@@ -111,9 +131,10 @@ int pa_draft_tree(const int32_t* parents, const int32_t* lengths, const int32_t*
   return hip_status(hipGetLastError(), name);
 }
 
-int64_t pa_verify_draft_workspace(int64_t seqs, int64_t vocab) {
+int64_t pa_verify_draft_workspace(int64_t seqs, int64_t vocab, int drawn) {
   if (int rc = check_verify_sizes("verify_draft", seqs, vocab)) return rc;
-  return verify_state_bytes(seqs) + seqs * verify_splits(vocab) * (int64_t)sizeof(double);
+  if (verify_in_one(vocab, drawn != 0)) return 0;
+  return verify_state_bytes(seqs) + seqs * verify_runs(vocab) * (int64_t)sizeof(double);
 }
 
 int pa_verify_draft(const int64_t* tokens, const int32_t* parents, const float* target_probs, int64_t target_stride,
@@ -129,26 +150,32 @@ int pa_verify_draft(const int64_t* tokens, const int32_t* parents, const float* 
   if (max_new <= 0 || max_new > pa::kTreeMax)
     return fail(PA_ERR_INVALID, "%s: max_new must be a number of tokens from 1 to %d", name, pa::kTreeMax);
   if (target_stride < 0 || draft_stride < 0) return fail(PA_ERR_INVALID, "%s: strides must not be negative", name);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < pa_verify_draft_workspace(seqs, vocab))
+  const bool in_one = verify_in_one(vocab, draft_probs != nullptr);
+  if (!in_one && (!workspace || !aligned16(workspace) || workspace_bytes < pa_verify_draft_workspace(seqs, vocab, draft_probs != nullptr)))
     return fail(PA_ERR_INVALID, "%s: the workspace is too small, null or not 16-byte aligned", name);
-  const int splits = (int)verify_splits(vocab);
+  const int runs = (int)verify_runs(vocab);
   pa::VerifyState* states = static_cast<pa::VerifyState*>(workspace);
   const pa::VerifyArgs a{tokens, parents, target_probs, draft_probs, uniform, cu_seqlens, target_stride, draft_stride,
-                         (int)n_tokens, (int)vocab, (int)max_new, splits, path, accepted, next_tokens, states,
+                         (int)n_tokens, (int)vocab, (int)max_new, runs, path, accepted, next_tokens, states,
                          reinterpret_cast<double*>(static_cast<char*>(workspace) + verify_state_bytes(seqs))};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 chunks((unsigned)splits, (unsigned)seqs), each((unsigned)seqs);
-  const unsigned lds = (unsigned)(splits * sizeof(double));
+  const dim3 four((unsigned)((runs + 3) / 4), (unsigned)seqs), each((unsigned)seqs);
+  if (in_one) {
+    const unsigned lds = (unsigned)(runs * sizeof(double));
+    if (draft_probs) hipLaunchKernelGGL((pa::verify_whole<true>), each, dim3(1024), lds, st, a);
+    else hipLaunchKernelGGL((pa::verify_whole<false>), each, dim3(1024), lds, st, a);
+    return hip_status(hipGetLastError(), name);
+  }
   if (draft_probs) {
     hipLaunchKernelGGL(pa::verify_drawn, each, dim3(1024), 0, st, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return hip_status(e, name);
-    hipLaunchKernelGGL((pa::verify_sums<true>), chunks, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((pa::verify_sums<true>), four, dim3(256), 0, st, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return hip_status(e, name);
-    hipLaunchKernelGGL((pa::verify_pick<true>), each, dim3(256), lds, st, a);
+    hipLaunchKernelGGL((pa::verify_pick<true>), each, dim3(pa::kWave), 0, st, a);
   } else {
-    hipLaunchKernelGGL((pa::verify_sums<false>), chunks, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((pa::verify_sums<false>), four, dim3(256), 0, st, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return hip_status(e, name);
-    hipLaunchKernelGGL((pa::verify_pick<false>), each, dim3(256), lds, st, a);
+    hipLaunchKernelGGL((pa::verify_pick<false>), each, dim3(pa::kWave), 0, st, a);
   }
   return hip_status(hipGetLastError(), name);
 }

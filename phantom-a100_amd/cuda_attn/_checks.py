@@ -393,6 +393,23 @@ def _tokens_apart(q, k, token: int) -> bool:
     return at >= wide[0] and at + wide[1] <= step
 
 
+def rope_ok(q, k, positions, freqs) -> bool:
+    """Whether a call into new tensors passes check_rope, each property read once: a small call is bound by this host path.
+    Anything that this does not accept goes through that check for its message."""
+    shape, dtype, device, at = q.shape, q.dtype, q.device, positions.shape
+    axes = len(shape)
+    if not ((axes == 3 and at == shape[:1] or axes == 4 and at in ((shape[2],), (shape[0], shape[2]))) and q.is_cuda
+            and dtype in ROPE_DTYPES and 0 not in shape and shape[-1] <= ROPE_MAX_DIM and q.stride(-1) == 1
+            and positions.dtype in (torch.int32, torch.int64) and positions.device == device and freqs.device == device
+            and freqs.dtype is torch.float64 and freqs.dim() == 1 and freqs.is_contiguous() and 1 <= freqs.shape[0] <= shape[-1] // 2):
+        return False
+    if k is None:
+        return True
+    other = k.shape
+    return (k.dtype is dtype and k.device == device and len(other) == axes and 0 not in other and other[0] == shape[0]
+            and other[2:] == shape[2:] and k.stride(-1) == 1)
+
+
 def check_rope(name: str, q, k, positions, freqs, inplace: bool, *, require_cuda: bool = True) -> None:
     device, dtype, shape = q.device, q.dtype, q.shape
     for t in (q, k, positions, freqs):

@@ -30,13 +30,12 @@ class PagedCacheArgs(ctypes.Structure):
 
 
 class RopeRows(ctypes.Structure):
-    """pa_rope_rows."""
+    """pa_rope_rows; passed by its address, or as its bytes."""
     _fields_ = [("in_", _p), ("out", _p), ("in_b", _i64), ("in_n", _i64), ("in_h", _i64), ("out_b", _i64),
                 ("out_n", _i64), ("out_h", _i64), ("heads", _i64)]
 
 
 _cache = ctypes.POINTER(PagedCacheArgs)
-_rope = ctypes.POINTER(RopeRows)
 
 
 # name -> (restype, argtypes); must list every function the header declares.
@@ -58,9 +57,9 @@ PROTOTYPES = {
     "pa_paged_attn_workspace": (_i64, [_cache, _i, _i64, _i64, _p, _i64]),
     "pa_draft_tree": (_i, [_p, _p, _p, _i64, _i64, _i64, _p, _p, _p]),
     "pa_paged_tree_attn_fwd": (_i, [_cache, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _p]),
-    "pa_rope": (_i, [_rope, _rope, _i, _i64, _i64, _i64, _p, _i, _i64, _i64, _p, _i64, _i, _i, ctypes.c_float, _p]),
+    "pa_rope": (_i, [_p, _p, _i, _i64, _i64, _i64, _p, _i, _i64, _i64, _p, _i64, _i, _i, ctypes.c_float, _p]),
     "pa_verify_draft": (_i, [_p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
-    "pa_verify_draft_workspace": (_i64, [_i64, _i64]),
+    "pa_verify_draft_workspace": (_i64, [_i64, _i64, _i]),
     "pa_cache_keep": (_i, [_cache, _p, _i64, _i64, _p, _p, _p, _p]),
     "pa_last_error": (ctypes.c_char_p, []),
     "pa_version": (ctypes.c_char_p, []),

@@ -123,14 +123,15 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target_probs: torc
     path = torch.empty((seqs, most), dtype=torch.int32, device=device)
     accepted = torch.empty(seqs, dtype=torch.int32, device=device)
     drawn = torch.empty(seqs, dtype=torch.int64, device=device)
-    need = _native.lib().pa_verify_draft_workspace(seqs, vocab)
+    need = _native.lib().pa_verify_draft_workspace(seqs, vocab, 0 if draft_probs is None else 1)
     if need < 0:
         _native.check(need, name)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call("pa_verify_draft", name, device, tokens.data_ptr(), parents.data_ptr(), target_probs.data_ptr(),
           target_probs.stride(0), None if draft_probs is None else draft_probs.data_ptr(),
           0 if draft_probs is None else draft_probs.stride(0), uniform.data_ptr(), cu_seqlens.data_ptr(), n, seqs, vocab,
-          most, path.data_ptr(), accepted.data_ptr(), drawn.data_ptr(), workspace.data_ptr(), need, _stream_ptr(device))
+          most, path.data_ptr(), accepted.data_ptr(), drawn.data_ptr(), None if workspace is None else workspace.data_ptr(),
+          need, _stream_ptr(device))
     return path, accepted, drawn
 
 

@@ -6,6 +6,7 @@
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 
@@ -67,24 +68,32 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs
     turn in 32."""
     from . import _call, _stream_ptr
 
-    _checks.check_rope("rope", q, k, positions, freqs, inplace)
-    dense = q.dim() == 4
-    b, n = (q.shape[0], q.shape[2]) if dense else (1, q.shape[0])
-    outs, rows = [], []
-    for x in (q, k):
-        if x is None:
-            outs.append(None)
-            rows.append(None)
-            continue
-        y = x if inplace else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        xs, ys = x.stride(), y.stride()
-        at = (0, 2, 1) if dense else (None, 0, 1)
-        strides = [0 if i is None else s[i] for s in (xs, ys) for i in at]
-        rows.append(_native.RopeRows(x.data_ptr(), y.data_ptr(), *strides, x.shape[1]))
-        outs.append(y)
+    if inplace or not _checks.rope_ok(q, k, positions, freqs):
+        _checks.check_rope("rope", q, k, positions, freqs, inplace)
+    shape, device = q.shape, q.device
+    dense = len(shape) == 4
+    q_out, rows = _rows(q, dense, inplace)
+    k_out, k_rows = (None, None) if k is None else _rows(k, dense, inplace)
     ps = positions.stride()
-    pb, pn = (ps[0], ps[1]) if positions.dim() == 2 else (0, ps[0])
-    _call("pa_rope", "rope", q.device, rows[0], rows[1], _DTYPE_CODE[q.dtype], b, n, q.shape[-1], positions.data_ptr(),
+    pb, pn = ps if len(ps) == 2 else (0, ps[0])
+    b, n = (shape[0], shape[2]) if dense else (1, shape[0])
+    _call("pa_rope", "rope", device, rows, k_rows, _DTYPE_CODE[q.dtype], b, n, shape[-1], positions.data_ptr(),
           1 if positions.dtype is torch.int64 else 0, pb, pn, freqs.data_ptr(), freqs.shape[0], 1 if interleaved else 0,
-          1 if inverse else 0, scale, _stream_ptr(q.device))
-    return outs[0], outs[1]
+          1 if inverse else 0, scale, _stream_ptr(device))
+    return q_out, k_out
+
+
+_pack = struct.Struct("PP7q").pack   # pa_rope_rows
+
+
+def _rows(x, dense, inplace):
+    """Where x's rows go, and the rows as the library takes them."""
+    shape = x.shape
+    y = x if inplace else torch.empty(shape, dtype=x.dtype, device=x.device)
+    if dense:
+        xb, xh, xn, _ = x.stride()
+        yb, yh, yn, _ = y.stride()
+        return y, _pack(x.data_ptr(), y.data_ptr(), xb, xn, xh, yb, yn, yh, shape[1])
+    xn, xh, _ = x.stride()
+    yn, yh, _ = y.stride()
+    return y, _pack(x.data_ptr(), y.data_ptr(), 0, xn, xh, 0, yn, yh, shape[1])

@@ -171,7 +171,7 @@ def test_c_entries_refuse_trees_and_verification():
                           ({"seqs": 0}, -1, "non-empty"), ({"tokens": 2 ** 31}, -2, "2^30"), ({"seqs": 2 ** 23}, -2, "2^22"),
                           ({"most": 0}, -1, "max_new"), ({"most": 1025}, -1, "max_new"), ({"tokens": 7, "cu": None}, -1, "divide evenly")):
         refused(tree(**kw), rc, match)
-    verify = lambda tokens=P, p=P, u=P, cu=P, n=6, seqs=3, vocab=100, most=4, path=P, ws=P, room=2 ** 40, ps=100, qs=0: \
+    verify = lambda tokens=P, p=P, u=P, cu=P, n=6, seqs=3, vocab=100000, most=4, path=P, ws=P, room=2 ** 40, ps=100000, qs=0: \
         lib.pa_verify_draft(tokens, P, p, ps, None, qs, u, cu, n, seqs, vocab, most, path, P, P, ws, room, None)  # noqa: E731
     for kw, rc, match in (({"tokens": None}, -1, "null"), ({"p": None}, -1, "null"), ({"u": None}, -1, "null"), ({"cu": None}, -1, "null"),
                           ({"path": None}, -1, "null"), ({"n": 0}, -1, "non-empty"), ({"vocab": 0}, -1, "non-empty"),
@@ -179,8 +179,8 @@ def test_c_entries_refuse_trees_and_verification():
                           ({"ps": -1}, -1, "strides"), ({"qs": -1}, -1, "strides"), ({"ws": None}, -1, "workspace"), ({"ws": ODD}, -1, "workspace"),
                           ({"room": 8}, -1, "workspace"), ({"n": 2 ** 31}, -2, "2^30")):
         refused(verify(**kw), rc, match)
-    assert lib.pa_verify_draft_workspace(3, 100) > 0
-    assert lib.pa_verify_draft_workspace(0, 100) == -1 and lib.pa_verify_draft_workspace(3, 2 ** 25) == -2
+    assert lib.pa_verify_draft_workspace(3, 100, 1) == 0 and lib.pa_verify_draft_workspace(3, 100000, 0) > 0
+    assert lib.pa_verify_draft_workspace(0, 100, 0) == -1 and lib.pa_verify_draft_workspace(3, 2 ** 25, 0) == -2
 
 
 def native_cache(**change):
@@ -210,8 +210,9 @@ def test_c_entries_refuse_rope():
     lib, f16 = _native.lib(), _native.DTYPE_F16
     rows = lambda **kw: _native.RopeRows(*(kw.get(n, v) for n, v in zip(  # noqa: E731
         ("i", "o", "ib", "inn", "ih", "ob", "on", "oh", "heads"), (256, 256, 0, 256, 64, 0, 256, 64, 4))))
+    ref = lambda x: None if x is None else ctypes.byref(x)  # noqa: E731
     rope = lambda q=rows(), k=None, dt=f16, b=1, n=6, d=64, pos=P, f=P, pairs=32: \
-        lib.pa_rope(q, k, dt, b, n, d, pos, 0, 0, 1, f, pairs, 0, 0, 1.0, None)  # noqa: E731
+        lib.pa_rope(ref(q), ref(k), dt, b, n, d, pos, 0, 0, 1, f, pairs, 0, 0, 1.0, None)  # noqa: E731
     for kw, rc, match in (({"q": None}, -1, "null"), ({"pos": None}, -1, "null"), ({"f": None}, -1, "null"), ({"q": rows(i=None)}, -1, "null"),
                           ({"k": rows(o=None)}, -1, "null"), ({"dt": _native.DTYPE_I8}, -2, "float32"), ({"n": 0}, -1, "non-empty"),
                           ({"pairs": 0}, -1, "non-empty"), ({"d": 2048}, -2, "1024"), ({"pairs": 33}, -1, "more pairs"), ({"b": 2 ** 20, "n": 2 ** 20}, -2, "2^30"),
