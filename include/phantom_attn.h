@@ -216,11 +216,13 @@ int pa_draft_tree(const int32_t* parents, const int32_t* lengths, const int32_t*
 
 /* pa_paged_attn_fwd with a mask in the place of `causal`: a new token sees the positions before its sequence's new tokens,
  * and the new token j whose bit j % 32 of word j / 32 is set in its row mask + i * mask_stride (mask_words words, those past
- * them 0; any bits, not only a tree's). Workspace: pa_paged_attn_workspace(). */
+ * them 0; any bits, not only a tree's). Workspace: pa_paged_tree_attn_workspace() bytes, otherwise as there. */
 int pa_paged_tree_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int dtype, int64_t tokens, int64_t heads_q,
                            int64_t q_token_stride, int64_t q_head_stride, int64_t o_token_stride, int64_t o_head_stride,
                            const int32_t* cu_seqlens, int64_t max_new, const int32_t* mask, int64_t mask_words,
                            int64_t mask_stride, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t pa_paged_tree_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
+                                     const int32_t* cu_seqlens, int64_t max_new);
 
 /* Rows to turn: [b][n][heads][d] with the strides given, in elements; the d elements of a row contiguous. out may be in,
  * with its strides; otherwise they share no memory. */

@@ -639,14 +639,16 @@ paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
 // workgroups on a CU as the registers allow, three in 16 bits (4 x 2048 tokens f16 88 us, with two 100), two in 8
 // (with three 24 x 700 over 4096 in int8 takes 493 for 480).
 constexpr int chunk_rows_of(int d) { return d == 128 ? 256 : 128; }
-constexpr int chunk_wgs(int d, bool k8) { return d == 128 ? 1 : k8 ? 2 : 3; }   // workgroups on a CU
+constexpr int chunk_wgs(int d, bool k8, int rows, bool tree) {   // workgroups on a CU
+  return d == 128 ? 1 : !tree ? (k8 ? 2 : 3) : rows == 64 ? 4 : 2;
+}
 
 // WIDE: caches (or their scales) past a buffer's 32-bit offsets. 16-bit rows then come from 64-bit addresses by
 // instructions of the flat kind, after which the compiler waits for all LDS reads instead of the oldest; 8-bit ones
 // are not pipelined at all. The case above takes 2108 us (in buffers 1976), in int8 3129 (2312), with D = 64 2659 (1756).
 constexpr uint32_t kPastBuffer = 0xffffe000u;
 template <typename T, typename C, int D, int BM, bool WIDE, bool TREE = false>
-__global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chunk_wgs(D, cache_type<C>::k8bit) * BM / 128)))
+__global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chunk_wgs(D, cache_type<C>::k8bit, BM, TREE) * BM >= 256 ? chunk_wgs(D, cache_type<C>::k8bit, BM, TREE) * BM / 128 : 1)))
 paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;
@@ -755,14 +757,15 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
       const bool there = (key < key_end) & ((unsigned)page < (unsigned)c.pages);
       return there ? (int)at : -1;
     };
-    // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row (loads
-    // are 32 rows apart, so the swizzle is the same).
-    static_assert(k8 || THREADS / LPR == 32, "loads 32 rows apart");
+    // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row (of loads 8 rows
+    // apart K's swizzle alternates in its highest bit; V's is the same, and both are for loads farther apart).
+    constexpr int APART = THREADS / LPR;   // rows between a thread's loads
+    static_assert(k8 || APART % 16 == 0 || (APART == 8 && CR == 16), "loads whose swizzles are alike, or alternate in one bit");
     const int k_off = (tid % LPR ^ k_swz<CR>(tid / LPR)) * 16, v_off = (tid % LPR ^ v_swz<CR>(tid / LPR)) * 16;
     auto to_lds = [&](const void* cache, rsrc_t rs, const int (&rows)[CPT], unsigned char* stage, bool is_v) {
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
-        unsigned off = is_v ? v_off : k_off;
+        unsigned off = is_v ? v_off : APART == 8 && i % 2 ? k_off ^ 128 : k_off;
         asm("" : "+v"(off));   // (not to be added to the base once for all loads: that spills)
         unsigned char* to = stage + (i * THREADS + wave * kWave) * 16;
         if constexpr (WIDE) {
@@ -774,25 +777,33 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
       }
     };
     // 8-bit rows: through registers, or into the thread's 16 bytes of a raw buffer; then widened and stored.
-    static_assert(!k8 || CPT == 1, "one load of 8-bit rows a thread");
     auto to_regs = [&](const void* cache, rsrc_t rs, const int (&rows)[CPT], u32x4 (&x)[CPT]) {
-      if constexpr (WIDE) x[0] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(cache) + (uint64_t)(unsigned)rows[0] * CB + tid % LPR * 16);
-      else x[0] = load16(rs, (unsigned)rows[0] + tid % LPR * 16);
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        if constexpr (WIDE) x[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(cache) + (uint64_t)(unsigned)rows[i] * CB + tid % LPR * 16);
+        else x[i] = load16(rs, (unsigned)rows[i] + tid % LPR * 16);
+      }
     };
     auto to_raw = [&](rsrc_t rs, const int (&rows)[CPT], unsigned char* raw) {
-      load16_to_lds(rs, raw + wave * kWave * 16, (unsigned)rows[0] + tid % LPR * 16, 0);
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) load16_to_lds(rs, raw + (i * THREADS + wave * kWave) * 16, (unsigned)rows[i] + tid % LPR * 16, 0);
     };
-    auto from_raw = [&](const unsigned char* raw, u32x4 (&x)[CPT]) { x[0] = *reinterpret_cast<const u32x4*>(raw + tid * 16); };
+    auto from_raw = [&](const unsigned char* raw, u32x4 (&x)[CPT]) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) x[i] = *reinterpret_cast<const u32x4*>(raw + (i * THREADS + tid) * 16);
+    };
     auto widen = [&](const u32x4 (&x)[CPT], unsigned char* stage, bool is_v) {
-      if constexpr (k8) {
-        int at = tid;
-        asm("" : "+v"(at));   // (addresses made each time, not held)
-        const int r = at / LPR, ch = (at % LPR * 2) ^ (is_v ? v_swz<CR>(r) : k_swz<CR>(r));
-        u32x4 lo16, hi16;
-        widen16<C, T>(x[0], lo16, hi16);
-        *reinterpret_cast<u32x4*>(stage + r * RB + ch * 16) = lo16;
-        *reinterpret_cast<u32x4*>(stage + r * RB + (ch ^ 1) * 16) = hi16;
-      }
+      if constexpr (k8)
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          int at = tid;
+          asm("" : "+v"(at));   // (addresses made each time, not held)
+          const int r = i * APART + at / LPR, ch = (at % LPR * 2) ^ (is_v ? v_swz<CR>(r) : k_swz<CR>(r));
+          u32x4 lo16, hi16;
+          widen16<C, T>(x[i], lo16, hi16);
+          *reinterpret_cast<u32x4*>(stage + r * RB + ch * 16) = lo16;
+          *reinterpret_cast<u32x4*>(stage + r * RB + (ch ^ 1) * 16) = hi16;
+        }
     };
     auto present_of = [&](int row) -> uint64_t { return __builtin_amdgcn_ballot_w64(row >= 0); };
     // The row that each of the thread's loads reads; where loads are from a buffer, its byte offset, past the
@@ -1096,7 +1107,42 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
       };
       f32x16 sa[NKB], sb[NKB];
       V8 pa[PV_STEPS], pb[PV_STEPS];
-      if (fits(0, present[0])) {
+      // A wave without rows (of a sequence with fewer new tokens than the tile has room for) moves the keys, in step with the
+      // others, and leaves its SIMD's time to them.
+      const bool idle = TREE && wave_any == 0;
+      if (idle && fits(0, present[0])) {
+        __syncthreads();
+#pragma unroll 1
+        do {
+          const int P = t0 & 1;
+          unsigned char* const k_cur = P ? k_lds1 : k_lds0;
+          unsigned char* const v_nxt = P ? v_lds0 : v_lds1;
+          if constexpr (k8) {
+            to_raw(v_rs, rows[1], P ? v_raw1 : v_raw0);
+            to_raw(k_rs, rows[2], P ? k_raw0 : k_raw1);
+            scales_to_lds(t0 + 2, row[1]);
+          } else {
+            to_lds(c.v, v_rs, rows[0], v_nxt, true);
+            to_lds(c.k, k_rs, rows[1], k_cur, false);
+          }
+          const int row_new = find_row(t0 + 1 + AHEAD, page, in_page);
+          const uint64_t present_new = present_of(row_new);
+          page = load_page(t0 + 2 + AHEAD, in_page);
+          advance(row_new, present_new);
+          chunk_rows(row_new, present_new, rows[AHEAD - 1]);
+          if constexpr (k8) {
+            u32x4 x[CPT];
+            from_raw(P ? k_raw1 : k_raw0, x);
+            widen(x, k_cur, false);
+            from_raw(P ? v_raw0 : v_raw1, x);
+            widen(x, v_nxt, true);
+          }
+          __builtin_amdgcn_s_waitcnt(0);
+          if (t0 + 1 < nt && !whole_tile(t0 + 1, present[0])) check_values(t0 + 1, v_nxt);
+          __syncthreads();
+        } while (fits(++t0, present[0]));
+      }
+      if (!idle && fits(0, present[0])) {
         qk(sa, k_stage(even));
         scale_scores(sa, 0);
         raise(row_max(sa, is_clean(0, present[0]) ? kLowest : mask(sa, 0, present[0])));

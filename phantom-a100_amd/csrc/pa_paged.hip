@@ -14,7 +14,6 @@ using pa::check_strides;
 using pa::check_tokens;
 using pa::fail;
 using pa::hip_status;
-using pa::is_8bit;
 using pa::with_types;
 
 }  // namespace
@@ -79,15 +78,7 @@ int pa_paged_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, int d
 
 int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
                                 const int32_t* cu_seqlens, int64_t max_new) {
-  const char* name = "paged_attn";
-  pa::PagedCache c;
-  if (int rc = check_cache(name, cache, dtype, &c)) return rc;
-  if (int rc = check_tokens(name, tokens, cu_seqlens, &c)) return rc;
-  if (heads_q <= 0 || heads_q > (1 << 16) || heads_q % cache->heads != 0 || max_new < 0)
-    return fail(PA_ERR_INVALID, "%s: the query heads must be a multiple of the cache's heads, max_new not negative", name);
-  const pa::AttnPlan plan = pa::attn_plan(c, cache->d, is_8bit(cache->dtype), heads_q, max_new);
-  if (int rc = pa::check_work(name, c, plan, heads_q)) return rc;
-  return pa::attn_workspace(plan.wgs, plan.rows, (int)cache->d);
+  return pa::attn_workspace_of("paged_attn", cache, dtype, tokens, heads_q, cu_seqlens, max_new, false);
 }
 
 }  // extern "C"

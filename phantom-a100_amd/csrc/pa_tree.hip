@@ -23,4 +23,9 @@ int pa_paged_tree_attn_fwd(const pa_paged_cache* cache, const void* q, void* o, 
                              dtype, tokens, heads_q, cu_seqlens, max_new, w, workspace, workspace_bytes, stream);
 }
 
+int64_t pa_paged_tree_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
+                                     const int32_t* cu_seqlens, int64_t max_new) {
+  return pa::attn_workspace_of("paged_tree_attn", cache, dtype, tokens, heads_q, cu_seqlens, max_new, true);
+}
+
 }  // extern "C"

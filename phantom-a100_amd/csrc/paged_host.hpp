@@ -79,16 +79,59 @@ hipError_t with_types(int dtype, int cache_dtype, int64_t d, F f) {
 
 constexpr int kCUs = 256;   // MI355X / gfx950. (A constant: a workspace's size is asked for without a GPU.)
 
+// Whether a cache, or its scales, reach past the 32-bit offsets of a buffer.
+inline bool past_buffer(const PagedCache& c, int64_t d, bool k8) {
+  return (uint64_t)c.pages * c.heads * c.page_size * std::max<uint64_t>(d * (k8 ? 1 : 2), 4) > kPastBuffer;
+}
+
+// Rows of a tile for trees of more than 32 rows a key/value head: the tile whose time is the least by a start and a rate,
+// a us and f times the time that reading the keys and values once takes, for each tile that goes over them. (The table's
+// capacity stands for the lengths, which the host does not know.) Measured, D = 128, 32 heads over 8, us:
+//                                              32      64     128     256 rows
+//   bf16  s 32, 16 tokens over 8192 (1 GB)     371     203    206
+//         32 tokens                                    254    220
+//         64 tokens                                    510    317     316
+//         s 4, 64 tokens over 4000 (66 MB)      86      67     50      55
+//         over 1000 (16 MB)                     34      32     35      40
+//         s 4, 16 tokens over 1000              22      25     29
+//   e4m3  s 32, 16 tokens over 8192            285     297    265
+//         64 tokens                                   1165    530     344
+//         s 16, 40 tokens over 1000             77      95     50      51
+//         s 4, 16 tokens over 1000              31      46     35
+// 64 dims, 16 heads over 4: f16, 24 x 24 over 4096 54 with 32 rows, 128 44; e4m3 16 x 40 over 1000 32, 128 39.
+struct TileTime {
+  int rows;
+  double a, f;
+};
+inline int tree_rows(const PagedCache& c, int64_t d, bool k8, int64_t most) {
+  static const TileTime kTimes[4][4] = {{{32, 14, 0.9}, {64, 18, 0.95}, {128, 20, 1.02}, {256, 34, 1.45}},     // D = 128
+                                        {{32, 17, 1.6}, {128, 28, 2.5}, {256, 34, 3.2}, {0, 0, 0}},            // in 8 bits
+                                        {{32, 12, 1.0}, {64, 22, 1.0}, {128, 29, 0.75}, {0, 0, 0}},            // D = 64
+                                        {{32, 18, 1.3}, {128, 26, 2.6}, {0, 0, 0}, {0, 0, 0}}};
+  const double once = 2.0 * c.seqs * c.heads * (double)c.capacity * d * (k8 ? 1 : 2) / 5e6;   // us at 5 TB/s
+  int rows = 0;
+  double least = 0;
+  for (const TileTime& t : kTimes[(d == 64 ? 2 : 0) + (k8 ? 1 : 0)]) {
+    if (t.rows == 0) break;
+    const double us = t.a + t.f * once * (double)((most + t.rows - 1) / t.rows);
+    if (rows == 0 || us < least) rows = t.rows, least = us;
+  }
+  return rows;
+}
+// Least units of a workgroup with larger tiles, whose parts cost as much to write and join as that many keys: 4 x 64
+// tokens over 4000, 256 rows, at least 128 units 65 us, 1024 55; 24 x 24 over 2048, 64 dims, 128 rows, 37 and (512) 34.
+inline int tree_units(int rows) { return 4 * rows; }
+
 // The launch of an attention call: rows of a tile, workgroups, and whether tiles are cut.
 struct AttnPlan {
-  int rows, wgs;
+  int rows, wgs, min_units;
   bool whole;
 };
 // A cache of at most so many positions a sequence is read in a few steps: its tiles are not cut over workgroups,
 // which saves the second launch that joins them. One to 32 tokens over 200 keys: a call takes 17 to 18 us, cut 22;
 // 2 x 100 tokens over 900 take 27 us cut and 47 whole.
 constexpr int kWholeCapacity = 256;
-inline AttnPlan attn_plan(const PagedCache& c, int64_t d, bool k8, int64_t heads_q, int64_t max_new) {
+inline AttnPlan attn_plan(const PagedCache& c, int64_t d, bool k8, int64_t heads_q, int64_t max_new, bool tree) {
   const int64_t group = heads_q / c.heads;
   const int64_t new_tokens = !c.cu ? c.per_seq : max_new > 0 ? std::min<int64_t>(max_new, c.tokens) : c.tokens;
   const int64_t most = new_tokens * group;   // rows of a sequence and key/value head
@@ -96,14 +139,16 @@ inline AttnPlan attn_plan(const PagedCache& c, int64_t d, bool k8, int64_t heads
   // over 8192 keys as two tiles of 32 and as a chunk: 16 bits 325 and 322 us, 8 bits 228 and 378 (64 dims, 16 bits:
   // 156 and 137); 128 x 16 of 64 dims over 1000 in 8 bits 46 and 55. 17 to 32 rows as two
   // tiles of 16: 272 for 226. Tiles of 64 were between the two (315, 314), and slower at 128 rows than chunks (434, 308).
-  const int rows = most <= 16 ? 16 : most <= 64 ? 32 : chunk_rows_of((int)d);
+  const int rows = tree && most > 32 && !past_buffer(c, d, k8) ? tree_rows(c, d, k8, most)
+                   : most <= 16 ? 16 : most <= 64 ? 32 : chunk_rows_of((int)d);
   // As many workgroups as are resident at once, or fewer where the work's bound is below their least share.
   const TileShape t = make_tiles((int)group, rows);
   const double tiles = (double)c.tokens / t.tokens + c.seqs;
   const double units = tiles * c.heads * t.splits * ((double)kTileCost + c.capacity);
-  const int resident = kCUs * (rows > 64 ? chunk_wgs((int)d, k8) : few_wgs((int)d, k8, rows / 16));
-  const int wgs = (int)std::max(1.0, std::min<double>(resident, units / kMinUnits + 1));
-  return {rows, wgs, c.capacity <= kWholeCapacity};
+  const int resident = kCUs * (rows > 32 ? chunk_wgs((int)d, k8, rows, tree) : few_wgs((int)d, k8, rows / 16));
+  const int least = tree && rows > 32 ? tree_units(rows) : kMinUnits;
+  const int wgs = (int)std::max(1.0, std::min<double>(resident, units / least + 1));
+  return {rows, wgs, least, c.capacity <= kWholeCapacity};
 }
 // The kernels count a call's work in 63 bits: each sequence could have all tokens (offsets out of order), each token
 // the longest keys.
@@ -119,7 +164,7 @@ template <typename T, int D, int ROWS, typename Kernel, typename Work>
 hipError_t launch_attn(Kernel kernel, int threads, const PagedCache& c, const RowsQ& a, const AttnPlan& plan, Work w,
                        void* workspace, hipStream_t stream) {
   w.tiles = make_tiles(a.group, ROWS);
-  w.min_units = kMinUnits;
+  w.min_units = plan.min_units;
   w.whole = plan.whole;
   w.scale_log2 = kLog2e / sqrtf((float)D);
   w.records = static_cast<PartRecord*>(workspace);
@@ -150,7 +195,7 @@ int attn_call(const char* name, const pa_paged_cache* cache, RowsQ a, int dtype,
   if (!apart(a.o_token, tokens, a.o_head, heads_q) && !apart(a.o_head, heads_q, a.o_token, tokens))
     return fail(PA_ERR_INVALID, "%s: out's rows must not overlap", name);
   if (max_new < 0) return fail(PA_ERR_INVALID, "%s: max_new must not be negative", name);
-  const AttnPlan plan = attn_plan(c, cache->d, is_8bit(cache->dtype), heads_q, max_new);
+  const AttnPlan plan = attn_plan(c, cache->d, is_8bit(cache->dtype), heads_q, max_new, TREE);
   if (int rc = check_work(name, c, plan, heads_q)) return rc;
   if (workspace_bytes < attn_workspace(plan.wgs, plan.rows, (int)cache->d) || !workspace || !aligned16(workspace))
     return fail(PA_ERR_INVALID, "%s: the workspace is too small, null or not 16-byte aligned", name);
@@ -166,12 +211,30 @@ int attn_call(const char* name, const pa_paged_cache* cache, RowsQ a, int dtype,
       case 32: return launch_attn<T, D, 32>(paged_attn_few<T, C, D, 2, TREE>, 256, c, a, plan, w, workspace, st);
       default: break;
     }
-    const uint64_t cache_rows = (uint64_t)c.pages * c.heads * c.page_size;
-    if (cache_rows * std::max<size_t>(D * sizeof(C), 4) > kPastBuffer)
+    if (past_buffer(c, D, cache_type<C>::k8bit))
       return launch_attn<T, D, CR>(paged_attn_chunk<T, C, D, CR, true, TREE>, 2 * CR, c, a, plan, w, workspace, st);
+    if constexpr (TREE) {
+      if constexpr (!cache_type<C>::k8bit)
+        if (plan.rows == 64) return launch_attn<T, D, 64>(paged_attn_chunk<T, C, D, 64, false, TREE>, 128, c, a, plan, w, workspace, st);
+      if constexpr (CR != 128)
+        if (plan.rows == 128) return launch_attn<T, D, 128>(paged_attn_chunk<T, C, D, 128, false, TREE>, 256, c, a, plan, w, workspace, st);
+    }
     return launch_attn<T, D, CR>(paged_attn_chunk<T, C, D, CR, false, TREE>, 2 * CR, c, a, plan, w, workspace, st);
   });
   return hip_status(e, name);
+}
+
+// Bytes of workspace of an attention call.
+inline int64_t attn_workspace_of(const char* name, const pa_paged_cache* cache, int dtype, int64_t tokens, int64_t heads_q,
+                                 const int32_t* cu_seqlens, int64_t max_new, bool tree) {
+  PagedCache c;
+  if (int rc = check_cache(name, cache, dtype, &c)) return rc;
+  if (int rc = check_tokens(name, tokens, cu_seqlens, &c)) return rc;
+  if (heads_q <= 0 || heads_q > (1 << 16) || heads_q % cache->heads != 0 || max_new < 0)
+    return fail(PA_ERR_INVALID, "%s: the query heads must be a multiple of the cache's heads, max_new not negative", name);
+  const AttnPlan plan = attn_plan(c, cache->d, is_8bit(cache->dtype), heads_q, max_new, tree);
+  if (int rc = check_work(name, c, plan, heads_q)) return rc;
+  return attn_workspace(plan.wgs, plan.rows, (int)cache->d);
 }
 
 }  // namespace pa

@@ -57,6 +57,7 @@ PROTOTYPES = {
     "pa_paged_attn_workspace": (_i64, [_cache, _i, _i64, _i64, _p, _i64]),
     "pa_draft_tree": (_i, [_p, _p, _p, _i64, _i64, _i64, _p, _p, _p]),
     "pa_paged_tree_attn_fwd": (_i, [_cache, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _p]),
+    "pa_paged_tree_attn_workspace": (_i64, [_cache, _i, _i64, _i64, _p, _i64]),
     "pa_rope": (_i, [_p, _p, _i, _i64, _i64, _i64, _p, _i, _i64, _i64, _p, _i64, _i, _i, ctypes.c_float, _p]),
     "pa_verify_draft": (_i, [_p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
     "pa_verify_draft_workspace": (_i64, [_i64, _i64, _i]),

@@ -75,7 +75,7 @@ def paged_tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     tokens, heads_q, _ = q.shape
     code = _DTYPE_CODE[q.dtype]
     cu = None if cu_seqlens is None else cu_seqlens.data_ptr()
-    need = _native.lib().pa_paged_attn_workspace(cache, code, tokens, heads_q, cu, bound)
+    need = _native.lib().pa_paged_tree_attn_workspace(cache, code, tokens, heads_q, cu, bound)
     if need < 0:
         _native.check(need, name)
     workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
