@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _checks, _native
+from . import _call, _checks, _native, _stream_ptr
 from .paged import _DTYPE_CODE, _cache_args, _check
 
 TREE_MAX = 1024
@@ -35,8 +35,6 @@ def draft_tree(parents: torch.Tensor, lengths: torch.Tensor, cu_seqlens: torch.T
     first new token is, plus the token's depth. lengths (B,) int32 counts the new tokens. max_new: the most new tokens of
     a sequence (default: tokens / B without cu_seqlens, else all tokens, up to 1024). Rows behind the last sequence's
     are not set."""
-    from . import _call, _stream_ptr
-
     most = _checks.check_tree("draft_tree", parents, lengths.shape[0] if lengths.dim() == 1 else 0, cu_seqlens, max_new)
     _checks.check_vector("draft_tree", "lengths", lengths, torch.int32, None, parents.device)
     tokens = parents.shape[0]
@@ -59,8 +57,6 @@ def paged_tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     0. Masks need not be a tree's: what a row sees is what its bits say, itself included. All else is paged_attn's:
     scores scaled by 1/sqrt(d), zeros for a token that sees nothing, query heads in groups, the cache in 16 or 8 bits,
     max_new a hint, out."""
-    from . import _call, _stream_ptr
-
     name = "paged_tree_attn"
     _check(name, q, k_cache, v_cache, page_table, lengths, cu_seqlens, k_scale, v_scale)
     _checks.check_query_heads(name, q, k_cache)
@@ -107,8 +103,6 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target_probs: torc
     tokens; p if they are all 0; -1 if p is too, or for a sequence without tokens (accepted 0). Elements that are not
     positive finite numbers are 0, a draft whose token is not in the vocabulary is none. Sums and comparisons are in 64 bits.
     max_new: the most new tokens of a sequence (default: all tokens, up to 1024)."""
-    from . import _call, _stream_ptr
-
     name = "verify_draft"
     _checks.check_vector(name, "cu_seqlens", cu_seqlens, torch.int32, None, parents.device)
     seqs = cu_seqlens.shape[0] - 1
@@ -143,8 +137,6 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     The row of sequence s's new token path[s, j] becomes that of its new token j, for j below accepted[s] (verify_draft's
     results: paths ascend); keys, values and, in 8 bits, their codes and scales as they are. An entry that is no new
     token of the sequence leaves its row as it is. The new length is lengths - count + accepted."""
-    from . import _call, _stream_ptr
-
     name = "cache_keep"
     _check(name, None, k_cache, v_cache, page_table, lengths, None, k_scale, v_scale)
     seqs, device = lengths.shape[0], k_cache.device

@@ -10,7 +10,7 @@ import struct
 
 import torch
 
-from . import _checks, _native
+from . import _call, _checks, _native, _stream_ptr
 
 _DTYPE_CODE = {torch.float32: _native.DTYPE_F32, torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16}
 
@@ -66,8 +66,6 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs
     p + r / 2, or 2 p and 2 p + 1 (interleaved). inverse: by the negative angle: applied to the gradients of the results,
     with the same scale, it gives those of q and k. Angles are computed in 64 bits (right at any 32-bit position), the
     turn in 32."""
-    from . import _call, _stream_ptr
-
     if inplace or not _checks.rope_ok(q, k, positions, freqs):
         _checks.check_rope("rope", q, k, positions, freqs, inplace)
     shape, device = q.shape, q.device
