@@ -240,6 +240,11 @@ __device__ __forceinline__ float unit_for(float unit, float top) {
 // 64 single tokens over up to 8192 keys, 32 heads over 8, D = 128, bf16: 215 us, 5.5 TB/s; 32 over 16384, 32 over 4,
 // e4m3: 60 us, 5.0 TB/s of codes and scales. One over 1031, which is latency: 9.8 us and 4.5 of the join.
 //
+// TREE: instead of an order, a mask says which of its sequence's new tokens a row sees; it is looked at in the steps that
+// reach past the sequence's earlier keys, of which all are seen. 32 x 8 tokens of 32 heads over 8 and 8192 keys, D = 128: bf16
+// 192 us, 5.6 TB/s, e4m3 181. One of 16 tokens over 1000, latency: 12.4 us (1.5 to find its share, 1.8 its place, 2.4 queries
+// and first keys, 1.6 the keys, 2.2 the waves' join) and 4.8 of the join.
+//
 // Workgroups on a CU: two, but for two blocks of 128 dims in 16 bits, whose queries (32 registers), O (64) and rows
 // on their way (64) leave too few of half the registers (64 x 8 tokens over 8192 keys: 226 us, with two 260). One
 // block with one, 16 bits, 256 x 1 over 700: 109 for 95; in 8 bits, 64 x 1 over 8192 and 64 dims, 108 for 81. Two blocks
@@ -634,6 +639,11 @@ paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
 // fp16, whose units cost three more VALU operations a pair of scores and 9 to 16 registers in memory, 2.51 and 2.58; D = 64
 // 1.28 ms, int8 1.75, with fp16 2.04.
 //
+// TREE, as above: tiles of 64 and 128 rows too, so that a tree's keys go past once. Then it is the keys' bytes that bound
+// it: 32 x 16 tokens of 32 heads over 8 and 8192 keys, D = 128, bf16, 64 rows a tile, 206 us, 5.3 TB/s; x 32, 128 rows, 221; x 64,
+// 256 rows, 327, of which 277 are left where all read one sequence's pages (the matrix core and the VALU, a third of their
+// time each: two waves of a SIMD keep step). In 8 bits VALU: x 32 in e4m3 268.
+//
 // Rows of a tile, D = 128, 256 and 128 (one workgroup of 8 waves on a CU, two of 4): that case 2015 and 2183 us, 4 x
 // 2048 120 and 117, 24 x 700 over 4096 456 and 491, 256 x 64 over 640 73 and 85. D = 64 has 128, and as many
 // workgroups on a CU as the registers allow, three in 16 bits (4 x 2048 tokens f16 88 us, with two 100), two in 8
@@ -642,13 +652,16 @@ constexpr int chunk_rows_of(int d) { return d == 128 ? 256 : 128; }
 constexpr int chunk_wgs(int d, bool k8, int rows, bool tree) {   // workgroups on a CU
   return d == 128 ? 1 : !tree ? (k8 ? 2 : 3) : rows == 64 ? 4 : 2;
 }
+constexpr int chunk_waves(int d, bool k8, int rows, bool tree) {   // waves on a SIMD
+  return chunk_wgs(d, k8, rows, tree) * rows >= 256 ? chunk_wgs(d, k8, rows, tree) * rows / 128 : 1;
+}
 
 // WIDE: caches (or their scales) past a buffer's 32-bit offsets. 16-bit rows then come from 64-bit addresses by
 // instructions of the flat kind, after which the compiler waits for all LDS reads instead of the oldest; 8-bit ones
 // are not pipelined at all. The case above takes 2108 us (in buffers 1976), in int8 3129 (2312), with D = 64 2659 (1756).
 constexpr uint32_t kPastBuffer = 0xffffe000u;
 template <typename T, typename C, int D, int BM, bool WIDE, bool TREE = false>
-__global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chunk_wgs(D, cache_type<C>::k8bit, BM, TREE) * BM >= 256 ? chunk_wgs(D, cache_type<C>::k8bit, BM, TREE) * BM / 128 : 1)))
+__global__ void __launch_bounds__(BM * 2) __attribute__((amdgpu_waves_per_eu(chunk_waves(D, cache_type<C>::k8bit, BM, TREE))))
 paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;

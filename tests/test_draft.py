@@ -295,3 +295,57 @@ def test_oracle_rope_turns_by_the_angle():
     assert math.isclose(float(z[1, 0, 3]), float(x[1, 0, 2].double() * math.sin(0.25) + x[1, 0, 3].double() * math.cos(0.25)), rel_tol=1e-12)
     back, _ = do.rope(y.float(), torch.tensor([0, 1, 5]), f, inverse=True)
     assert torch.allclose(back, x.double(), atol=1e-6)
+
+
+@pytest.mark.parametrize("change", [
+    {}, {"parents": ints(6, dtype=I64)}, {"parents": ints(12)[::2]}, {"parents": ints(0)}, {"tokens": ints(5, dtype=I64)}, {"tokens": ints(6)},
+    {"uniform": torch.zeros(6).double()}, {"uniform": torch.zeros(12)[::2]}, {"cu": ints(4, dtype=I64)}, {"cu": ints(8)[::2]}, {"most": 0},
+    {"most": 1025}, {"most": True}, {"most": 2.0}, {"p": torch.zeros(5, 9)}, {"p": torch.zeros(6, 9).half()}, {"p": torch.zeros(9, 6).t()},
+    {"p": torch.zeros(6, 0)}, {"q": torch.zeros(6, 8)}, {"q": torch.zeros(6, 9).double()}, {"q": None}, {"p": torch.zeros(6, 20)[:, 3:12]},
+    {"parents": torch.zeros(6, dtype=I32, device="meta")}, {"q": torch.zeros(6, 9, device="meta")}])
+def test_one_pass_acceptance_agrees_with_the_checks(change):
+    """trees_ok and probs_ok accept what the checks one by one accept (on CPU tensors that say they are on the GPU)."""
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+    t = {"parents": ints(6), "tokens": ints(6, dtype=I64), "uniform": torch.zeros(6), "cu": ints(4), "p": torch.zeros(6, 9), "q": torch.zeros(6, 9)}
+    t.update({n: x for n, x in change.items() if n != "most"})
+    t = {n: x if x is None else x.as_subclass(OnGpu) for n, x in t.items()}
+    most = change.get("most", 4)
+
+    def one_by_one():
+        try:
+            device, n = t["parents"].device, t["parents"].shape[0]
+            _checks.check_tree("verify_draft", t["parents"], 3, t["cu"], most)
+            _checks.check_vector("verify_draft", "tokens", t["tokens"], I64, n, device)
+            _checks.check_vector("verify_draft", "uniform", t["uniform"], torch.float32, n, device)
+            _checks.check_probs("verify_draft", "target_probs", t["p"], n, device)
+            if t["q"] is not None:
+                _checks.check_probs("verify_draft", "draft_probs", t["q"], n, device, t["p"].shape[1])
+        except RuntimeError:
+            return False
+        return True
+    shape = t["parents"].shape
+    ok = _checks.trees_ok(t["parents"], ((t["tokens"], I64, shape), (t["uniform"], torch.float32, shape), (t["cu"], I32, torch.Size([4]))), most) and all(
+        x is None or _checks.probs_ok(x, shape[0], t["parents"].device, t["p"].shape[1]) for x in (t["p"], t["q"]))
+    assert ok == one_by_one(), change
+
+
+@pytest.mark.parametrize("change", [
+    {}, {"k": None}, {"q": torch.zeros(6, 4, 64, dtype=torch.float64)}, {"q": torch.zeros(6, 4)}, {"q": torch.zeros(0, 4, 64)},
+    {"q": torch.zeros(6, 64, 4).transpose(1, 2)}, {"k": torch.zeros(6, 2, 32)}, {"k": torch.zeros(5, 2, 64)}, {"k": torch.zeros(6, 2, 64).half()},
+    {"positions": ints(5)}, {"positions": torch.zeros(6)}, {"positions": ints(12)[::2]}, {"positions": ints(6, dtype=I64)}, {"freqs": torch.ones(33, dtype=torch.float64)},
+    {"freqs": torch.ones(8)}, {"freqs": torch.ones(16, dtype=torch.float64)[::2]}, {"freqs": torch.ones(0, dtype=torch.float64)},
+    {"q": torch.zeros(2, 4, 6, 64), "k": torch.zeros(2, 1, 6, 64)}, {"q": torch.zeros(2, 4, 6, 64), "k": None, "positions": ints(2, 6)},
+    {"q": torch.zeros(2, 4, 6, 64), "k": None, "positions": ints(6, 2)}, {"k": torch.zeros(6, 2, 64, device="meta")}])
+def test_one_pass_acceptance_of_rope_agrees_with_its_check(change):
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+    t = {"q": torch.zeros(6, 4, 64), "k": torch.zeros(6, 2, 64), "positions": ints(6), "freqs": torch.ones(16, dtype=torch.float64)}
+    t.update(change)
+    t = {n: x if x is None else x.as_subclass(OnGpu) for n, x in t.items()}
+    try:
+        _checks.check_rope("rope", t["q"], t["k"], t["positions"], t["freqs"], False)
+        fine = True
+    except RuntimeError:
+        fine = False
+    assert _checks.rope_ok(t["q"], t["k"], t["positions"], t["freqs"]) == fine
