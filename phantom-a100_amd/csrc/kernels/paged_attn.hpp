@@ -639,9 +639,8 @@ paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
 // fp16, whose units cost three more VALU operations a pair of scores and 9 to 16 registers in memory, 2.51 and 2.58; D = 64
 // 1.28 ms, int8 1.75, with fp16 2.04.
 //
-// TREE, as above: tiles of 64 and 128 rows too, so that a tree's keys go past once. Then it is the keys' bytes that bound
-// it: 32 x 16 tokens of 32 heads over 8 and 8192 keys, D = 128, bf16, 64 rows a tile, 206 us, 5.3 TB/s; x 32, 128 rows, 221; x 64,
-// 256 rows, 327, of which 277 are left where all read one sequence's pages (the matrix core and the VALU, a third of their
+// TREE, as above: tiles of 128 rows at D = 128 too, for trees that have no more. The keys' bytes then bound it: 32 x 12
+// tokens of 32 heads over 8 and 8192 keys, bf16, 202 us, 5.3 TB/s, x 28 213 to 229; x 64, 256 rows, 327, of which 277 are left where all read one sequence's pages (the matrix core and the VALU, a third of their
 // time each: two waves of a SIMD keep step). In 8 bits VALU: x 32 in e4m3 268.
 //
 // Rows of a tile, D = 128, 256 and 128 (one workgroup of 8 waves on a CU, two of 4): that case 2015 and 2183 us, 4 x
@@ -649,11 +648,11 @@ paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
 // workgroups on a CU as the registers allow, three in 16 bits (4 x 2048 tokens f16 88 us, with two 100), two in 8
 // (with three 24 x 700 over 4096 in int8 takes 493 for 480).
 constexpr int chunk_rows_of(int d) { return d == 128 ? 256 : 128; }
-constexpr int chunk_wgs(int d, bool k8, int rows, bool tree) {   // workgroups on a CU
-  return d == 128 ? 1 : !tree ? (k8 ? 2 : 3) : rows == 64 ? 4 : 2;
+constexpr int chunk_wgs(int d, bool k8, bool tree) {   // workgroups on a CU
+  return d == 128 ? 1 : tree || k8 ? 2 : 3;
 }
 constexpr int chunk_waves(int d, bool k8, int rows, bool tree) {   // waves on a SIMD
-  return chunk_wgs(d, k8, rows, tree) * rows >= 256 ? chunk_wgs(d, k8, rows, tree) * rows / 128 : 1;
+  return chunk_wgs(d, k8, tree) * rows / 128;
 }
 
 // WIDE: caches (or their scales) past a buffer's 32-bit offsets. 16-bit rows then come from 64-bit addresses by
@@ -770,15 +769,15 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
       const bool there = (key < key_end) & ((unsigned)page < (unsigned)c.pages);
       return there ? (int)at : -1;
     };
-    // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row (of loads 8 rows
-    // apart K's swizzle alternates in its highest bit; V's is the same, and both are for loads farther apart).
+    // 16-bit rows: thread's load i fills LDS slot i THREADS + tid, which holds the swizzled chunk of its row (loads are 16 or
+    // 32 rows apart, so the swizzle is the same).
     constexpr int APART = THREADS / LPR;   // rows between a thread's loads
-    static_assert(k8 || APART % 16 == 0 || (APART == 8 && CR == 16), "loads whose swizzles are alike, or alternate in one bit");
+    static_assert(k8 || APART % 16 == 0, "loads whose swizzles are alike");
     const int k_off = (tid % LPR ^ k_swz<CR>(tid / LPR)) * 16, v_off = (tid % LPR ^ v_swz<CR>(tid / LPR)) * 16;
     auto to_lds = [&](const void* cache, rsrc_t rs, const int (&rows)[CPT], unsigned char* stage, bool is_v) {
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
-        unsigned off = is_v ? v_off : APART == 8 && i % 2 ? k_off ^ 128 : k_off;
+        unsigned off = is_v ? v_off : k_off;
         asm("" : "+v"(off));   // (not to be added to the base once for all loads: that spills)
         unsigned char* to = stage + (i * THREADS + wave * kWave) * 16;
         if constexpr (WIDE) {

@@ -86,28 +86,33 @@ inline bool past_buffer(const PagedCache& c, int64_t d, bool k8) {
 
 // Rows of a tile for trees of more than 32 rows a key/value head: the tile whose time is the least by a start and a rate,
 // a us and f times the time that reading the keys and values once takes, for each tile that goes over them. (The table's
-// capacity stands for the lengths, which the host does not know.) Measured, D = 128, 32 heads over 8, us:
-//                                              32      64     128     256 rows
-//   bf16  s 32, 16 tokens over 8192 (1 GB)     371     203    206
-//         32 tokens                                    254    220
-//         64 tokens                                    510    317     316
-//         s 4, 64 tokens over 4000 (66 MB)      86      67     50      55
-//         over 1000 (16 MB)                     34      32     35      40
-//         s 4, 16 tokens over 1000              22      25     29
-//   e4m3  s 32, 16 tokens over 8192            285     297    265
-//         64 tokens                                   1165    530     344
-//         s 16, 40 tokens over 1000             77      95     50      51
-//         s 4, 16 tokens over 1000              31      46     35
-// 64 dims, 16 heads over 4: f16, 24 x 24 over 4096 54 with 32 rows, 128 44; e4m3 16 x 40 over 1000 32, 128 39.
+// capacity stands for the lengths, which the host does not know.) Measured, us:
+//                                                                 32     128     256 rows
+//   D = 128, 32 heads over 8, bf16   32 x 12 over 8192 (1 GB)    372     202
+//                                    32 x 28                     732     213
+//                                    32 x 48                    1095     411     291
+//                                    24 x 48 over 4096           374     175     128
+//                                    16 x 48 over 1000 (66 MB)    85      39      56
+//                                    16 x 12                      31      32
+//                                     4 x 48 over 500             29      32      48
+//                            e4m3    32 x 12 over 8192           287     268
+//                                    24 x 48 over 4096           315     226     153
+//                                    16 x 48 over 1000            86      49      70
+//                                     4 x 48 over 500             34      37      60
+//   D = 64, 16 heads over 4, f16     24 x 16 over 4096            46      40
+//                                    16 x 32 over 1000            26      28
+//                            int8    24 x 24 over 4096            61      50
+//                                    16 x 24 over 1000            26      29
+// (Tiles of 64 rows were within 5 % of one of these everywhere but 32 x 12 tokens of D = 64 over 8192, 66 and 59.)
 struct TileTime {
   int rows;
   double a, f;
 };
 inline int tree_rows(const PagedCache& c, int64_t d, bool k8, int64_t most) {
-  static const TileTime kTimes[4][4] = {{{32, 14, 0.9}, {64, 18, 0.95}, {128, 20, 1.02}, {256, 34, 1.45}},     // D = 128
-                                        {{32, 17, 1.6}, {128, 28, 2.5}, {256, 34, 3.2}, {0, 0, 0}},            // in 8 bits
-                                        {{32, 12, 1.0}, {64, 22, 1.0}, {128, 29, 0.75}, {0, 0, 0}},            // D = 64
-                                        {{32, 18, 1.3}, {128, 26, 2.6}, {0, 0, 0}, {0, 0, 0}}};
+  static const TileTime kTimes[4][3] = {{{32, 14, 0.9}, {128, 25, 1.02}, {256, 34, 1.45}},   // D = 128
+                                        {{32, 17, 1.6}, {128, 28, 2.5}, {256, 50, 3.2}},     // in 8 bits
+                                        {{32, 12, 1.0}, {128, 27, 0.75}, {0, 0, 0}},         // D = 64
+                                        {{32, 18, 1.3}, {128, 26, 2.6}, {0, 0, 0}}};
   const double once = 2.0 * c.seqs * c.heads * (double)c.capacity * d * (k8 ? 1 : 2) / 5e6;   // us at 5 TB/s
   int rows = 0;
   double least = 0;
@@ -148,7 +153,7 @@ inline AttnPlan attn_plan(const PagedCache& c, int64_t d, bool k8, int64_t heads
   const TileShape t = make_tiles((int)group, rows);
   const double tiles = (double)c.tokens / t.tokens + c.seqs;
   const double units = tiles * c.heads * t.splits * ((double)kTileCost + c.capacity);
-  const int resident = kCUs * (rows > 32 ? chunk_wgs((int)d, k8, rows, tree) : few_wgs((int)d, k8, rows / 16));
+  const int resident = kCUs * (rows > 32 ? chunk_wgs((int)d, k8, tree) : few_wgs((int)d, k8, rows / 16));
   const int least = tree && rows > 32 ? tree_units(rows) : kMinUnits;
   const int wgs = (int)std::max(1.0, std::min<double>(resident, units / least + 1));
   return {rows, wgs, least, c.capacity <= (tree && rows <= 32 ? kTreeWholeCapacity : kWholeCapacity)};
@@ -216,12 +221,8 @@ int attn_call(const char* name, const pa_paged_cache* cache, RowsQ a, int dtype,
     }
     if (past_buffer(c, D, cache_type<C>::k8bit))
       return launch_attn<T, D, CR>(paged_attn_chunk<T, C, D, CR, true, TREE>, 2 * CR, c, a, plan, w, workspace, st);
-    if constexpr (TREE) {
-      if constexpr (!cache_type<C>::k8bit)
-        if (plan.rows == 64) return launch_attn<T, D, 64>(paged_attn_chunk<T, C, D, 64, false, TREE>, 128, c, a, plan, w, workspace, st);
-      if constexpr (CR != 128)
-        if (plan.rows == 128) return launch_attn<T, D, 128>(paged_attn_chunk<T, C, D, 128, false, TREE>, 256, c, a, plan, w, workspace, st);
-    }
+    if constexpr (TREE && CR != 128)
+      if (plan.rows == 128) return launch_attn<T, D, 128>(paged_attn_chunk<T, C, D, 128, false, TREE>, 256, c, a, plan, w, workspace, st);
     return launch_attn<T, D, CR>(paged_attn_chunk<T, C, D, CR, false, TREE>, 2 * CR, c, a, plan, w, workspace, st);
   });
   return hip_status(e, name);

@@ -218,6 +218,10 @@ SEQS = {
 }
 
 
+# A page table of many columns lets the launcher expect long sequences: it then takes tiles of as many rows as a tree has.
+MANY = 60000
+
+
 @pytest.mark.parametrize("kind", list(SEQS))
 @pytest.mark.parametrize("dtype,cache", TYPES, ids=IDS)
 @pytest.mark.parametrize("d,hq,hkv,page", [(64, 4, 2, 16), (128, 8, 1, 24), (128, 3, 3, 64)])
@@ -226,24 +230,45 @@ def test_attention(kind, dtype, cache, d, hq, hkv, page):
 
 
 @pytest.mark.parametrize("dtype,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [9, 16, 17, 32, 33, 50, 64, 70, 130])
+def test_tiles_of_every_size(dtype, cache, d, n):
+    """4 query heads a key/value head: 36 to 520 rows, beside trees with fewer and sequences with none."""
+    seqs = [(n, n + 700), (1, 333), (0, 20), (n // 2, 64 + n // 2), (n, n), (3, 129)]
+    check_attn(po.make(seqs, hq=8, hkv=2, d=d, page=16, dtype=dtype, cache=cache, columns=MANY), tree_masks(seqs, seed=n), max_new=n)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (F16, E4M3), (BF16, I8)], ids=IDS)
+@pytest.mark.parametrize("d,n", [(64, 14), (64, 40), (128, 14), (128, 30), (128, 60)])
+def test_tiles_of_many_sequences(dtype, cache, d, n):
+    g = torch.Generator().manual_seed(n)
+    r = lambda k: int(torch.randint(k, (1,), generator=g))  # noqa: E731
+    seqs = [(0, r(50)) if i % 7 == 3 else (c := 1 + r(n), c + r(400)) for i in range(40)]
+    check_attn(po.make(seqs, hq=4, hkv=1, d=d, page=16, dtype=dtype, cache=cache, columns=MANY), tree_masks(seqs), max_new=n)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES, ids=IDS)
 @pytest.mark.parametrize("d,hq", [(64, 2), (128, 8)])
 @pytest.mark.parametrize("width", [1, 2, 5])
-def test_any_mask(dtype, cache, d, hq, width):
+@pytest.mark.parametrize("columns", [None, MANY])
+def test_any_mask(dtype, cache, d, hq, width, columns):
     """Bits of no tree: rows that see later tokens, not themselves, or nothing; fewer and more words than tokens."""
     seqs = [(70, 70), (40, 333), (9, 9), (1, 1), (3, 90)]
     g = torch.Generator().manual_seed(width)
     mask = torch.randint(-2 ** 31, 2 ** 31, (123, width), generator=g).to(torch.int32)
     mask[:5], mask[111:113] = 0, 0          # (rows of sequences without earlier keys: nothing to see)
     mask[20:25] = -1
-    got = check_attn(po.make(seqs, hq=hq, hkv=2, d=d, dtype=dtype, cache=cache), mask)
+    got = check_attn(po.make(seqs, hq=hq, hkv=2, d=d, dtype=dtype, cache=cache, columns=columns), mask)
     assert bool((got[:5] == 0).all()) and bool((got[111:113] == 0).all())
 
 
 @pytest.mark.parametrize("dtype,cache", [(F16, F16), (BF16, E4M3)], ids=IDS)
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (5, 1), (12, 4), (16, 1), (40, 2), (96, 1), (300, 1)])
-def test_head_groups(dtype, cache, hq, hkv):
+@pytest.mark.parametrize("columns", [None, MANY])
+def test_head_groups(dtype, cache, hq, hkv, columns):
     seqs = [(1, 70), (4, 100), (19, 40)]
-    check_attn(po.make(seqs, hq=hq, hkv=hkv, d=128, dtype=dtype, cache=cache), tree_masks(seqs))
+    for bound in (None, 19):
+        check_attn(po.make(seqs, hq=hq, hkv=hkv, d=128, dtype=dtype, cache=cache, columns=columns), tree_masks(seqs), max_new=bound)
 
 
 @pytest.mark.parametrize("page", [1, 7, 16, 48, 256])
@@ -269,14 +294,15 @@ def test_max_new_is_a_hint(dtype, cache, max_new):
 @pytest.mark.parametrize("dtype,cache", TYPES, ids=IDS)
 @pytest.mark.parametrize("n,d", [(20, 64), (20, 128), (120, 64), (120, 128)])
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
-def test_values_that_are_not_finite_reach_the_rows_that_see_them(dtype, cache, n, d, bad):
+@pytest.mark.parametrize("columns", [None, MANY])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(dtype, cache, n, d, bad, columns):
     """A value (8 bits: its scale) of one drafted token: rows that do not see it keep their results."""
     seqs = [(n, n + 70), (3, 50)]
     rng = random.Random(7)
     sets = [set(do.ancestors(t, i)) for c, _ in seqs for t in [do.random_tree(c, 3, rng)] for i in range(c)]
     mask = do.words(sets, -(-n // 32))
     for which in ("v", "k"):
-        p = po.make(seqs, d=d, hq=4, hkv=2, dtype=dtype, cache=cache)
+        p = po.make(seqs, d=d, hq=4, hkv=2, dtype=dtype, cache=cache, columns=columns)
         pg, rw = po.slot(p, 0, 70 + 4)
         if p.scales:
             p.scales[which + "_scale"][pg, :, rw] = bad
@@ -305,16 +331,17 @@ def test_a_chain_is_causal_attention():
     assert bool(((got - ref).abs() <= bound).all())
 
 
-def test_pages_lengths_and_offsets_out_of_range():
+@pytest.mark.parametrize("columns", [None, MANY])
+def test_pages_lengths_and_offsets_out_of_range(columns):
     seqs = [(2, 40), (30, 64), (20, 50)]
     mask = tree_masks(seqs)
-    p = po.make(seqs, d=64, page=16, dtype=F16)
+    p = po.make(seqs, d=64, page=16, dtype=F16, columns=columns)
     p.table[0, 2], p.table[1, 3], p.table[1, 0] = -1, p.k_cache.shape[0], 2 ** 31 - 1
     check_attn(p, mask)
     p.table[2, :] = -5   # nothing to see
     check_attn(p, mask)
-    p = po.make(seqs, d=64, page=16, dtype=F16)
-    p.lengths[:] = torch.tensor([-7, 2 ** 31 - 1, 90], dtype=torch.int32)   # 90: past the table's columns
+    p = po.make(seqs, d=64, page=16, dtype=F16, columns=columns)
+    p.lengths[:] = torch.tensor([-7, 2 ** 31 - 1 if columns is None else 5000, 90], dtype=torch.int32)   # 90: past the table's columns
     check_attn(p, mask)
     p.cu[:] = torch.tensor([-3, 2, 1, 99], dtype=torch.int32)
     check_attn(p, mask)
