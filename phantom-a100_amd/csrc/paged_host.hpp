@@ -103,7 +103,7 @@ inline bool past_buffer(const PagedCache& c, int64_t d, bool k8) {
 //                                    16 x 32 over 1000            26      28
 //                            int8    24 x 24 over 4096            61      50
 //                                    16 x 24 over 1000            26      29
-// (Tiles of 64 rows were within 5 % of one of these everywhere but 32 x 12 tokens of D = 64 over 8192, 66 and 59.)
+// (Tiles of 64 rows were nowhere more than 2 % faster than the better of these.)
 struct TileTime {
   int rows;
   double a, f;

@@ -129,6 +129,33 @@ def test_rope_dense(dtype, interleaved):
     check_rope(q.transpose(1, 2).contiguous().transpose(1, 2), k[:, :, :, :].expand(3, 6, 50, 64), torch.arange(0, 100, 2), f)
 
 
+@pytest.mark.parametrize("shape", [(1, 1, 1, 64), (2, 3, 1, 64), (1, 2, 9, 96), (3, 1, 5, 2)])
+def test_rope_dense_shapes(shape):
+    g = torch.Generator().manual_seed(4)
+    q, k = torch.randn(shape, generator=g), torch.randn(shape[0], 2, *shape[2:], generator=g)
+    f = freqs_of(shape[3])
+    check_rope(q, k, torch.full((1,), 7).expand(shape[2]), f)   # (a stride of 0)
+    check_rope(q, k, torch.full((1, 1), 7).expand(shape[0], shape[2]), f, interleaved=True)
+    both = torch.randn(shape[0], shape[2], shape[1] + 3, shape[3], generator=g).cuda().transpose(1, 2)   # of one projection
+    q, k = both[:, :shape[1]], both[:, shape[1]:shape[1] + 2]
+    before, positions = both.clone(), torch.arange(shape[2]).cuda()
+    want = cuda_attn.rope(q.clone(), k.clone(), positions, f.cuda())
+    cuda_attn.rope(q, k, positions, f.cuda(), inplace=True)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(both[:, -1], before[:, -1])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_past_32_bits(interleaved):
+    """More than 2^31 elements, in place; the last rows are those of a small call."""
+    tokens = 2 ** 31 // (64 * 128) + 100
+    q = torch.zeros(tokens, 64, 128, dtype=F16, device="cuda")
+    q[-50:] = torch.randn(50, 64, 128, device="cuda").to(F16)
+    positions, f = torch.arange(tokens, device="cuda"), freqs_of(128).cuda()
+    want = cuda_attn.rope(q[-50:].clone(), None, positions[-50:], f, interleaved=interleaved)[0]
+    cuda_attn.rope(q, None, positions, f, interleaved=interleaved, inplace=True)
+    assert torch.equal(q[-50:], want) and not bool(q[-100:-50].any()) and not bool(q[:50].any())
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS)
 @pytest.mark.parametrize("shift,pad", [(0, 0), (1, 3), (2, 2), (4, 4), (8, 8)])
 def test_rope_strides_and_alignment(dtype, shift, pad):
@@ -435,6 +462,32 @@ def test_verify_rows_at_any_address(drawn):
 
 
 @pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("vocab", [3000, 70001])
+def test_verify_one_row_for_all(drawn, vocab):
+    """Rows that are the same memory (a stride of 0)."""
+    tokens, parents, p, u, cu, q = do.drafts([5, 9, 4], vocab, 2, 1, drawn)
+    p, q = p[:1].expand(18, vocab), None if q is None else q[:1].expand(18, vocab)
+    one = lambda x: x[:1].cuda().expand(18, vocab)  # noqa: E731
+    check_verify(tokens, parents, p, u, cu, q, max_new=9, place=one)
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_past_32_bits(drawn):
+    """Probabilities of more than 2^31 elements, the sequences at their end."""
+    vocab, rows = 128001, 2 ** 31 // 128001 + 30
+    tokens, parents, p, u, cu, q = do.drafts([9, 4], vocab, 2, 1, drawn, 0.5)
+    def place(x):
+        room = torch.empty(rows, vocab, device="cuda")
+        room[-13:] = x.cuda()
+        return room
+    wide = lambda x: torch.cat([torch.zeros(rows - 13, dtype=x.dtype), x]).cuda()  # noqa: E731
+    got = cuda_attn.verify_draft(wide(tokens), wide(parents), place(p), wide(u), (cu + rows - 13).to(torch.int32).cuda(),
+                                 draft_probs=None if q is None else place(q), max_new=9)
+    for a, b in zip(got, do.verify(tokens, parents, p, u, cu, q, 9)):
+        assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("drawn", [True, False])
 def test_verify_unusual_rows(drawn):
     """One-hot rows, equal models, rows without mass, elements that are not finite or negative, drafts out of the vocabulary or
     twice the same, numbers at the ends of their range, entries of parents that are no earlier token."""
@@ -459,6 +512,8 @@ def test_verify_unusual_rows(drawn):
     p[96:102] *= 2.0 ** -140                 # subnormal
     p[102:108] *= 2.0 ** 100
     check_verify(tokens, parents, p, u, cu, q, max_new=6)
+    long = lambda x: x if x is None else torch.cat([x, torch.zeros(x.shape[0], 70000)], 1)  # noqa: E731
+    check_verify(tokens, parents, long(p), u, cu, long(q), max_new=6)   # (a vocabulary that takes more than one launch)
     check_verify(tokens, parents, p, u, cu, q, max_new=4)   # the last two tokens of each are not looked at
     check_verify(tokens, parents, p, u, torch.tensor([-5, 6, 3, 20, 200], dtype=torch.int32), q, max_new=20)
 
