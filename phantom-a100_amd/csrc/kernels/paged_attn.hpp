@@ -640,19 +640,24 @@ paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
 // 1.28 ms, int8 1.75, with fp16 2.04.
 //
 // TREE, as above: tiles of 128 rows at D = 128 too, for trees that have no more. The keys' bytes then bound it: 32 x 12
-// tokens of 32 heads over 8 and 8192 keys, bf16, 202 us, 5.3 TB/s, x 28 213 to 229; x 64, 256 rows, 327, of which 277 are left where all read one sequence's pages (the matrix core and the VALU, a third of their
-// time each: two waves of a SIMD keep step). In 8 bits VALU: x 32 in e4m3 268.
+// tokens of 32 heads over 8 and 8192 keys, bf16, 202 us, 5.3 TB/s, x 28 213 to 229; x 64, 256 rows, 327, of which 277 are
+// left where all read one sequence's pages (the matrix core and the VALU, a third of their time each: two waves of a
+// SIMD keep step). In 8 bits two tiles of 64 keys and their raw rows leave no LDS for a second workgroup of 128 rows, and one
+// wave a SIMD waits for each step of its own: tiles of 32 keys, two workgroups. x 12 in e4m3 266 us, now 206, x 32 269 and
+// 234, x 12 fp16 in int8 306 and 245. The steps behind one another still bound it, of two waves now (206 where all read one
+// sequence's pages 196; the other workgroup's waves with rows on the SIMDs without 203). x 64, 256 rows, 350.
 //
 // Rows of a tile, D = 128, 256 and 128 (one workgroup of 8 waves on a CU, two of 4): that case 2015 and 2183 us, 4 x
 // 2048 120 and 117, 24 x 700 over 4096 456 and 491, 256 x 64 over 640 73 and 85. D = 64 has 128, and as many
 // workgroups on a CU as the registers allow, three in 16 bits (4 x 2048 tokens f16 88 us, with two 100), two in 8
 // (with three 24 x 700 over 4096 in int8 takes 493 for 480).
 constexpr int chunk_rows_of(int d) { return d == 128 ? 256 : 128; }
-constexpr int chunk_wgs(int d, bool k8, bool tree) {   // workgroups on a CU
-  return d == 128 ? 1 : tree || k8 ? 2 : 3;
+constexpr int chunk_keys(int d, bool k8, int rows) { return d == 128 && k8 && rows == 128 ? 32 : 64; }   // keys of a tile
+constexpr int chunk_wgs(int d, bool k8, int rows, bool tree) {   // workgroups on a CU
+  return chunk_keys(d, k8, rows) == 32 ? 2 : d == 128 ? 1 : tree || k8 ? 2 : 3;
 }
 constexpr int chunk_waves(int d, bool k8, int rows, bool tree) {   // waves on a SIMD
-  return chunk_wgs(d, k8, tree) * rows / 128;
+  return chunk_wgs(d, k8, rows, tree) * rows / 128;
 }
 
 // WIDE: caches (or their scales) past a buffer's 32-bit offsets. 16-bit rows then come from 64-bit addresses by
@@ -665,13 +670,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   typedef typename vec8<T>::type V8;
   constexpr bool k8 = cache_type<C>::k8bit;
   constexpr bool kUnits = k8 && std::is_same<T, f16>::value;   // each row's O in a unit of its own
-  constexpr int BN = 64, THREADS = BM * 2, RB = D * 2, CB = k8 ? D : 2 * D, CR = D / 8;
+  constexpr int BN = chunk_keys(D, k8, BM), THREADS = BM * 2, RB = D * 2, CB = k8 ? D : 2 * D, CR = D / 8;
   constexpr int TILE_BYTES = BN * RB;
   constexpr int QK_STEPS = D / 16, NKB = BN / 32, NDB = D / 32, PV_STEPS = BN / 16;
   constexpr int CPT = BN * CB / 16 / THREADS;   // 16-byte loads per thread, matrix and tile
   constexpr int LPR = CB / 16;                  // lanes a cache row
   static_assert(CPT * THREADS * 16 == BN * CB, "a tile's loads split evenly");
   constexpr float kLazyLog2 = 8.f;
+  constexpr uint64_t kWhole = BN == kWave ? ~0ull : (1ull << BN % kWave) - 1;   // a tile's keys as bits
   __shared__ __attribute__((aligned(1024))) unsigned char k_lds0[TILE_BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char v_lds0[TILE_BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char k_lds1[TILE_BYTES];
@@ -679,7 +685,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   // 8 bits: rows as they are, each thread's own, on their way to the stages; and four tiles' scales.
   constexpr int RAW = k8 && !WIDE ? BN * CB : 16, SLOTS = k8 ? 4 : 1;
   __shared__ __attribute__((aligned(1024))) unsigned char k_raw0[RAW], k_raw1[RAW], v_raw0[RAW], v_raw1[RAW];
-  __shared__ __attribute__((aligned(256))) float ks_lds[SLOTS][BN], vs_lds[SLOTS][BN];
+  __shared__ __attribute__((aligned(256))) float ks_lds[SLOTS][kWave], vs_lds[SLOTS][kWave];
   __shared__ float ones_lds[k8 ? BN : 1];
   __shared__ int odd_lds[2][BM / 32];   // of V(t), at t % 2: whether a wave's share has a value that is not finite
   __shared__ int64_t walk_lds[10];
@@ -817,7 +823,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
           *reinterpret_cast<u32x4*>(stage + r * RB + (ch ^ 1) * 16) = hi16;
         }
     };
-    auto present_of = [&](int row) -> uint64_t { return __builtin_amdgcn_ballot_w64(row >= 0); };
+    auto present_of = [&](int row) -> uint64_t { return __builtin_amdgcn_ballot_w64(row >= 0) & kWhole; };
     // The row that each of the thread's loads reads; where loads are from a buffer, its byte offset, past the
     // buffer's end (which loads as zeros) for an absent key. Elsewhere an absent key takes the row of the tile's
     // first present one: its scores are masked, and its P is 0, which a finite value leaves without effect.
@@ -1006,13 +1012,13 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
         top = max_bits(top, *reinterpret_cast<const u32x4*>(vs + at * 16));
       }
       bool odd_here = max(top[0], top[1]) >= kInfBits<T>;
-      if constexpr (k8) odd_here = odd_here || !(fabsf(vs_lds[t % SLOTS][lane]) < INFINITY);
+      if constexpr (k8) odd_here = odd_here || !(fabsf(vs_lds[t % SLOTS][lane % BN]) < INFINITY);
       const bool any = __builtin_amdgcn_ballot_w64(odd_here) != 0;
       if (lane == 0) odd_lds[t & 1][wave] = any;
     };
     auto values_finite = [&](int t) { return __builtin_amdgcn_ballot_w64(odd_lds[t & 1][lane % (BM / 32)] != 0) == 0; };
     const int wave_tiles = (min(wave_any, key_end) - key_begin + BN - 1) / BN;   // tiles with a key for some row of the wave
-    auto is_clean = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= wave_all; };
+    auto is_clean = [&](int t, uint64_t pres) { return pres == kWhole && key_begin + (t + 1) * BN <= wave_all; };
 
     // ---- the first tiles: K(0), V(0), K(1). At a tile t: rows[j] and row[j] are tile t + 1 + j's, present[j] tile
     // t + j's; page holds tile t + 1 + AHEAD's entries.
@@ -1020,7 +1026,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
     uint64_t present[AHEAD + 1];
     const int tile_all = TREE ? keys_before(sg.rows, c.capacity)   // the first row's keys, which all see
                               : keys_seen(sg.rows, sg.tile * w.tiles.tokens, c.capacity, w.causal);
-    auto whole_tile = [&](int t, uint64_t pres) { return pres == ~0ull && key_begin + (t + 1) * BN <= tile_all; };
+    auto whole_tile = [&](int t, uint64_t pres) { return pres == kWhole && key_begin + (t + 1) * BN <= tile_all; };
     auto advance = [&](int next_row, uint64_t next_present) {   // to the next tile (its new rows[AHEAD - 1] apart)
 #pragma unroll
       for (int j = 0; j + 1 < AHEAD; ++j) {
@@ -1185,7 +1191,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
           __builtin_amdgcn_sched_barrier(0);
           __builtin_amdgcn_s_setprio(2);
           {
-            constexpr int N = NKB * QK_STEPS, EACH = N / 4;   // MFMAs; four exponentials after each EACH of them
+            constexpr int N = NKB * QK_STEPS, EACH = N / (2 * HALF);   // MFMAs; four exponentials after each EACH of them
             const unsigned char* ks = k_stage(nxt);
             int kb = k_base;
             asm("" : "+v"(kb));
@@ -1237,7 +1243,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
           // Phase B: O += V(t) P(t) with the row sums of P(t), the row maxima of S(t+1) and the first half of P(t+1)
           // against the reference as it is; where that is raised after all, the half is taken again.
           {
-            constexpr int N = PV_STEPS * NDB, EACH = N / 4;
+            constexpr int N = PV_STEPS * NDB, EACH = N / (2 * HALF);
             u32x4 kx[CPT], vx[CPT];
             const unsigned char* vs = v_stage(cur);
             int vb = v_base;
@@ -1250,6 +1256,9 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
               return __builtin_bit_cast(V8, x);
             };
             const float neg_m = neg_ref(), inv = inverse_unit();
+            auto key_scales = [&](int k) { return *reinterpret_cast<const f32x4*>(ks_next + k / 16 * 32 + k % 16 * 2 + 4 * hi); };
+            f32x4 scales = {1.f, 1.f, 1.f, 1.f};   // of four scores, read one step before their use
+            if constexpr (k8) scales = key_scales(0);
             V8 ahead[2] = {operand(0), operand(1)};
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -1260,9 +1269,9 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
               for (int k = 16 * NKB / N * i; k < 16 * NKB / N * (i + 1); k += 2) {
                 if constexpr (k8) {   // (four scores at a time)
                   if (k % 4 == 0) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(ks_next + k / 16 * 32 + k % 16 * 2 + 4 * hi);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sn[k / 16][k % 16 + r] *= x[r];
+                    for (int r = 0; r < 4; ++r) sn[k / 16][k % 16 + r] *= scales[r];
+                    if (k + 4 < 16 * NKB) scales = key_scales(k + 4);
                   }
                 }
                 mx = max_nan(mx, max_nan(sn[k / 16][k % 16], sn[k / 16][k % 16 + 1]));
@@ -1376,14 +1385,14 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
       for (int t = from; t < wave_tiles; ++t) {
         int rest;
         const int page_t = load_page(t, rest), row_t = find_row(t, page_t, rest);
-        uint64_t keys = __builtin_amdgcn_ballot_w64(row_t >= 0);
+        uint64_t keys = present_of(row_t);
         if (kInfinite && again) {
           u16x2 largest = {0, 0};
           if (row_t >= 0)
 #pragma unroll 1
             for (int i = 0; i < D / 8; ++i)
               largest = max_bits(largest, *reinterpret_cast<const u32x4*>(static_cast<const C*>(c.v) + (int64_t)row_t * D + 8 * i));
-          keys = __builtin_amdgcn_ballot_w64(max(largest[0], largest[1]) >= kInfBits<T>);
+          keys &= __builtin_amdgcn_ballot_w64(max(largest[0], largest[1]) >= kInfBits<T>);
         } else if (is_clean(t, keys)) {
           continue;
         }

@@ -95,10 +95,11 @@ inline bool past_buffer(const PagedCache& c, int64_t d, bool k8) {
 //                                    16 x 48 over 1000 (66 MB)    85      39      56
 //                                    16 x 12                      31      32
 //                                     4 x 48 over 500             29      32      48
-//                            e4m3    32 x 12 over 8192           287     268
-//                                    24 x 48 over 4096           315     226     153
-//                                    16 x 48 over 1000            86      49      70
-//                                     4 x 48 over 500             34      37      60
+//                            e4m3    32 x 12 over 8192           286     206     247
+//                                    32 x 48                     842     370     310
+//                                    16 x 48 over 4000           211     118     103
+//                                    16 x 16 over 1000            42      39      53
+//                                     4 x 24                      31      33      46
 //   D = 64, 16 heads over 4, f16     24 x 16 over 4096            46      40
 //                                    16 x 32 over 1000            26      28
 //                            int8    24 x 24 over 4096            61      50
@@ -110,7 +111,7 @@ struct TileTime {
 };
 inline int tree_rows(const PagedCache& c, int64_t d, bool k8, int64_t most) {
   static const TileTime kTimes[4][3] = {{{32, 14, 0.9}, {128, 25, 1.02}, {256, 34, 1.45}},   // D = 128
-                                        {{32, 17, 1.6}, {128, 28, 2.5}, {256, 50, 3.2}},     // in 8 bits
+                                        {{32, 17, 2.1}, {128, 31, 1.9}, {256, 50, 2.8}},     // in 8 bits
                                         {{32, 12, 1.0}, {128, 27, 0.75}, {0, 0, 0}},         // D = 64
                                         {{32, 18, 1.3}, {128, 26, 2.6}, {0, 0, 0}}};
   const double once = 2.0 * c.seqs * c.heads * (double)c.capacity * d * (k8 ? 1 : 2) / 5e6;   // us at 5 TB/s
@@ -153,7 +154,7 @@ inline AttnPlan attn_plan(const PagedCache& c, int64_t d, bool k8, int64_t heads
   const TileShape t = make_tiles((int)group, rows);
   const double tiles = (double)c.tokens / t.tokens + c.seqs;
   const double units = tiles * c.heads * t.splits * ((double)kTileCost + c.capacity);
-  const int resident = kCUs * (rows > 32 ? chunk_wgs((int)d, k8, tree) : few_wgs((int)d, k8, rows / 16));
+  const int resident = kCUs * (rows > 32 ? chunk_wgs((int)d, k8, rows, tree) : few_wgs((int)d, k8, rows / 16));
   const int least = tree && rows > 32 ? tree_units(rows) : kMinUnits;
   const int wgs = (int)std::max(1.0, std::min<double>(resident, units / least + 1));
   return {rows, wgs, least, c.capacity <= (tree && rows <= 32 ? kTreeWholeCapacity : kWholeCapacity)};

@@ -354,7 +354,7 @@ def test_one_pass_acceptance_of_rope_agrees_with_its_check(change):
 @pytest.mark.parametrize("dtype,d,new,rows,wgs", [
     ("f16", 128, 4, 16, 512), ("f16", 128, 8, 32, 256), ("f16", 128, 9, 128, 256), ("f16", 128, 16, 128, 256), ("f16", 128, 17, 128, 256),
     ("f16", 128, 32, 128, 256), ("f16", 128, 33, 256, 256), ("f16", 128, 200, 256, 256), ("f16", 64, 8, 32, 512), ("f16", 64, 17, 128, 512),
-    ("f16", 64, 64, 128, 512), ("i8", 128, 8, 32, 512), ("i8", 128, 17, 128, 256), ("i8", 128, 64, 256, 256), ("i8", 64, 17, 128, 512)])
+    ("f16", 64, 64, 128, 512), ("i8", 128, 8, 32, 512), ("i8", 128, 17, 128, 512), ("i8", 128, 64, 256, 256), ("i8", 64, 17, 128, 512)])
 def test_rows_of_a_tile(dtype, d, new, rows, wgs):
     """The tile that a call of long sequences takes (4 query heads a key/value head), by the workspace that it asks for."""
     lib = _native.lib()
@@ -365,4 +365,4 @@ def test_rows_of_a_tile(dtype, d, new, rows, wgs):
     assert need == -(-wgs * 16 // 256) * 256 + wgs * 2 * rows * (d + 2) * 4, (need - wgs * 16) / (wgs * 2 * (d + 2) * 4)
     # short ones: as few as there are
     c.table_cols = 20
-    assert lib.pa_paged_tree_attn_workspace(c, _native.DTYPE_F16, 32 * new, 32, P, new) <= max(need, wgs * (16 + 64 * (d + 2) * 4) + 256)
+    assert lib.pa_paged_tree_attn_workspace(c, _native.DTYPE_F16, 32 * new, 32, P, new) <= max(need + 256 * 16, wgs * (16 + 64 * (d + 2) * 4) + 256)
