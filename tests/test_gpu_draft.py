@@ -374,6 +374,20 @@ def test_pages_lengths_and_offsets_out_of_range(columns):
     check_attn(p, mask)
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("page", [5, 16])
+@pytest.mark.parametrize("n", [20, 40])
+def test_absent_pages_in_every_tile(dtype, cache, page, n):
+    """80 and 160 rows of 128 dims; pages that begin and end inside a tile are absent, one by one and in a row."""
+    seqs = [(n, n + 300), (3, 200), (n - 1, 2 * n)]
+    p = po.make(seqs, d=128, hq=8, hkv=2, page=page, dtype=dtype, cache=cache, columns=MANY)
+    p.table[0, 2], p.table[0, 5:8], p.table[1, 0], p.table[1, 9], p.table[2, 1] = -1, -3, p.k_cache.shape[0], 2 ** 31 - 1, -1
+    p.table[0, (n + 299) // page] = -1   # the last one
+    check_attn(p, tree_masks(seqs, seed=n), max_new=n)
+    p.table[0] = -1
+    check_attn(p, tree_masks(seqs, seed=n), max_new=n)
+
+
 @pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, I8)], ids=IDS)
 @pytest.mark.parametrize("new", [3, 70])
 def test_out_mask_strides_and_rows_behind(dtype, cache, new):
