@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256) draft_tree_rows(TreeArgs a) {
 // runs' sums first and in one run then. Short vocabularies go in one workgroup a sequence and one launch, long ones in as
 // many waves as the rows have runs, a launch behind the walk. What bounds them: 48 chains of up to 8 of 128000 tokens, latency in
 // the walk (4.9 us) and the choice (4.6), bytes between (8.8 us, 45 MB); one chain of 32000 in one workgroup, latency (9.4);
-// 16 trees of 21 of 65537 tokens, three drafts behind a token, the walk's own sums, up to four behind one another (36 us).
+// 16 trees of 21 of 65537 tokens, three drafts behind a token, the walk's own sums, up to four behind one another (26 us).
 struct VerifyState;
 struct VerifyArgs {
   const int64_t* tokens;
@@ -135,35 +135,55 @@ struct Drafts {
   float p[kTreeMax], q[kTreeMax], u[kTreeMax];
 };
 
-// S(off) of a row, by a workgroup of 1024 threads, 16 elements a thread and step. Rows of p and q of 256 KB each take 7.5 us,
-// of 512 KB 11, near the 64 bytes a clock that a CU reads. (Four elements a load and the class of a number by v_cmp_class:
-// with single ones, clamped indexes and comparisons it was bound by the VALU, 10 to 12 us for the first.)
+// Adds what is left of N elements to a sum. Where none of the wave's is negative or not finite, which their bits show for half an
+// operation an element, without the weights' own tests (16 trees of 21 of 65537 tokens 42 us and 34).
+template <int N>
+__device__ __forceinline__ void add_left(const float (&p)[N], const float (&q)[N], double off, double& sum) {
+  unsigned top = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) top = max(top, max(__builtin_bit_cast(unsigned, p[k]), __builtin_bit_cast(unsigned, q[k])));
+  if (__builtin_amdgcn_ballot_w64(top >= 0x7f800000u) == 0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) sum += left_of((double)p[k], off, (double)q[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) sum += left_of(weight_of(p[k]), off, weight_of(q[k]));
+  }
+}
+// S(off) of a row, by a workgroup of 1024 threads, 8 elements a thread and step, the next step's and the rest's on their way
+// meanwhile. What bounds it is the VALU of the one CU (66 % busy), six operations in 64 bits or on their way there a pair of elements: rows
+// of p and q of 256 KB each take 5 us. (Each element tested by its class, 16 a step and nothing ahead, 7.5; loads of single
+// elements and comparisons for the class, 10 to 12.)
 __device__ __forceinline__ double row_left(const VerifyArgs& a, int64_t row, double off, double* lds) {
-  constexpr int EACH = 4, STEP = EACH * 4096;
+  constexpr int EACH = 2, N = 4 * EACH, STEP = N * 1024;
   const float* pr = a.p + row * a.p_stride;
   const float* qr = a.q + row * a.q_stride;
-  double sum = 0;
-  int v0 = 0;
-  for (; v0 + STEP <= a.vocab; v0 += STEP) {
-    f32x4u p[EACH], q[EACH];
+  const int steps = a.vocab / STEP;
+  float p0[N], q0[N], p1[N], q1[N], p[N], q[N];
+  auto load = [&](int step, float (&ps)[N], float (&qs)[N]) {
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
-      const int v = v0 + 4 * ((int)threadIdx.x + 1024 * k);
-      p[k] = *reinterpret_cast<const f32x4u*>(pr + v), q[k] = *reinterpret_cast<const f32x4u*>(qr + v);
+      const int v = step * STEP + 4 * ((int)threadIdx.x + 1024 * k);
+      const f32x4u x = *reinterpret_cast<const f32x4u*>(pr + v), y = *reinterpret_cast<const f32x4u*>(qr + v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ps[4 * k + j] = x[j], qs[4 * k + j] = y[j];
     }
+  };
+  if (steps > 0) load(0, p0, q0);
 #pragma unroll
-    for (int k = 0; k < EACH; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum += left_of(weight_of(p[k][j]), off, weight_of(q[k][j]));
-  }
-  float p[4 * EACH], q[4 * EACH];   // the rest, all loads on their way together
-#pragma unroll
-  for (int k = 0; k < 4 * EACH; ++k) {
-    const int v = v0 + (int)threadIdx.x + 1024 * k;
+  for (int k = 0; k < N; ++k) {   // the rest
+    const int v = steps * STEP + (int)threadIdx.x + 1024 * k;
     p[k] = v < a.vocab ? pr[v] : 0.f, q[k] = v < a.vocab ? qr[v] : 0.f;
   }
-#pragma unroll
-  for (int k = 0; k < 4 * EACH; ++k) sum += left_of(weight_of(p[k]), off, weight_of(q[k]));
+  double sum = 0;
+  for (int i = 0; i < steps; i += 2) {
+    if (i + 1 < steps) load(i + 1, p1, q1);
+    add_left(p0, q0, off, sum);
+    if (i + 1 == steps) break;
+    if (i + 2 < steps) load(i + 2, p0, q0);
+    add_left(p1, q1, off, sum);
+  }
+  add_left(p, q, off, sum);
   return block_sum(sum, lds);
 }
 
