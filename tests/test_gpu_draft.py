@@ -532,6 +532,21 @@ def test_verify_unusual_rows(drawn):
     check_verify(tokens, parents, p, u, torch.tensor([-5, 6, 3, 20, 200], dtype=torch.int32), q, max_new=20)
 
 
+@pytest.mark.parametrize("vocab", [8191, 8192, 16385, 25353, 70001])
+@pytest.mark.parametrize("some", [1, 40])
+def test_verify_rows_with_unusual_elements_anywhere(vocab, some):
+    """Rejections behind which another draft is tried: sums over rows with elements that count as 0, in the first and last places too."""
+    tokens, parents, p, u, cu, q = do.drafts([13] * 12, vocab, 3, vocab, True, 0.2)
+    g = torch.Generator().manual_seed(vocab)
+    odd = torch.tensor([math.nan, math.inf, -math.inf, -0.25, -0.0, 2.0 ** -140, -(2.0 ** -149)])
+    for x in (p, q):
+        for row in range(0, x.shape[0], 2):
+            at = torch.randint(vocab, (some,), generator=g)
+            at[0] = (0, vocab - 1, vocab // 2)[row % 3]
+            x[row, at] = odd[torch.randint(len(odd), (some,), generator=g)]
+    check_verify(tokens, parents, p, u, cu, q, max_new=13)
+
+
 def test_verify_same_results_every_time():
     tokens, parents, p, u, cu, q = do.drafts([9] * 40, 30011, 3, 4, True, 0.5)
     call = lambda: cuda_attn.verify_draft(tokens.cuda(), parents.cuda(), p.cuda(), u.cuda(), cu.cuda(), draft_probs=q.cuda(), max_new=9)  # noqa: E731
