@@ -93,9 +93,9 @@ __device__ __forceinline__ float uniform_f(float x) { return __builtin_bit_cast(
 __device__ __forceinline__ SeqRows uniform(SeqRows s) { return {uniform(s.first), uniform(s.count), uniform(s.length)}; }
 
 // The workgroup's number `wg` among the shares and, where it has a share, its walk (false: it has none). All
-// threads of the workgroup take part; `lds` holds 10 numbers. by_xcd: shares that follow each other go to one
-// XCD, whose L2 then serves the tiles of a head together.
-template <int THREADS>
+// threads of the workgroup take part; `lds` holds 10 numbers, 18 with COUNT. by_xcd: shares that follow each other go to one
+// XCD, whose L2 then serves the tiles of a head together. COUNT: a least share may be more than a tile's units.
+template <int THREADS, bool COUNT>
 __device__ __forceinline__ bool start_walk(const PagedCache& c, const AttnWork& w, bool by_xcd, int64_t* lds, int& wg, WorkWalk& walk) {
   const int heads = c.heads * w.tiles.splits, tid = (int)threadIdx.x, lane = tid % kWave;
   const int per = (c.seqs + THREADS - 1) / THREADS, s0 = min(tid * per, c.seqs), s1 = min(s0 + per, c.seqs);
@@ -106,12 +106,19 @@ __device__ __forceinline__ bool start_walk(const PagedCache& c, const AttnWork& 
   int64_t mine = 0;
   for (int s = s0; s < s1; ++s) mine += units(s);
   int64_t upto = mine;
+  int tiles = 0;   // (no more of a thread's, and of all, than the grid has workgroups)
+  if constexpr (COUNT)
+    for (int s = s0; s < s1; ++s) tiles = (int)min(tiles + (int64_t)heads * tiles_of(load_seq(c, s), w.tiles), (int64_t)gridDim.x);
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
     const int64_t other = __shfl_up(upto, d);
     if (lane >= d) upto += other;
+    if constexpr (COUNT) tiles += __shfl_xor(tiles, d);
   }
-  if (lane == kWave - 1) lds[tid / kWave] = upto;
+  if (lane == kWave - 1) {
+    lds[tid / kWave] = upto;
+    if constexpr (COUNT) lds[10 + tid / kWave] = tiles;
+  }
   __syncthreads();
   int64_t total = 0, before = upto - mine;
 #pragma unroll
@@ -120,8 +127,12 @@ __device__ __forceinline__ bool start_walk(const PagedCache& c, const AttnWork& 
     total += lds[i];
   }
   total = uniform(total);
-  const int64_t most = total / w.min_units;
-  const int active = most < 1 ? 1 : most < (int64_t)gridDim.x ? (int)most : (int)gridDim.x;
+  tiles = 0;
+  if constexpr (COUNT) {
+#pragma unroll
+    for (int i = 0; i < THREADS / kWave; ++i) tiles += uniform((int)lds[10 + i]);
+  }
+  const int active = share_count(total, tiles, w.min_units, (int)gridDim.x);
   wg = by_xcd && active == (int)gridDim.x ? xcd_remap((int)blockIdx.x, active) : (int)blockIdx.x;
   if (wg >= active || total == 0) return false;
   const int64_t at = share_of(total, active, wg), end = share_of(total, active, wg + 1);
@@ -279,7 +290,7 @@ paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   PartRecord rec = {0, 0, 0, 0};
   WorkWalk walk;
   int wg;
-  const bool active = start_walk<256>(c, w, false, walk_lds, wg, walk);
+  const bool active = start_walk<256, false>(c, w, false, walk_lds, wg, walk);
   Segment sg;
   unsigned char* vw = v_lds[wave];
   // Swizzled 16-byte chunk of a V row: the 8 rows x 2 chunks that 32 lanes of a transposing read touch lie in
@@ -688,7 +699,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   __shared__ __attribute__((aligned(256))) float ks_lds[SLOTS][kWave], vs_lds[SLOTS][kWave];
   __shared__ float ones_lds[k8 ? BN : 1];
   __shared__ int odd_lds[2][BM / 32];   // of V(t), at t % 2: whether a wave's share has a value that is not finite
-  __shared__ int64_t walk_lds[10];
+  __shared__ int64_t walk_lds[TREE ? 18 : 10];
   const std::integral_constant<int, 0> even{};
   const std::integral_constant<int, 1> odd{};
   auto k_stage = [&](auto par) -> unsigned char* { if constexpr (decltype(par)::value) return k_lds1; else return k_lds0; };
@@ -709,7 +720,7 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
   PartRecord rec = {0, 0, 0, 0};
   WorkWalk walk;
   int wg;
-  const bool active = start_walk<THREADS>(c, w, true, walk_lds, wg, walk);
+  const bool active = start_walk<THREADS, TREE>(c, w, true, walk_lds, wg, walk);
   Segment sg;
   const InTile in_row = in_tile(w.tiles, 32 * wave + lq);
   constexpr int AHEAD = k8 ? 3 : 2;

@@ -128,7 +128,10 @@ inline int tree_rows(const PagedCache& c, int64_t d, bool k8, int64_t most) {
 // tokens 16.8 and 17.5, 24 and 18.
 constexpr int kTreeWholeCapacity = 512;
 // Least units of a workgroup with larger tiles, whose parts cost as much to write and join as that many keys: 4 x 64
-// tokens over 4000, 256 rows, at least 128 units 65 us, 1024 55; 24 x 24 over 2048, 64 dims, 128 rows, 37 and (512) 34.
+// tokens over 4000, 256 rows, at least 128 units 65 us, 1024 55; 24 x 24 over 2048, 64 dims, 128 rows, 37 and (512) 34. It
+// limits how tiles are cut, not how many workgroups take whole ones: tiles of fewer units have one each (share_count). Under a
+// table of 8192 positions, 32 heads over 8, bf16, 32 x 48 tokens over 200 take 28 us so and 58 with the limit alone, over 50
+// to 350 45 and 59, over 500 34 and 57; fp16 over e4m3 37, 61, 47 and 78, 80, 76.
 inline int tree_units(int rows) { return 4 * rows; }
 
 // The launch of an attention call: rows of a tile, workgroups, and whether tiles are cut.
@@ -156,7 +159,8 @@ inline AttnPlan attn_plan(const PagedCache& c, int64_t d, bool k8, int64_t heads
   const double units = tiles * c.heads * t.splits * ((double)kTileCost + c.capacity);
   const int resident = kCUs * (rows > 32 ? chunk_wgs((int)d, k8, rows, tree) : few_wgs((int)d, k8, rows / 16));
   const int least = tree && rows > 32 ? tree_units(rows) : kMinUnits;
-  const int wgs = (int)std::max(1.0, std::min<double>(resident, units / least + 1));
+  const double shares = std::max(units / least, least > kMinUnits ? tiles * c.heads * t.splits : 0);
+  const int wgs = (int)std::max(1.0, std::min<double>(resident, shares + 1));
   return {rows, wgs, least, c.capacity <= (tree && rows <= 32 ? kTreeWholeCapacity : kWholeCapacity)};
 }
 // The kernels count a call's work in 63 bits: each sequence could have all tokens (offsets out of order), each token

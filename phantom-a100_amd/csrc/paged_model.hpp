@@ -108,6 +108,12 @@ __host__ __device__ __forceinline__ int tile_steps(const SeqRows& s, const TileS
   const int keys = keys_seen(s, last, capacity, causal);
   return keys == 0 ? 1 : (keys - 1) / kStep + 1;
 }
+// Workgroups of `grid` that take shares: as many as have min_units units each, but one for each of `tiles` tiles in any case
+// (a share of that size cuts none where they are alike).
+__host__ __device__ __forceinline__ int share_count(int64_t total, int64_t tiles, int min_units, int grid) {
+  const int64_t by_units = total / min_units, most = by_units > tiles ? by_units : tiles;
+  return most < 1 ? 1 : most < grid ? (int)most : grid;
+}
 __host__ __device__ __forceinline__ int64_t share_of(int64_t total, int n, int w) {
   const int64_t each = total / n, rest = total % n;
   return each * w + (w < rest ? w : rest);
