@@ -806,33 +806,26 @@ paged_attn_chunk(PagedCache c, RowsQ a, WorkOf<TREE> w) {
       }
     };
     // 8-bit rows: through registers, or into the thread's 16 bytes of a raw buffer; then widened and stored.
+    // (One load a thread: check_values below takes the rows that a wave stored, before a barrier, as its own side by side.)
+    static_assert(!k8 || CPT == 1, "one load of 8-bit rows a thread");
     auto to_regs = [&](const void* cache, rsrc_t rs, const int (&rows)[CPT], u32x4 (&x)[CPT]) {
-#pragma unroll
-      for (int i = 0; i < CPT; ++i) {
-        if constexpr (WIDE) x[i] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(cache) + (uint64_t)(unsigned)rows[i] * CB + tid % LPR * 16);
-        else x[i] = load16(rs, (unsigned)rows[i] + tid % LPR * 16);
-      }
+      if constexpr (WIDE) x[0] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(cache) + (uint64_t)(unsigned)rows[0] * CB + tid % LPR * 16);
+      else x[0] = load16(rs, (unsigned)rows[0] + tid % LPR * 16);
     };
     auto to_raw = [&](rsrc_t rs, const int (&rows)[CPT], unsigned char* raw) {
-#pragma unroll
-      for (int i = 0; i < CPT; ++i) load16_to_lds(rs, raw + (i * THREADS + wave * kWave) * 16, (unsigned)rows[i] + tid % LPR * 16, 0);
+      load16_to_lds(rs, raw + wave * kWave * 16, (unsigned)rows[0] + tid % LPR * 16, 0);
     };
-    auto from_raw = [&](const unsigned char* raw, u32x4 (&x)[CPT]) {
-#pragma unroll
-      for (int i = 0; i < CPT; ++i) x[i] = *reinterpret_cast<const u32x4*>(raw + (i * THREADS + tid) * 16);
-    };
+    auto from_raw = [&](const unsigned char* raw, u32x4 (&x)[CPT]) { x[0] = *reinterpret_cast<const u32x4*>(raw + tid * 16); };
     auto widen = [&](const u32x4 (&x)[CPT], unsigned char* stage, bool is_v) {
-      if constexpr (k8)
-#pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-          int at = tid;
-          asm("" : "+v"(at));   // (addresses made each time, not held)
-          const int r = i * APART + at / LPR, ch = (at % LPR * 2) ^ (is_v ? v_swz<CR>(r) : k_swz<CR>(r));
-          u32x4 lo16, hi16;
-          widen16<C, T>(x[i], lo16, hi16);
-          *reinterpret_cast<u32x4*>(stage + r * RB + ch * 16) = lo16;
-          *reinterpret_cast<u32x4*>(stage + r * RB + (ch ^ 1) * 16) = hi16;
-        }
+      if constexpr (k8) {
+        int at = tid;
+        asm("" : "+v"(at));   // (addresses made each time, not held)
+        const int r = at / LPR, ch = (at % LPR * 2) ^ (is_v ? v_swz<CR>(r) : k_swz<CR>(r));
+        u32x4 lo16, hi16;
+        widen16<C, T>(x[0], lo16, hi16);
+        *reinterpret_cast<u32x4*>(stage + r * RB + ch * 16) = lo16;
+        *reinterpret_cast<u32x4*>(stage + r * RB + (ch ^ 1) * 16) = hi16;
+      }
     };
     auto present_of = [&](int row) -> uint64_t { return __builtin_amdgcn_ballot_w64(row >= 0) & kWhole; };
     // The row that each of the thread's loads reads; where loads are from a buffer, its byte offset, past the
