@@ -196,6 +196,15 @@ int pa_cache_keep(const pa_paged_cache* cache, const int32_t* path, int64_t path
   const int64_t bytes = cache->d * (pa::is_8bit(cache->dtype) ? 1 : 2), columns = 2 * cache->heads * (bytes / 16);
   const int64_t y = (columns + 255) / 256;
   if (y > 65535) return fail(PA_ERR_UNSUPPORTED, "%s: too many heads for one launch", name);
+  // (the first workgroup of a sequence writes its length while others still read what the call is given)
+  const int64_t seqs = cache->seqs, after = seqs * 4, rows = cache->pages * cache->heads * cache->page_size, scales = c.k_scale ? rows * 4 : 0;
+  const struct { const void* p; int64_t bytes; } taken[] = {
+      {cache->lengths, seqs * 4}, {accepted, seqs * 4}, {cu_seqlens, (seqs + 1) * 4}, {path, pa::span_bytes(seqs, path_stride, path_width, 4)},
+      {cache->page_table, pa::span_bytes(seqs, cache->table_stride, cache->table_cols, 4)}, {cache->k, rows * bytes},
+      {cache->v, rows * bytes}, {c.k_scale, scales}, {c.v_scale, scales}};
+  for (const auto& x : taken)
+    if (pa::share_memory(new_lengths, after, x.p, x.bytes))
+      return fail(PA_ERR_INVALID, "%s: new_lengths must share no memory with what the call reads", name);
   const pa::KeepArgs a{path, accepted, new_lengths, path_stride, (int)path_width};
   const dim3 grid((unsigned)cache->seqs, (unsigned)y);
   const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -62,6 +62,17 @@ inline int check_strides(const char* name, std::initializer_list<int64_t> stride
   return PA_OK;
 }
 
+// Whether two ranges of bytes share memory (a null one does not).
+inline bool share_memory(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && (x < y ? y - x < (uint64_t)a_bytes : x - y < (uint64_t)b_bytes);
+}
+// Bytes from the first to the last of `rows` rows of `cols` elements, `stride` apart (not negative).
+inline int64_t span_bytes(int64_t rows, int64_t stride, int64_t cols, int64_t size) {
+  const int64_t far = rows > 1 && stride > (INT64_MAX >> 8) / rows ? INT64_MAX >> 8 : (rows - 1) * stride;
+  return (far + cols) * size;
+}
+
 // Calls f(T{}, C{}, integral_constant<int, D>{}) for the tensors' type, the cache's and the head dim.
 template <typename T, typename F>
 hipError_t with_cache_type(int cache_dtype, int64_t d, F f) {
