@@ -124,6 +124,10 @@ int pa_draft_tree(const int32_t* parents, const int32_t* lengths, const int32_t*
   if (!cu_seqlens && tokens % seqs != 0)
     return fail(PA_ERR_INVALID, "%s: without cu_seqlens the tokens must divide evenly over the sequences", name);
   const int words = (int)((max_new + 31) / 32);
+  // (a sequence's workgroups write rows while others still read its parents)
+  if (pa::any_shared({{mask, tokens * words * 4}, {positions, tokens * 4}},
+                     {{parents, tokens * 4}, {lengths, seqs * 4}, {cu_seqlens, (seqs + 1) * 4}}))
+    return fail(PA_ERR_INVALID, "%s: results must share no memory with each other or with what the call reads", name);
   const pa::TreeArgs a{parents, lengths, cu_seqlens, (int)tokens, cu_seqlens ? 0 : (int)(tokens / seqs), (int)max_new, words,
                        mask, positions};
   const int64_t y = std::min<int64_t>((max_new * words + 255) / 256, 64);
@@ -153,6 +157,12 @@ int pa_verify_draft(const int64_t* tokens, const int32_t* parents, const float* 
   const bool in_one = verify_in_one(vocab, draft_probs != nullptr);
   if (!in_one && (!workspace || !aligned16(workspace) || workspace_bytes < pa_verify_draft_workspace(seqs, vocab, draft_probs != nullptr)))
     return fail(PA_ERR_INVALID, "%s: the workspace is too small, null or not 16-byte aligned", name);
+  // (one workgroup of a sequence writes its path while others still walk)
+  if (pa::any_shared({{path, seqs * max_new * 4}, {accepted, seqs * 4}, {next_tokens, seqs * 8}, {in_one ? nullptr : workspace, workspace_bytes}},
+                     {{tokens, n_tokens * 8}, {parents, n_tokens * 4}, {uniform, n_tokens * 4}, {cu_seqlens, (seqs + 1) * 4},
+                      {target_probs, pa::span_bytes(n_tokens, target_stride, vocab, 4)},
+                      {draft_probs, pa::span_bytes(n_tokens, draft_stride, vocab, 4)}}))
+    return fail(PA_ERR_INVALID, "%s: results and workspace must share no memory with each other or with what the call reads", name);
   const int runs = (int)verify_runs(vocab);
   pa::VerifyState* states = static_cast<pa::VerifyState*>(workspace);
   const pa::VerifyArgs a{tokens, parents, target_probs, draft_probs, uniform, cu_seqlens, target_stride, draft_stride,
@@ -197,14 +207,13 @@ int pa_cache_keep(const pa_paged_cache* cache, const int32_t* path, int64_t path
   const int64_t y = (columns + 255) / 256;
   if (y > 65535) return fail(PA_ERR_UNSUPPORTED, "%s: too many heads for one launch", name);
   // (the first workgroup of a sequence writes its length while others still read what the call is given)
-  const int64_t seqs = cache->seqs, after = seqs * 4, rows = cache->pages * cache->heads * cache->page_size, scales = c.k_scale ? rows * 4 : 0;
-  const struct { const void* p; int64_t bytes; } taken[] = {
-      {cache->lengths, seqs * 4}, {accepted, seqs * 4}, {cu_seqlens, (seqs + 1) * 4}, {path, pa::span_bytes(seqs, path_stride, path_width, 4)},
-      {cache->page_table, pa::span_bytes(seqs, cache->table_stride, cache->table_cols, 4)}, {cache->k, rows * bytes},
-      {cache->v, rows * bytes}, {c.k_scale, scales}, {c.v_scale, scales}};
-  for (const auto& x : taken)
-    if (pa::share_memory(new_lengths, after, x.p, x.bytes))
-      return fail(PA_ERR_INVALID, "%s: new_lengths must share no memory with what the call reads", name);
+  const int64_t seqs = cache->seqs, rows = cache->pages * cache->heads * cache->page_size, scales = c.k_scale ? rows * 4 : 0;
+  if (pa::any_shared({{new_lengths, seqs * 4}},
+                     {{cache->lengths, seqs * 4}, {accepted, seqs * 4}, {cu_seqlens, (seqs + 1) * 4},
+                      {path, pa::span_bytes(seqs, path_stride, path_width, 4)},
+                      {cache->page_table, pa::span_bytes(seqs, cache->table_stride, cache->table_cols, 4)}, {cache->k, rows * bytes},
+                      {cache->v, rows * bytes}, {c.k_scale, scales}, {c.v_scale, scales}}))
+    return fail(PA_ERR_INVALID, "%s: new_lengths must share no memory with what the call reads", name);
   const pa::KeepArgs a{path, accepted, new_lengths, path_stride, (int)path_width};
   const dim3 grid((unsigned)cache->seqs, (unsigned)y);
   const hipStream_t st = static_cast<hipStream_t>(stream);

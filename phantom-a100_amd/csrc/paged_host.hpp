@@ -67,6 +67,20 @@ inline bool share_memory(const void* a, int64_t a_bytes, const void* b, int64_t 
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return a && b && (x < y ? y - x < (uint64_t)a_bytes : x - y < (uint64_t)b_bytes);
 }
+struct Bytes {
+  const void* p;
+  int64_t n;
+};
+// Whether one of `written` shares memory with one of `read`, or with another of `written`.
+inline bool any_shared(std::initializer_list<Bytes> written, std::initializer_list<Bytes> read) {
+  for (const Bytes& w : written) {
+    for (const Bytes& r : read)
+      if (share_memory(w.p, w.n, r.p, r.n)) return true;
+    for (const Bytes& o : written)
+      if (&o != &w && share_memory(w.p, w.n, o.p, o.n)) return true;
+  }
+  return false;
+}
 // Bytes from the first to the last of `rows` rows of `cols` elements, `stride` apart (not negative).
 inline int64_t span_bytes(int64_t rows, int64_t stride, int64_t cols, int64_t size) {
   const int64_t far = rows > 1 && stride > (INT64_MAX >> 8) / rows ? INT64_MAX >> 8 : (rows - 1) * stride;
