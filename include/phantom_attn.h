@@ -206,8 +206,8 @@ int64_t pa_paged_attn_workspace(const pa_paged_cache* cache, int dtype, int64_t 
  * sequence's new tokens, before i; anything else: none) is the token that token i was drafted behind. The new tokens of all
  * sequences are packed as above, tokens of sequence s being the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1. The first
  * max_new (at most 1024) of a sequence are its tree. All of this is read by the kernels, and whatever it holds, no access
- * leaves the tensors. Results and workspaces share no memory with each other
- * or with anything that a call reads, where nothing else is said. */
+ * leaves the tensors. Results and workspaces share no memory with each other or with anything that a call reads, where nothing
+ * else is said. */
 
 /* mask[i], ceil(max_new / 32) words a token: bit j % 32 of word j / 32 is set for j the token itself or one of its
  * ancestors (tokens behind the tree: none). positions[i]: that of the sequence's first new token, lengths[s] - count, plus

@@ -465,6 +465,8 @@ def check_rope(name: str, q, k, positions, freqs, inplace: bool, *, require_cuda
     if freqs.dim() != 1 or freqs.dtype is not torch.float64 or not freqs.is_contiguous() or not 1 <= freqs.shape[0] <= shape[-1] // 2:
         _fail(f"{name}: freqs must be a contiguous float64 vector of 1 to d / 2 elements")
     if inplace:
+        if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+            _fail(f"{name}: tensors that require a gradient are not turned in place")
         for x in (q, k):
             if x is not None and _rows_overlap(x):
                 _fail(f"{name}: rows that are written must not overlap")

@@ -9,6 +9,7 @@ import math
 import struct
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _call, _checks, _native, _stream_ptr
 
@@ -64,8 +65,9 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs
     freqs (r / 2,) float64, r <= d: pair p of a row's first r elements is turned by the angle position * freqs[p],
     (x, y) -> scale * (x cos - y sin, x sin + y cos); the d - r others pass as they are. Pairs are the elements p and
     p + r / 2, or 2 p and 2 p + 1 (interleaved). inverse: by the negative angle: applied to the gradients of the results,
-    with the same scale, it gives those of q and k. Angles are computed in 64 bits (right at any 32-bit position), the
-    turn in 32."""
+    with the same scale, it gives those of q and k. There is no autograd function: results are cut from its graph, and tensors
+    that require a gradient are refused in place while it records. Angles are computed in 64 bits (right at any 32-bit
+    position), the turn in 32."""
     if inplace or not _checks.rope_ok(q, k, positions, freqs):
         _checks.check_rope("rope", q, k, positions, freqs, inplace)
     shape, device = q.shape, q.device
@@ -78,6 +80,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs
     _call("pa_rope", "rope", device, rows, k_rows, _DTYPE_CODE[q.dtype], b, n, shape[-1], positions.data_ptr(),
           1 if positions.dtype is torch.int64 else 0, pb, pn, freqs.data_ptr(), freqs.shape[0], 1 if interleaved else 0,
           1 if inverse else 0, scale, _stream_ptr(device))
+    if inplace:   # what autograd has saved of them is no longer what it was
+        increment_version(q if k is None else (q, k))
     return q_out, k_out
 
 
