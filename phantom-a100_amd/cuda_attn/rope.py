@@ -36,6 +36,8 @@ def rope_frequencies(dim: int, base: float = 10000.0, *, scaling: str | None = N
         raise RuntimeError("rope_frequencies: scaling must be None, 'linear', 'ntk', 'smooth' or 'parts'")
     if not base > 0 or not factor >= 1.0 or not original >= 1 or scaling in ("smooth", "parts") and not 0 < low < high:
         raise RuntimeError("rope_frequencies: base, factor (from 1 on), original and 0 < low < high must be numbers")
+    if scaling == "parts" and not (base > 1 and all(math.isfinite(x) for x in (base, factor, original, high))):
+        raise RuntimeError("rope_frequencies: 'parts' takes a base above 1 (pairs that turn ever slower) and finite numbers")
     if scaling == "ntk" and dim > 2:
         base = base * factor ** (dim / (dim - 2))
     pair = torch.arange(dim // 2, dtype=torch.float64)
