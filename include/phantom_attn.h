@@ -266,7 +266,7 @@ int64_t pa_verify_draft_workspace(int64_t seqs, int64_t vocab, int drawn);
 /* Leaves of a step's new tokens the accepted ones: row path[s * path_stride + j] of sequence s's new tokens becomes row j,
  * j = 0 .. accepted[s] - 1, keys, values and scales, in place. Paths must ascend (as pa_verify_draft's do); an entry that is
  * no new token leaves its row as it is. new_lengths[s] = lengths[s] - count + accepted[s], at least 0; it shares no memory with
- * lengths or anything else that the call reads. */
+ * lengths or anything else that the call reads (every layer's call takes the same lengths). */
 int pa_cache_keep(const pa_paged_cache* cache, const int32_t* path, int64_t path_width, int64_t path_stride,
                   const int32_t* accepted, const int32_t* cu_seqlens, int32_t* new_lengths, void* stream);
 

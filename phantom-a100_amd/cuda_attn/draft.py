@@ -6,8 +6,9 @@
     # the target's and the draft's probabilities behind each token
     path, accepted, token = cuda_attn.verify_draft(tokens, parents, target_probs, uniform, cu_seqlens,
                                                    draft_probs=draft_probs, max_new=n)
-    # each layer's cache
-    lengths = cuda_attn.cache_keep(k_cache, v_cache, page_table, lengths, path, accepted, cu_seqlens)
+    for k_cache, v_cache in caches:   # each layer's, all from the lengths with the new tokens
+        after = cuda_attn.cache_keep(k_cache, v_cache, page_table, lengths, path, accepted, cu_seqlens)
+    lengths = after
 
 A sequence's new tokens are a tree. Its token 0, the root, is certain: the one that the last step drew. parents (tokens,)
 int32 holds for each other token the one that it was drafted behind, as an index among the sequence's new tokens and
@@ -145,7 +146,8 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
 
     The row of sequence s's new token path[s, j] becomes that of its new token j, for j below accepted[s] (verify_draft's
     results: paths ascend); keys, values and, in 8 bits, their codes and scales as they are. An entry that is no new
-    token of the sequence leaves its row as it is. The new length is lengths - count + accepted."""
+    token of the sequence leaves its row as it is. The new length is lengths - count + accepted. lengths itself stays as it is:
+    every layer's call takes the same, and the result is the next step's."""
     name = "cache_keep"
     _check(name, None, k_cache, v_cache, page_table, lengths, None, k_scale, v_scale)
     seqs, device = lengths.shape[0], k_cache.device
