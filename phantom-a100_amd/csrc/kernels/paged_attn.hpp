@@ -646,17 +646,20 @@ paged_attn_few(PagedCache c, RowsQ a, WorkOf<TREE> w) {
 // ends there. The tiles from it on go one by one, those with such a value leave P . V out, and it is added at the
 // end in fp32 over the visible pairs.
 // 4096 tokens at the end of 32768 keys, 32 heads over 8, D = 128, causal: bf16 1.93 to 2.09 ms, 990 to 1070
-// TFLOP/s (the card's large matrix products reach 1290), fp16 2.03 to 2.07; e4m3 and int8 with bf16 2.24 and 2.33 ms, with
-// fp16, whose units cost three more VALU operations a pair of scores and 9 to 16 registers in memory, 2.51 and 2.58; D = 64
-// 1.28 ms, int8 1.75, with fp16 2.04.
+// TFLOP/s (the card's large matrix products reach 1290), fp16 2.03 to 2.07; e4m3 and int8 with bf16 2.17 and 2.26 ms, with
+// fp16, whose units cost three more VALU operations a pair of scores and 23 to 25 registers in memory, 2.45 and 2.55; D = 64
+// 1.28 ms, int8 1.69, with fp16 1.97. Keys' scales are read a step ahead of their use: read where they are used, with up to 16
+// fewer registers in memory, 8 bits take 2.23, 2.30, 2.52, 2.60, 1.75 and 2.00 (24 x 700 over 4096 1 to 4 % more).
 //
 // TREE, as above: tiles of 128 rows at D = 128 too, for trees that have no more. The keys' bytes then bound it: 32 x 12
-// tokens of 32 heads over 8 and 8192 keys, bf16, 202 us, 5.3 TB/s, x 28 213 to 229; x 64, 256 rows, 327, of which 277 are
-// left where all read one sequence's pages (the matrix core and the VALU, a third of their time each: two waves of a
-// SIMD keep step). In 8 bits two tiles of 64 keys and their raw rows leave no LDS for a second workgroup of 128 rows, and one
+// tokens of 32 heads over 8 and 8192 keys, bf16, 202 us, 5.3 TB/s, x 28 213 to 229; x 64, 256 rows, 327, as long as the
+// same shape takes without a mask, and 277 where all read one sequence's pages: the rate of these two stages, in which the
+// matrix core and the VALU wait for each other (a third of their time busy each). In 8 bits two tiles of 64 keys and their raw rows leave no LDS for a second workgroup of 128 rows, and one
 // wave a SIMD waits for each step of its own: tiles of 32 keys, two workgroups. x 12 in e4m3 266 us, now 206, x 32 269 and
-// 234, x 12 fp16 in int8 306 and 245. The steps behind one another still bound it, of two waves now (206 where all read one
-// sequence's pages 196; the other workgroup's waves with rows on the SIMDs without 203). x 64, 256 rows, 350.
+// 234, x 12 fp16 in int8 306 and 245, in e4m3 238. The steps behind one another still bound it, of two waves now (206 where all read one
+// sequence's pages 196; the other workgroup's waves with rows on the SIMDs without 203). x 64, 256 rows, 358. What the mask costs, by the same shape
+// without one: x 64 over 8192 bf16 332 us and 327, e4m3 363 and 343 (fp16 404 and 374), int8 376 and 360 (397 and 379): 32 to 36
+// more registers in memory with bf16, 21 with fp16; in tiles of 32 rows (x 8) bf16 197 and 195, e4m3 188 and 156.
 //
 // Rows of a tile, D = 128, 256 and 128 (one workgroup of 8 waves on a CU, two of 4): that case 2015 and 2183 us, 4 x
 // 2048 120 and 117, 24 x 700 over 4096 456 and 491, 256 x 64 over 640 73 and 85. D = 64 has 128, and as many

@@ -15,8 +15,11 @@ using pa::aligned16;
 using pa::fail;
 using pa::hip_status;
 
-// (B, heads, N, d) of 4 x 4096 tokens, 64 heads of 128: with 4096 workgroups or more of four tokens 101 us, with 2048 of
-// eight 122, with one token each 111; packed tokens of 40 heads, 32768 of them, one each 120 us, four 129.
+// Where a head's tokens follow each other, (B, heads, N, d), groups of several tokens read longer runs of memory, and 4096
+// workgroups are enough. us with groups of 1, 2, 4 and 8: 4 x 4096 tokens, 64 heads of 128, half turned 116, 106, 104, 108 (of 4
+// on 2048 workgroups 105; all turned 109, 108, 102, on 2048 112); 4 x 8192, 32 heads of 64 71, 57, 54, 51; 8 x 8192, 32 of 128, half
+// turned 248, 241, 222, 209; 16 x 4096, 16 of 64, half turned 89, 64, 54, 49 (of 16, as the rule has it, 51); 2 x 4096, 32 of 128
+// 29, 29, 27. Packed tokens of 40 heads, 32768 of them, one each 120 us, four 129.
 constexpr int64_t kRopeBlocks = 4096;
 template <typename T, int W>
 hipError_t launch_rope(const pa::RopeArgs& a, bool interleaved, hipStream_t stream) {

@@ -113,22 +113,24 @@ inline bool past_buffer(const PagedCache& c, int64_t d, bool k8) {
 // a us and f times the time that reading the keys and values once takes, for each tile that goes over them. (The table's
 // capacity stands for the lengths, which the host does not know.) Measured, us:
 //                                                                 32     128     256 rows
-//   D = 128, 32 heads over 8, bf16   32 x 12 over 8192 (1 GB)    372     202
-//                                    32 x 28                     732     213
-//                                    32 x 48                    1095     411     291
-//                                    24 x 48 over 4096           374     175     128
-//                                    16 x 48 over 1000 (66 MB)    85      39      56
-//                                    16 x 12                      31      32
-//                                     4 x 48 over 500             29      32      48
-//                            e4m3    32 x 12 over 8192           286     206     247
-//                                    32 x 48                     842     370     310
-//                                    16 x 48 over 4000           211     118     103
-//                                    16 x 16 over 1000            42      39      53
-//                                     4 x 24                      31      33      46
-//   D = 64, 16 heads over 4, f16     24 x 16 over 4096            46      40
-//                                    16 x 32 over 1000            26      28
-//                            int8    24 x 24 over 4096            61      50
-//                                    16 x 24 over 1000            26      29
+//   D = 128, 32 heads over 8, bf16   32 x 12 over 8192 (1 GB)    371     205     205
+//                                    32 x 28                     730     214     215
+//                                    32 x 48                    1089     406     272
+//                                    24 x 48 over 4096           373     181     130
+//                                    16 x 48 over 1000 (66 MB)    82      38      59
+//                                    16 x 12                      33      34      45
+//                                     4 x 48 over 500             22      35      30
+//                            e4m3    32 x 12 over 8192           284     209     231
+//                                    32 x 48                     825     388     316
+//                                    16 x 48 over 4000           207     120     105
+//                                    16 x 16 over 1000            44      43      59
+//                                     4 x 24                      34      37      53
+//                 fp16 over e4m3     32 x 12 over 8192           293     238     272
+//                                    16 x 16 over 1000            46      53      65
+//   D = 64, 16 heads over 4, f16     24 x 16 over 4096            48      44
+//                                    16 x 32 over 1000            28      31
+//                            int8    24 x 24 over 4096            67      57
+//                                    16 x 24 over 1000            28      34
 // (Tiles of 64 rows were nowhere more than 2 % faster than the better of these.)
 struct TileTime {
   int rows;

@@ -24,12 +24,12 @@ def rope_frequencies(dim: int, base: float = 10000.0, *, scaling: str | None = N
     base ** (-2 p / dim) for pair p; for contexts `factor` times as long as the `original` ones that a model was trained
     on, by `scaling`:
       None       as they are
-      "linear"   divided by factor: positions interpolated
-      "ntk"      base times factor ** (dim / (dim - 2)): the slowest pair interpolated, the fastest as it is
+      "linear"   divided by factor: positions interpolated (published as position interpolation)
+      "ntk"      base times factor ** (dim / (dim - 2)): the slowest pair interpolated, the fastest as it is (NTK-aware)
       "smooth"   by the turns r = original f / (2 pi) that a pair makes in an original context: divided by factor below
                  `low` turns, as they are above `high`, between them f ((1 - w) / factor + w), w = (r - low) / (high - low)
       "parts"    interpolated linearly in the pair's number instead, between the numbers (rounded outwards) of the pairs that
-                 make `high` and `low` turns, and the result times 0.1 ln(factor) + 1"""
+                 make `high` and `low` turns, and the result times 0.1 ln(factor) + 1 (YaRN)"""
     if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or dim % 2:
         raise RuntimeError("rope_frequencies: dim must be a positive even number")
     if scaling not in (None, "linear", "ntk", "smooth", "parts"):
