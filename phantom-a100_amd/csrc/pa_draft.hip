@@ -158,10 +158,11 @@ int pa_verify_draft(const int64_t* tokens, const int32_t* parents, const float* 
     return fail(PA_ERR_INVALID, "%s: max_new must be a number of tokens from 1 to %d", name, pa::kTreeMax);
   if (target_stride < 0 || draft_stride < 0) return fail(PA_ERR_INVALID, "%s: strides must not be negative", name);
   const bool in_one = verify_in_one(vocab, draft_probs != nullptr);
-  if (!in_one && (!workspace || !aligned16(workspace) || workspace_bytes < pa_verify_draft_workspace(seqs, vocab, draft_probs != nullptr)))
+  const int64_t need = pa_verify_draft_workspace(seqs, vocab, draft_probs != nullptr);
+  if (!in_one && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(PA_ERR_INVALID, "%s: the workspace is too small, null or not 16-byte aligned", name);
   // (one workgroup of a sequence writes its path while others still walk)
-  if (pa::any_shared({{path, seqs * max_new * 4}, {accepted, seqs * 4}, {next_tokens, seqs * 8}, {in_one ? nullptr : workspace, workspace_bytes}},
+  if (pa::any_shared({{path, seqs * max_new * 4}, {accepted, seqs * 4}, {next_tokens, seqs * 8}, {need ? workspace : nullptr, need}},
                      {{tokens, n_tokens * 8}, {parents, n_tokens * 4}, {uniform, n_tokens * 4}, {cu_seqlens, (seqs + 1) * 4},
                       {target_probs, pa::span_bytes(n_tokens, target_stride, vocab, 4)},
                       {draft_probs, pa::span_bytes(n_tokens, draft_stride, vocab, 4)}}))
